@@ -13,6 +13,8 @@ CW_OK, CW_ENOTSUP, CW_EINVAL, CW_EHIP, CW_EFULL = 0, 1, 2, 3, 4
 NO_SLOT = 0xFFFFFFFF
 # include/cwmoe.h: the MoE-layer workspace's sync-state bytes and the offset of its status word
 CW_MOE_STATE_BYTES, CW_MOE_STATUS_OFFSET = 8448, 8320
+# include/cwmoe.h: the most codes in a row of the 8-bit integer path
+CW_I8_MAX_K = 32768
 
 
 class CwError(RuntimeError):
@@ -42,6 +44,13 @@ class MoeDesc(ctypes.Structure):
 class SharedDesc(ctypes.Structure):
     """struct cw_shared_desc (include/cwmoe.h)."""
     _fields_ = [("hidden", _I), ("inter", _I), ("dtype", _I * 3), ("w", _P * 3), ("gate_inp", _P)]
+
+
+class I8MoeDesc(ctypes.Structure):
+    """struct cw_i8_moe_desc (include/cwmoe.h)."""
+    _fields_ = [("n_experts", _I), ("top_k", _I), ("hidden", _I), ("inter", _I), ("norm", _I), ("act", _I),
+                ("alpha", ctypes.c_float), ("limit", ctypes.c_float), ("w", _P * 3), ("slot_stride", _L * 3),
+                ("scale", _P * 3), ("bias", _P * 3)]
 
 
 class BankSource(ctypes.Structure):
@@ -81,6 +90,14 @@ SIGNATURES = {
     "cw_moe_layer_noalloc": ([ctypes.POINTER(MoeDesc), _P, _P, _I, _P, _P, _P, _P, _P], _I),
     "cw_shared_expert_workspace_size": ([ctypes.POINTER(SharedDesc), _I], ctypes.c_size_t),
     "cw_shared_expert": ([ctypes.POINTER(SharedDesc), _P, _I, _P, _I, _P, ctypes.c_size_t, _P], _I),
+    "cw_i8_row_bytes": ([_L], _L),
+    "cw_quantize_i8": ([_I, _P, _L, _L, _L, _P, _P, _P], _I),
+    "cw_swiglu_i8": ([_I, _P, _P, _L, _L, _L, _I, ctypes.c_float, ctypes.c_float, _P, _P, _P], _I),
+    "cw_rmsnorm_i8": ([_I, _P, _L, _P, _L, _P, ctypes.c_float, _L, _L, _P, _P, _P, _P, _P], _I),
+    "cw_dequantize_i8": ([_P, _P, _L, _L, _I, _P, _P], _I),
+    "cw_i8_matmul": ([_P, _P, _L, _L, _P, _P, _L, _P, _I, _P, _L, _P], _I),
+    "cw_i8_moe_workspace_size": ([ctypes.POINTER(I8MoeDesc), _I], ctypes.c_size_t),
+    "cw_i8_moe_layer": ([ctypes.POINTER(I8MoeDesc), _P, _P, _P, _I, _I, _P, _P, _P, _P, ctypes.c_size_t, _P], _I),
     "cw_gguf_open": ([ctypes.c_char_p], _P),
     "cw_gguf_close": ([_P], None),
     "cw_gguf_version": ([_P], _I),

@@ -1,0 +1,101 @@
+// Device code shared by the 8-bit integer kernels.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "cw_wave.h"
+
+namespace cw {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------------------------ 16- and 32-bit floats
+
+struct bf16_t { uint16_t b; };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
+__device__ __forceinline__ float to_f32(bf16_t v) { return __uint_as_float((uint32_t)v.b << 16); }
+// to the nearest, ties to even; a NaN stays one
+template <class T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ _Float16 from_f32<_Float16>(float v) { return (_Float16)v; }
+template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) { return __builtin_bit_cast(bf16_t, (__bf16)v); }
+
+// N values from p, which may be at any address of its type: one wide load (the target takes unaligned ones)
+// where all N are inside the row, else the `valid` first ones, zeros after them
+template <int N, class T>
+__device__ __forceinline__ void load_row(const T *p, int valid, float (&v)[N]) {
+    T t[N];
+    if (valid >= N) {
+        memcpy(t, p, sizeof t);
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = to_f32(t[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = i < valid ? to_f32(p[i]) : 0.f;
+    }
+}
+template <int N, class T>
+__device__ __forceinline__ void store_row(T *p, int valid, const float (&v)[N]) {
+    T t[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) t[i] = from_f32<T>(v[i]);
+    if (valid >= N) {
+        memcpy(p, t, sizeof t);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i < valid) p[i] = t[i];
+    }
+}
+
+// ------------------------------------------------------------------------------ reductions in 64 bits
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = dpp_u<CTRL>((uint32_t)u), hi = dpp_u<CTRL>((uint32_t)(u >> 32));
+    return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+}
+__device__ __forceinline__ double readlane_d(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+}
+__device__ __forceinline__ double wave_sum_d(double v) {
+    v += dpp_d<0xB1>(v);
+    v += dpp_d<0x4E>(v);
+    v += dpp_d<0x141>(v);
+    v += dpp_d<0x140>(v);
+    return (readlane_d(v, 0) + readlane_d(v, 16)) + (readlane_d(v, 32) + readlane_d(v, 48));
+}
+__device__ __forceinline__ double wave_max_d(double v) {
+    v = fmax(v, dpp_d<0xB1>(v));
+    v = fmax(v, dpp_d<0x4E>(v));
+    v = fmax(v, dpp_d<0x141>(v));
+    v = fmax(v, dpp_d<0x140>(v));
+    return fmax(fmax(readlane_d(v, 0), readlane_d(v, 16)), fmax(readlane_d(v, 32), readlane_d(v, 48)));
+}
+
+// ------------------------------------------------------------------------------ codes
+
+// The code of y at inv = 127 / max|y|: y inv rounded to the nearest integer by one fma, whose addend
+// 1.5 * 2^52 leaves it in the low bits of the sum (two's complement).
+__device__ __forceinline__ uint32_t code(double y, double inv) {
+    return (uint32_t)__builtin_bit_cast(uint64_t, fma(y, inv, 6755399441055744.0)) & 0xFFu;
+}
+__device__ __forceinline__ uint32_t codes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return a | b << 8 | c << 16 | d << 24; }
+
+// h = act(g, u): silu(g) u, or the clamped form of gpt-oss (cw_clamped_swiglu, without its biases)
+__device__ __forceinline__ float glu(float g, float u, int act, float alpha, float limit) {
+    if (act == CW_ACT_SILU) return g / (1.0f + expf(-g)) * u;
+    // (comparisons rather than fminf: a NaN stays one)
+    g = g > limit ? limit : g;
+    u = u > limit ? limit : u < -limit ? -limit : u;
+    return (u + 1.0f) * (g * (1.0f / (1.0f + expf(-(g * alpha)))));
+}
+
+}  // namespace cw

@@ -5,6 +5,7 @@ Type ids are GGUF's (vendor/candle-core/src/quantized/mod.rs:314-339), plus 21 (
 type enum does not. Sizes: k_quants.rs:125-200, 631-635, 2959-2968; quantized.metal:217-296.
 """
 F32, F16 = 0, 1
+BF16 = 30  # activations of the 8-bit integer path
 Q8_0 = 8
 Q2_K = 10
 Q3_K = 11

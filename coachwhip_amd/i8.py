@@ -1,0 +1,298 @@
+"""The 8-bit integer path of a MoE block: weights with a scale per output channel, activations with a
+scale per token, products summed exactly in 32-bit integers.
+
+- ``rmsnorm_i8``: the residual's addition and an RMS norm, its rows as codes;
+- ``quantize_i8`` / ``swiglu_i8``: rows of floats, or of a SwiGLU, as codes;
+- ``I8MatMul``: codes times an ``I8Matrix``, beside ``ops.QMatMul``;
+- ``I8MoeLayer``: a layer of 8-bit experts, beside ``ops.MoeLayer``.
+
+``I8Matrix.from_qtensor`` and ``I8ExpertBank.from_bank`` lay GGUF weights out once, when a model is
+loaded. No counterpart in the reference, whose activations are floats. Activations are f32, f16 or
+bf16 tensors, on the current stream of their own device; all arithmetic runs in libcwmoe.so. Shape and type errors raise
+``CwError``.
+"""
+import contextlib
+import ctypes
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import formats as F
+from . import ops
+from ._lib import CW_EINVAL, CW_I8_MAX_K, CwError, I8MoeDesc, check, lib
+
+_DTYPES = {torch.float32: F.F32, torch.float16: F.F16, torch.bfloat16: F.BF16}
+
+
+def row_bytes(k: int) -> int:
+    """Bytes of a row of k codes: whole 128 bytes, zeros past k."""
+    return (k + 127) // 128 * 128
+
+
+def _fail(msg, *a):
+    raise CwError(CW_EINVAL, msg % a)
+
+
+def _same_device(first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            _fail("tensors on %s and %s", first.device, t.device)
+
+
+def _on(t):
+    """The tensor's device as the current one (a launch, and the current stream, belong to a device)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _floats(t, what, cols=None):
+    """A device tensor of rows of floats whose elements are adjacent; the stride between its rows."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _DTYPES:
+        _fail("%s must be an f32, f16 or bf16 device tensor", what)
+    if t.dim() != 2 or (cols is not None and t.shape[1] != cols):
+        _fail("%s must be rows of %s, got %s", what, cols if cols is not None else "values", tuple(t.shape))
+    if t.shape[1] == 0 or (t.shape[1] > 1 and t.stride(1) != 1):
+        _fail("%s: rows of adjacent elements, got strides %s", what, t.stride())
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if ld < t.shape[1]:
+        _fail("%s: rows %d elements apart overlap", what, ld)
+    return ld
+
+
+def _vector(t, n, what):
+    if t is not None:
+        ops._need(t, torch.float32, what)
+        if t.numel() != n:
+            _fail("%s of %d values, expected %d", what, t.numel(), n)
+
+
+def _codes(q, scale, k, lead, what):
+    ops._need(q, torch.int8, "%s codes" % what)
+    ops._need(scale, torch.float32, "%s scales" % what)
+    if q.dim() != lead + 1 or k <= 0 or q.shape[-1] != row_bytes(k):
+        _fail("%s codes %s: rows of %d bytes for %d codes", what, tuple(q.shape), row_bytes(k), k)
+    if tuple(scale.shape) != tuple(q.shape[:-1]):
+        _fail("%s scales %s for codes %s", what, tuple(scale.shape), tuple(q.shape))
+    if q.data_ptr() % 16:
+        _fail("%s codes must be 16-byte aligned", what)
+    _same_device(q, scale)
+
+
+@dataclass
+class I8Rows:
+    """Rows of k codes: ``q`` (rows, row_bytes(k)) int8, zeros past k, and ``scale`` (rows,) f32."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    k: int
+
+    def __post_init__(self):
+        _codes(self.q, self.scale, self.k, 1, "rows")
+
+    def __len__(self):
+        return self.q.shape[0]
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """(rows, k) of code * scale."""
+        if dtype not in _DTYPES:
+            _fail("dequantize to %s", dtype)
+        with _on(self.q):
+            out = torch.empty((len(self), self.k), dtype=dtype, device=self.q.device)
+            check(lib().cw_dequantize_i8(ops._p(self.q), ops._p(self.scale), len(self), self.k, _DTYPES[dtype], ops._p(out), ops._stream()))
+        return out
+
+
+def _new_rows(rows, k, device):
+    if k > CW_I8_MAX_K:
+        _fail("rows of %d codes above %d", k, CW_I8_MAX_K)
+    r = object.__new__(I8Rows)
+    r.q = torch.empty((rows, row_bytes(k)), dtype=torch.int8, device=device)
+    r.scale = torch.empty(rows, dtype=torch.float32, device=device)
+    r.k = k
+    return r
+
+
+def quantize_i8(x: torch.Tensor) -> I8Rows:
+    """Rows (any stride between them) as codes: scale = max|x| / 127, code = x / scale to the nearest."""
+    ld = _floats(x, "x")
+    with _on(x):
+        r = _new_rows(x.shape[0], x.shape[1], x.device)
+        check(lib().cw_quantize_i8(_DTYPES[x.dtype], ops._p(x), ld, x.shape[0], x.shape[1], ops._p(r.q), ops._p(r.scale), ops._stream()))
+    return r
+
+
+def swiglu_i8(g: torch.Tensor, u: torch.Tensor, act: Optional[ops.ExpertAct] = None) -> I8Rows:
+    """silu(g) * u, or the clamped SwiGLU of ``act``, as codes. g and u: rows of one type and stride (the
+    halves of one product's rows). Biases belong to the product (``I8MatMul``): ``act`` must have none."""
+    act = act or ops.ExpertAct.silu()
+    if act.gate_b is not None or act.up_b is not None or act.down_b is not None or act.pad:
+        _fail("swiglu_i8: an activation with biases or padding")
+    ld = _floats(g, "gate")
+    if _floats(u, "up", g.shape[1]) != ld or u.dtype != g.dtype or u.shape != g.shape:
+        _fail("gate %s %s and up %s %s differ in shape, type or stride", tuple(g.shape), g.dtype, tuple(u.shape), u.dtype)
+    _same_device(g, u)
+    with _on(g):
+        r = _new_rows(g.shape[0], g.shape[1], g.device)
+        check(lib().cw_swiglu_i8(_DTYPES[g.dtype], ops._p(g), ops._p(u), ld, g.shape[0], g.shape[1], act.kind, act.alpha, act.limit,
+                                 ops._p(r.q), ops._p(r.scale), ops._stream()))
+    return r
+
+
+def rmsnorm_i8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optional[torch.Tensor] = None, keep_y: bool = False):
+    """(rows as codes, the sum or None, y or None): h = x + residual in x's type (returned as the sum when a
+    residual is given), y = h * weight / sqrt(mean(h^2) + eps) as codes, and as f32 rows with ``keep_y``
+    (``ops.router_logits`` reads them)."""
+    ldx = _floats(x, "x")
+    rows, k = x.shape
+    _vector(weight, k, "weight")
+    ldr = 0
+    if residual is not None:
+        ldr = _floats(residual, "residual", k)
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            _fail("residual %s %s for x %s %s", tuple(residual.shape), residual.dtype, tuple(x.shape), x.dtype)
+    _same_device(x, weight, residual)
+    with _on(x):
+        r = _new_rows(rows, k, x.device)
+        total = None if residual is None else torch.empty((rows, k), dtype=x.dtype, device=x.device)
+        y = torch.empty((rows, k), dtype=torch.float32, device=x.device) if keep_y else None
+        check(lib().cw_rmsnorm_i8(_DTYPES[x.dtype], ops._p(x), ldx, ops._p(residual), ldr, ops._p(weight), eps, rows, k, ops._p(total),
+                                  ops._p(y), ops._p(r.q), ops._p(r.scale), ops._stream()))
+    return r, total, y
+
+
+@dataclass
+class I8Matrix:
+    """An (n, k) weight: ``q`` (n, row_bytes(k)) int8 and ``scale`` (n,) f32, one per output channel."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    k: int
+
+    def __post_init__(self):
+        _codes(self.q, self.scale, self.k, 1, "matrix")
+
+    @property
+    def shape(self):
+        return self.q.shape[0], self.k
+
+    @classmethod
+    def from_float(cls, w: torch.Tensor):
+        r = quantize_i8(w)
+        return cls(r.q, r.scale, r.k)
+
+    @classmethod
+    def from_qtensor(cls, w: ops.QTensor):
+        return cls.from_float(w.dequantize())
+
+
+class I8MatMul:
+    """y = x . W^T (+ bias) for 8-bit rows x and an 8-bit W: each output one exact integer sum, scaled."""
+
+    def __init__(self, matrix: I8Matrix, bias: Optional[torch.Tensor] = None):
+        _vector(bias, matrix.shape[0], "bias")
+        _same_device(matrix.q, bias)
+        self.w, self.bias = matrix, bias
+
+    def forward(self, xs: I8Rows, dtype=torch.float32) -> torch.Tensor:
+        n, k = self.w.shape
+        if xs.k != k:
+            _fail("rows of %d incompatible with (%d, %d)", xs.k, n, k)
+        if dtype not in _DTYPES:
+            _fail("i8 matmul to %s", dtype)
+        _same_device(self.w.q, xs.q)
+        m = len(xs)
+        with _on(xs.q):
+            y = torch.empty((m, n), dtype=dtype, device=xs.q.device)
+            check(lib().cw_i8_matmul(ops._p(self.w.q), ops._p(self.w.scale), n, k, ops._p(xs.q), ops._p(xs.scale), m, ops._p(self.bias),
+                                     _DTYPES[dtype], ops._p(y), n, ops._stream()))
+        return y
+
+    __call__ = forward
+
+
+@dataclass
+class I8ExpertBank:
+    """One matrix of every expert: ``q`` (experts, n, row_bytes(k)) int8, ``scale`` (experts, n) f32."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    k: int
+
+    def __post_init__(self):
+        _codes(self.q, self.scale, self.k, 2, "bank")
+
+    @property
+    def n(self):
+        return self.q.shape[1]
+
+    @classmethod
+    def from_float(cls, w: torch.Tensor):
+        """Of (experts, n, k) floats."""
+        if w.dim() != 3:
+            _fail("bank: (experts, n, k) weights, got %s", tuple(w.shape))
+        e, n, k = w.shape
+        r = quantize_i8(w.reshape(e * n, k))
+        return cls(r.q.view(e, n, -1), r.scale.view(e, n), k)
+
+    @classmethod
+    def from_bank(cls, bank: ops.ExpertBank):
+        """Of a bank of GGUF blocks, one expert's floats at a time."""
+        n, k, e = bank.n, bank.k, bank.n_slots
+        q = torch.empty((e, n, row_bytes(k)), dtype=torch.int8, device=bank.data.device)
+        scale = torch.empty((e, n), dtype=torch.float32, device=bank.data.device)
+        size = F.matrix_bytes(bank.dtype, n, k)
+        for s in range(e):
+            raw = bank.data[s * bank.slot_stride:s * bank.slot_stride + size]
+            r = quantize_i8(ops.dequantize(bank.dtype, raw, n * k).view(n, k))
+            q[s], scale[s] = r.q, r.scale
+        return cls(q, scale, k)
+
+
+class I8MoeLayer:
+    """A MoE layer of 8-bit experts, all resident: ``ops.MoeLayer`` on 8-bit rows."""
+
+    def __init__(self, gate: I8ExpertBank, up: I8ExpertBank, down: I8ExpertBank, top_k: int, norm_topk_prob: bool = True,
+                 act: Optional[ops.ExpertAct] = None):
+        act = act or ops.ExpertAct.silu()
+        e, inter, hidden = gate.q.shape[0], gate.n, gate.k
+        for b, n, k, what in ((up, inter, hidden, "up"), (down, hidden, inter, "down")):
+            if b.q.shape[0] != e or b.n != n or b.k != k:
+                _fail("%s bank of %d (%d, %d) for %d experts (%d, %d)", what, b.q.shape[0], b.n, b.k, e, n, k)
+        if act.pad not in (0, inter):
+            _fail("i8 moe: padding (rows of codes are padded by themselves)")
+        biases = (act.gate_b, act.up_b, act.down_b)
+        for b, n, what in zip(biases, (inter, inter, hidden), ("gate", "up", "down")):
+            _vector(b, e * n, "%s bias" % what)
+        _same_device(gate.q, up.q, down.q, *biases)
+        self.banks, self.act = (gate, up, down), act
+        self.n_experts, self.top_k, self.hidden, self.inter = e, top_k, hidden, inter
+        d = I8MoeDesc()
+        d.n_experts, d.top_k, d.hidden, d.inter, d.norm = e, top_k, hidden, inter, int(norm_topk_prob)
+        d.act, d.alpha, d.limit = act.kind, act.alpha, act.limit
+        for m, b in enumerate(self.banks):
+            d.w[m], d.scale[m], d.slot_stride[m] = b.q.data_ptr(), b.scale.data_ptr(), b.q.stride(0)
+            d.bias[m] = None if biases[m] is None else biases[m].data_ptr()
+        self.desc = d
+
+    def forward(self, xs: I8Rows, logits: torch.Tensor, dtype=torch.float32):
+        """xs T rows of hidden, logits (T, E) f32 -> (out (T, hidden), ids (T, K), w (T, K)). The workspace is
+        allocated for the call (on the stream, or in the graph that captures it)."""
+        ops._need(logits, torch.float32, "logits")
+        t = len(xs)
+        if xs.k != self.hidden or logits.shape != (t, self.n_experts):
+            _fail("rows of %d / logits %s do not fit the layer", xs.k, tuple(logits.shape))
+        if dtype not in _DTYPES:
+            _fail("i8 moe to %s", dtype)
+        device = xs.q.device
+        _same_device(self.banks[0].q, xs.q, logits)
+        d = ctypes.byref(self.desc)
+        with _on(xs.q):
+            need = lib().cw_i8_moe_workspace_size(d, t)
+            if need == 0 and t > 0:
+                raise CwError(CW_EINVAL, lib().cw_last_error().decode(errors="replace"))
+            out = torch.empty((t, self.hidden), dtype=dtype, device=device)
+            ids = torch.empty((t, self.top_k), dtype=torch.int32, device=device)
+            w = torch.empty((t, self.top_k), dtype=torch.float32, device=device)
+            ws = torch.empty(need, dtype=torch.uint8, device=device)
+            check(lib().cw_i8_moe_layer(d, ops._p(xs.q), ops._p(xs.scale), ops._p(logits), t, _DTYPES[dtype], ops._p(out), ops._p(ids),
+                                        ops._p(w), ops._p(ws), need, ops._stream()))
+        return out, ids, w

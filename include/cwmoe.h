@@ -50,6 +50,7 @@ enum cw_status { CW_OK = 0, CW_ENOTSUP = 1, CW_EINVAL = 2, CW_EHIP = 3, CW_EFULL
 enum cw_dtype {
     CW_F32 = 0,
     CW_F16 = 1,
+    CW_BF16 = 30,    /* activations of the 8-bit integer path */
     CW_Q8_0 = 8,     /* {f16 d; i8 qs[32]}: 34 B per 32 weights */
     CW_Q2_K = 10,    /* {u8 scales[16]; u8 qs[64]; f16 d, dmin}: 84 B per 256 (the shrink's output) */
     CW_Q3_K = 11,    /* {u8 hmask[32]; u8 qs[64]; u8 scales[12]; f16 d}: 110 B per 256 (shrink input) */
@@ -289,6 +290,73 @@ typedef struct cw_shared_desc {
 size_t cw_shared_expert_workspace_size(const cw_shared_desc *desc, int T);
 int cw_shared_expert(const cw_shared_desc *desc, const float *x, int T, float *out, int accumulate,
                      void *ws, size_t ws_bytes, cw_stream_t stream);
+
+/* ---- the 8-bit integer path ---------------------------------------------------------------- */
+
+/* A block in 8-bit integers: weights with a scale per output channel, activations with a scale per
+ * row (token), products summed exactly in 32-bit integers. No counterpart in the reference, whose
+ * activations are floats. Rows of codes: row r of k codes (signed bytes) starts at byte
+ * r * cw_i8_row_bytes(k), k rounded up to whole 128 bytes, 16-byte aligned; the bytes past k are
+ * zero (the calls that write codes write them); value = code * scale of the row. Activations and
+ * results are f32, f16 or bf16 (CW_F32, CW_F16, CW_BF16). Rows of at most CW_I8_MAX_K codes:
+ * CW_ENOTSUP above. None of the calls needs memory that was cleared, and none keeps anything for
+ * the next one. */
+#define CW_I8_MAX_K 32768
+int64_t cw_i8_row_bytes(int64_t k);
+
+/* Rows of k values (ldx elements apart, of type dtype, at any address of that type) to codes:
+ * scale = max|x| / 127 rounded to f32, code = x * 127 / max|x| to the nearest integer (computed in
+ * 64 bits; halfway between two codes either may come out). A row of zeros gets the scale 0; a row
+ * with an infinity or a NaN the scale NaN and zero codes, so that what is made of it is NaN.
+ * Weights are laid out by the same call: a row per output channel. */
+int cw_quantize_i8(int dtype, const void *x, int64_t ldx, int64_t rows, int64_t k, int8_t *q, float *scale,
+                   cw_stream_t stream);
+
+/* The same of h = silu(g) * u, or of the clamped SwiGLU of cw_clamped_swiglu (without its biases,
+ * which cw_i8_matmul adds): g and u are rows of width values, ld elements apart (the two halves of
+ * one product's rows, or two matrices). h is computed in f32. */
+int cw_swiglu_i8(int dtype, const void *g, const void *u, int64_t ld, int64_t rows, int64_t width, int act, float alpha,
+                 float limit, int8_t *q, float *scale, cw_stream_t stream);
+
+/* The same of y = h * weight / sqrt(mean(h^2) + eps), h = x + residual rounded to dtype (h = x
+ * without a residual), in 64 bits: the codes do not depend on the order of a sum. sum (rows of k,
+ * may be NULL, and may be x or residual themselves where their rows are k apart) receives h,
+ * y (f32, rows of k, may be NULL) the values before quantizing, which cw_router_logits reads. */
+int cw_rmsnorm_i8(int dtype, const void *x, int64_t ldx, const void *residual, int64_t ldr, const float *weight, float eps,
+                  int64_t rows, int64_t k, void *sum, float *y, int8_t *q, float *scale, cw_stream_t stream);
+
+/* out (rows of k, of type dtype) = code * scale. */
+int cw_dequantize_i8(const int8_t *q, const float *scale, int64_t rows, int64_t k, int dtype, void *out,
+                     cw_stream_t stream);
+
+/* y[r][c] = x_scale[r] * w_scale[c] * sum_k x[r][k] w[c][k] (+ bias[c], f32, may be NULL), rounded
+ * once to ydtype; W is n rows of k codes, x m rows; rows of y are ldy elements apart. */
+int cw_i8_matmul(const int8_t *w, const float *w_scale, int64_t n, int64_t k, const int8_t *x, const float *x_scale,
+                 int64_t m, const float *bias, int ydtype, void *y, int64_t ldy, cw_stream_t stream);
+
+/* One MoE layer's experts in 8-bit integers, every expert resident: gate and up are
+ * [experts][inter] rows of hidden codes, down [experts][hidden] rows of inter codes. */
+typedef struct cw_i8_moe_desc {
+    int n_experts;           /* E <= 1024 */
+    int top_k;               /* K <= 32 */
+    int hidden, inter;
+    int norm;                /* renormalise the K weights */
+    int act;                 /* enum cw_act */
+    float alpha, limit;      /* clamped SwiGLU constants */
+    const int8_t *w[3];      /* gate, up, down */
+    int64_t slot_stride[3];  /* bytes per expert, a multiple of 16 */
+    const float *scale[3];   /* E x inter, E x inter, E x hidden */
+    const float *bias[3];    /* of the same sizes, or NULL (with either activation) */
+} cw_i8_moe_desc;
+
+/* out[T][hidden] = cw_moe_layer's contract on 8-bit rows: route the logits (cw_route_topk), gate
+ * and up of the picked experts, the activation in f32, the hidden row of each pick quantized as
+ * cw_quantize_i8 does, down, the weighted sum in f32, rounded once to ydtype. ids_out / w_out
+ * (T x K, may be NULL) receive the routing. A few tokens run as two launches. ws: 256-byte aligned,
+ * of cw_i8_moe_workspace_size bytes, any contents; calls that overlap in time need distinct ones. */
+size_t cw_i8_moe_workspace_size(const cw_i8_moe_desc *desc, int T);
+int cw_i8_moe_layer(const cw_i8_moe_desc *desc, const int8_t *x, const float *x_scale, const float *logits, int T, int ydtype,
+                    void *out, uint32_t *ids_out, float *w_out, void *ws, size_t ws_bytes, cw_stream_t stream);
 
 /* ---- GGUF files (host) -------------------------------------------------------------------- */
 
