@@ -28,11 +28,14 @@ __global__ __launch_bounds__(256, 2) void k_i8_tile(I8MatArgs a, int tiles_m) {
     extern __shared__ __align__(1024) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t m0 = (int64_t)(blockIdx.x % tiles_m) * 16 * MB, n0 = (int64_t)(blockIdx.x / tiles_m) * 64 * NW + wave * 16 * NW;
-    const uint8_t *wrow[NW];
+    const int64_t nb = min(n0, a.n - 1);
+    uint32_t wrow[NW];
 #pragma unroll
-    for (int j = 0; j < NW; j++) wrow[j] = a.w + min(n0 + 16 * j + (lane & 15), a.n - 1) * a.rb + 16 * (lane >> 4);
+    for (int j = 0; j < NW; j++) wrow[j] = (uint32_t)((min(n0 + 16 * j + (lane & 15), a.n - 1) - nb) * a.rb + 16 * (lane >> 4));
     i32x4 acc[MB][NW];
-    i8_loop<MB, NW, 4>(lds, [&](int r) { return a.x + min(m0 + r, a.m - 1) * a.rb; }, wrow, a.rb / I8_STEP, acc);
+    const uint8_t *w0[1] = {a.w + nb * a.rb};
+    i8_loop<MB, NW, 4, 1>(lds, a.x + m0 * a.rb, [&](int r) { return (uint32_t)((min(m0 + r, a.m - 1) - m0) * a.rb); }, w0, wrow,
+                       a.rb / I8_STEP, acc);
     float sw[NW][4], b[NW][4];
 #pragma unroll
     for (int j = 0; j < NW; j++)
@@ -59,7 +62,7 @@ template <class T>
 static int i8_matmul(const I8MatArgs &a, hipStream_t s) {
     auto go = [&](auto kernel, int mb, int nw) {
         const int64_t tm = (a.m + 16 * mb - 1) / (16 * mb), tn = (a.n + 64 * nw - 1) / (64 * nw);
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(256), 3 * 16 * mb * I8_STEP, s, a, (int)tm);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(256), 2 * 16 * mb * I8_STEP, s, a, (int)tm);
         return check_launch("k_i8_tile");
     };
     if (a.m <= 16) return go(k_i8_tile<T, 1, 1>, 1, 1);

@@ -159,12 +159,15 @@ template <int MB>
 __device__ __forceinline__ void gateup_tile(const I8MoeArgs &a, const MfTile &tl, int n0, uint8_t *lds) {
     constexpr int NB = 2;
     const int lane = threadIdx.x & 63;
-    const uint8_t *wrow[2 * NB];
+    const uint8_t *w0[2];
+    uint32_t wrow[2 * NB];
 #pragma unroll
-    for (int j = 0; j < 2 * NB; j++)
-        wrow[j] = a.w[j / NB] + (int64_t)tl.expert * a.stride[j / NB] + (int64_t)min(n0 + 16 * (j % NB) + (lane & 15), a.I - 1) * a.rbh + 16 * (lane >> 4);
+    for (int j = 0; j < 2; j++) w0[j] = a.w[j] + (int64_t)tl.expert * a.stride[j];
+#pragma unroll
+    for (int j = 0; j < 2 * NB; j++) wrow[j] = min(n0 + 16 * (j % NB) + (lane & 15), a.I - 1) * a.rbh + 16 * (lane >> 4);
     i32x4 acc[MB][2 * NB];
-    i8_loop<MB, 2 * NB, 4>(lds, [&](int r) { return a.x + (int64_t)a.pile_tok[tl.pos0 + min(r, tl.m - 1)] * a.rbh; }, wrow, a.rbh / I8_STEP, acc);
+    i8_loop<MB, 2 * NB, 4, 2>(lds, a.x, [&](int r) { return (uint32_t)a.pile_tok[tl.pos0 + min(r, tl.m - 1)] * (uint32_t)a.rbh; }, w0, wrow,
+                              a.rbh / I8_STEP, acc);
     float sw[2 * NB][4], b[2 * NB][4];
 #pragma unroll
     for (int j = 0; j < 2 * NB; j++)
@@ -198,12 +201,13 @@ template <int MB>
 __device__ __forceinline__ void down_tile(const I8MoeArgs &a, const MfTile &tl, int n0, uint8_t *lds) {
     constexpr int NW = 4;
     const int lane = threadIdx.x & 63;
-    const uint8_t *wrow[NW];
+    const uint8_t *w0[1] = {a.w[2] + (int64_t)tl.expert * a.stride[2]};
+    uint32_t wrow[NW];
 #pragma unroll
-    for (int j = 0; j < NW; j++)
-        wrow[j] = a.w[2] + (int64_t)tl.expert * a.stride[2] + (int64_t)min(n0 + 16 * j + (lane & 15), a.H - 1) * a.rbi + 16 * (lane >> 4);
+    for (int j = 0; j < NW; j++) wrow[j] = min(n0 + 16 * j + (lane & 15), a.H - 1) * a.rbi + 16 * (lane >> 4);
     i32x4 acc[MB][NW];
-    i8_loop<MB, NW, 4>(lds, [&](int r) { return a.hq + (int64_t)(tl.pos0 + min(r, tl.m - 1)) * a.rbi; }, wrow, a.rbi / I8_STEP, acc);
+    i8_loop<MB, NW, 4, 1>(lds, a.hq + (int64_t)tl.pos0 * a.rbi, [&](int r) { return (uint32_t)(min(r, tl.m - 1) * a.rbi); }, w0, wrow,
+                          a.rbi / I8_STEP, acc);
     float sw[NW][4];
 #pragma unroll
     for (int j = 0; j < NW; j++)

@@ -15,83 +15,91 @@ __device__ __forceinline__ i32x4 load16(const uint8_t *p) { return *(const i32x4
 constexpr int I8_STEP = 128;  // codes of k per step: whole cache lines of every row
 
 // A block of WAVES waves, MB blocks of 16 activation rows shared by all of them, NW groups of 16 weight rows for
-// each wave. The activations go through a ring of three LDS stages of 16 MB rows x 128 bytes (direct
-// global-to-LDS loads, two steps ahead, one barrier a step); a wave's weights, which no other wave reads, come
-// straight into its registers one step ahead. Chunk c (16 bytes) of row r lies at chunk c ^ (r & 7) of its LDS
-// row, which the loading lane's global address does: eight rows' reads of one chunk touch all banks once.
+// each wave. The activations go through registers (two steps ahead) into two LDS stages of 16 MB rows x 128 bytes,
+// one barrier a step; a wave's weights, which no other wave reads, come straight into its registers, each half of
+// a step's loaded as soon as that of the step before is used up. Chunk c (16 bytes) of row r lies at chunk
+// c ^ (r & 7) of its LDS row: eight rows' reads of one chunk touch all banks once.
 template <int MB, int WAVES>
 struct I8Stage {
-    static constexpr int ROWS = 16 * MB, BYTES = ROWS * I8_STEP, LDS = 3 * BYTES;
+    static constexpr int ROWS = 16 * MB, BYTES = ROWS * I8_STEP, LDS = 2 * BYTES;
     static constexpr int LOADS = 2 * MB;                        // of 1,024 bytes each, a stage
     static constexpr int PER = (LOADS + WAVES - 1) / WAVES;     // of a wave
 };
 
-// xrow(r): the first byte of activation row r < 16 MB of the tile (any valid row past its end); wrow[j]: that of
-// the lane's weight row of group j, + 16 (lane / 16)
-template <int MB, int NW, int WAVES, class XRow>
-__device__ __forceinline__ void i8_loop(uint8_t *lds, XRow xrow, const uint8_t *const (&wrow)[NW], int steps, i32x4 (&acc)[MB][NW]) {
+// x0 and w0 (NW / MATS groups each): wave-uniform, 4 GiB at most below any row used; xrow(r): the offset from x0 of
+// activation row r < 16 MB of the tile (any valid row past its end); wrow[j]: that from w0 of the lane's weight
+// row of group j, + 16 (lane / 16)
+template <int MB, int NW, int WAVES, int MATS, class XRow>
+__device__ __forceinline__ void i8_loop(uint8_t *lds, const uint8_t *x0, XRow xrow, const uint8_t *const (&w0)[MATS], const uint32_t (&wrow)[NW], int steps,
+                                        i32x4 (&acc)[MB][NW]) {
     using S = I8Stage<MB, WAVES>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint8_t *xp[S::PER];
-    uint32_t to[S::PER];
+    uint32_t xp[S::PER];
 #pragma unroll
     for (int i = 0; i < S::PER; i++) {
-        const int r = 8 * (wave + WAVES * i) + (lane >> 3);
-        xp[i] = xrow(r < S::ROWS ? r : S::ROWS - 1) + 16 * ((lane & 7) ^ (r & 7));
-        to[i] = lds_addr(lds) + 1024 * (wave + WAVES * i);
+        // (with fewer loads than waves some waves copy the same rows: the same bytes to the same place)
+        const int r = 8 * ((wave + WAVES * i) % S::LOADS) + (lane >> 3);
+        xp[i] = xrow(r) + 16 * ((lane & 7) ^ (r & 7));
     }
+    i32x4 xr[S::PER];
     auto fetch_x = [&](int step) __attribute__((always_inline)) {
-        const uint32_t stage = (step % 3) * S::BYTES;
 #pragma unroll
-        for (int i = 0; i < S::PER; i++)
-            if (S::LOADS % WAVES == 0 || wave + WAVES * i < S::LOADS) dma16(xp[i] + (int64_t)step * I8_STEP, __builtin_amdgcn_readfirstlane(to[i] + stage));
+        for (int i = 0; i < S::PER; i++) xr[i] = load16(x0 + (int64_t)step * I8_STEP + xp[i]);
     };
-    i32x4 w[2][NW][2];
-    auto fetch_w = [&](int step, i32x4 (&v)[NW][2]) __attribute__((always_inline)) {
+    auto store_x = [&](int step) __attribute__((always_inline)) {
+        uint8_t *at = lds + (step & 1) * S::BYTES + 16 * lane;
 #pragma unroll
-        for (int j = 0; j < NW; j++) {
-            v[j][0] = load16(wrow[j] + (int64_t)step * I8_STEP);
-            v[j][1] = load16(wrow[j] + (int64_t)step * I8_STEP + 64);
-        }
+        for (int i = 0; i < S::PER; i++) *(i32x4 *)(at + 1024 * ((wave + WAVES * i) % S::LOADS)) = xr[i];
     };
-    auto multiply = [&](int step, const i32x4 (&v)[NW][2]) __attribute__((always_inline)) {
-        const uint8_t *b = lds + (step % 3) * S::BYTES + (lane & 15) * I8_STEP;
+    i32x4 w[2][NW];  // both halves of a step's 128 codes of k
+    auto fetch_w = [&](int step, int kk) __attribute__((always_inline)) {
 #pragma unroll
-        for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-            for (int mb = 0; mb < MB; mb++) {
-                const i32x4 x = *(const i32x4 *)(b + mb * 16 * I8_STEP + 16 * ((4 * kk + (lane >> 4)) ^ (lane & 7)));
-#pragma unroll
-                for (int j = 0; j < NW; j++) acc[mb][j] = mfma_i8(v[j][kk], x, acc[mb][j]);
-            }
+        for (int j = 0; j < NW; j++) w[kk][j] = load16(w0[j / (NW / MATS)] + (int64_t)step * I8_STEP + wrow[j] + 64 * kk);
     };
-    // the stage of `step` is in LDS for every wave, and every wave is done with the stage before it. (Loads return
-    // in order: this wave's older ones, its part of the stage among them, are in when the weights of the step,
-    // which it waits for anyway, are.)
-    auto ready = [&]() __attribute__((always_inline)) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-    };
+    const uint32_t xl = (lane & 15) * I8_STEP;
+    const int c[2] = {16 * ((lane >> 4) ^ (lane & 7)), 16 * ((4 + (lane >> 4)) ^ (lane & 7))};
 #pragma unroll
     for (int mb = 0; mb < MB; mb++)
 #pragma unroll
         for (int j = 0; j < NW; j++) acc[mb][j] = i32x4{0, 0, 0, 0};
+    const int last = steps - 1;  // (loads past it repeat it, unused)
     fetch_x(0);
-    fetch_w(0, w[0]);
-    for (int step = 0; step < steps; step += 2) {
-        ready();
-        if (step + 1 < steps) {
-            fetch_x(step + 1);
-            fetch_w(step + 1, w[1]);
+    store_x(0);
+    // (in the order of the loop, from which the compiler counts how many loads a wait may leave open)
+    fetch_x(min(1, last));
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_w(0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_w(0, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    for (int step = 0; step < steps; step++) {
+        // every wave's part of the stage is in LDS, and every wave has multiplied the stage before it, whose buffer
+        // the next one takes
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        store_x(step + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_x(min(step + 2, last));
+        const uint8_t *b = lds + (step & 1) * S::BYTES + xl;
+        i32x4 x = *(const i32x4 *)(b + c[0]);
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+#pragma unroll
+            for (int mb = 0; mb < MB; mb++) {
+                // the next fragment of x is read while this one is multiplied; the fences keep the compiler from reading
+                // them all at once, and the weights of the next step before this one's are used up: there are no
+                // registers for that
+                const int f = kk * MB + mb + 1;
+                i32x4 xn = x;
+                if (f < 2 * MB) xn = *(const i32x4 *)(b + (f % MB) * 16 * I8_STEP + c[f / MB]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < NW; j++) acc[mb][j] = mfma_i8(w[kk][j], x, acc[mb][j]);
+                __builtin_amdgcn_sched_barrier(0);
+                x = xn;
+            }
+            fetch_w(min(step + 1, last), kk);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        multiply(step, w[0]);
-        if (step + 1 >= steps) break;
-        ready();
-        if (step + 2 < steps) {
-            fetch_x(step + 2);
-            fetch_w(step + 2, w[0]);
-        }
-        multiply(step + 1, w[1]);
     }
 }
 
