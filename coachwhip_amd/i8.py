@@ -11,7 +11,6 @@ loaded. No counterpart in the reference, whose activations are floats. Activatio
 bf16 tensors, on the current stream of their own device; all arithmetic runs in libcwmoe.so. Shape and type errors raise
 ``CwError``.
 """
-import contextlib
 import ctypes
 from dataclasses import dataclass
 from typing import Optional
@@ -23,6 +22,7 @@ from . import ops
 from ._lib import CW_EINVAL, CW_I8_MAX_K, CwError, I8MoeDesc, check, lib
 
 _DTYPES = {torch.float32: F.F32, torch.float16: F.F16, torch.bfloat16: F.BF16}
+_SILU = ops.ExpertAct.silu()
 
 
 def row_bytes(k: int) -> int:
@@ -35,16 +35,15 @@ def _fail(msg, *a):
 
 
 def _same_device(first, *others):
+    d = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            _fail("tensors on %s and %s", first.device, t.device)
+        if t is not None and t.device != d:
+            _fail("tensors on %s and %s", d, t.device)
 
 
-def _on(t):
-    """The tensor's device as the current one (a launch, and the current stream, belong to a device)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _elsewhere(t):
+    """Whether the tensor's device is not the current one, to which a launch would go."""
+    return t.device.index != torch.cuda.current_device()
 
 
 def _stream(t):
@@ -53,16 +52,23 @@ def _stream(t):
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
-def _floats(t, what, cols=None):
-    """A device tensor of rows of floats whose elements are adjacent; the stride between its rows."""
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _floats(t, what):
+    """A device tensor of rows of floats whose elements are adjacent; the elements from a row to the next."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _DTYPES:
         _fail("%s must be an f32, f16 or bf16 device tensor", what)
-    if t.dim() != 2 or (cols is not None and t.shape[1] != cols):
-        _fail("%s must be rows of %s, got %s", what, cols if cols is not None else "values", tuple(t.shape))
-    if t.shape[1] == 0 or (t.shape[1] > 1 and t.stride(1) != 1):
+    shape = t.shape
+    if len(shape) != 2 or shape[1] == 0:
+        _fail("%s must be rows of values, got %s", what, tuple(shape))
+    ld, one = t.stride()
+    if one != 1 and shape[1] > 1:
         _fail("%s: rows of adjacent elements, got strides %s", what, t.stride())
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if ld < t.shape[1]:
+    if shape[0] <= 1:
+        return shape[1]
+    if ld < shape[1]:
         _fail("%s: rows %d elements apart overlap", what, ld)
     return ld
 
@@ -75,15 +81,17 @@ def _vector(t, n, what):
 
 
 def _codes(q, scale, k, lead, what):
-    ops._need(q, torch.int8, "%s codes" % what)
-    ops._need(scale, torch.float32, "%s scales" % what)
-    if q.dim() != lead + 1 or k <= 0 or q.shape[-1] != row_bytes(k):
-        _fail("%s codes %s: rows of %d bytes for %d codes", what, tuple(q.shape), row_bytes(k), k)
-    if tuple(scale.shape) != tuple(q.shape[:-1]):
-        _fail("%s scales %s for codes %s", what, tuple(scale.shape), tuple(q.shape))
+    if not isinstance(q, torch.Tensor) or not isinstance(scale, torch.Tensor) or not q.is_cuda or q.dtype != torch.int8 or scale.dtype != torch.float32:
+        _fail("%s: int8 codes and f32 scales on a device", what)
+    if q.device != scale.device or not q.is_contiguous() or not scale.is_contiguous():
+        _fail("%s: contiguous codes and scales on one device", what)
+    shape = q.shape
+    if len(shape) != lead + 1 or k <= 0 or shape[-1] != row_bytes(k):
+        _fail("%s codes %s: rows of %d bytes for %d codes", what, tuple(shape), row_bytes(k), k)
+    if scale.shape != shape[:-1]:
+        _fail("%s scales %s for codes %s", what, tuple(scale.shape), tuple(shape))
     if q.data_ptr() % 16:
         _fail("%s codes must be 16-byte aligned", what)
-    _same_device(q, scale)
 
 
 @dataclass
@@ -103,45 +111,53 @@ class I8Rows:
         """(rows, k) of code * scale."""
         if dtype not in _DTYPES:
             _fail("dequantize to %s", dtype)
-        with _on(self.q):
-            out = torch.empty((len(self), self.k), dtype=dtype, device=self.q.device)
-            check(lib().cw_dequantize_i8(ops._p(self.q), ops._p(self.scale), len(self), self.k, _DTYPES[dtype], ops._p(out), _stream(self.q)))
+        q = self.q
+        if _elsewhere(q):
+            with torch.cuda.device(q.device):
+                return self.dequantize(dtype)
+        rows = q.shape[0]
+        out = q.new_empty((rows, self.k), dtype=dtype)
+        check(lib().cw_dequantize_i8(q.data_ptr(), self.scale.data_ptr(), rows, self.k, _DTYPES[dtype], out.data_ptr(), _stream(q)))
         return out
 
 
-def _new_rows(rows, k, device):
+def _new_rows(x, rows, k):
     if k > CW_I8_MAX_K:
         _fail("rows of %d codes above %d", k, CW_I8_MAX_K)
     r = object.__new__(I8Rows)
-    r.q = torch.empty((rows, row_bytes(k)), dtype=torch.int8, device=device)
-    r.scale = torch.empty(rows, dtype=torch.float32, device=device)
-    r.k = k
+    r.q, r.scale, r.k = x.new_empty((rows, row_bytes(k)), dtype=torch.int8), x.new_empty(rows, dtype=torch.float32), k
     return r
 
 
 def quantize_i8(x: torch.Tensor) -> I8Rows:
     """Rows (any stride between them) as codes: scale = max|x| / 127, code = x / scale to the nearest."""
     ld = _floats(x, "x")
-    with _on(x):
-        r = _new_rows(x.shape[0], x.shape[1], x.device)
-        check(lib().cw_quantize_i8(_DTYPES[x.dtype], ops._p(x), ld, x.shape[0], x.shape[1], ops._p(r.q), ops._p(r.scale), _stream(x)))
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return quantize_i8(x)
+    rows, k = x.shape
+    r = _new_rows(x, rows, k)
+    check(lib().cw_quantize_i8(_DTYPES[x.dtype], x.data_ptr(), ld, rows, k, r.q.data_ptr(), r.scale.data_ptr(), _stream(x)))
     return r
 
 
 def swiglu_i8(g: torch.Tensor, u: torch.Tensor, act: Optional[ops.ExpertAct] = None) -> I8Rows:
     """silu(g) * u, or the clamped SwiGLU of ``act``, as codes. g and u: rows of one type and stride (the
     halves of one product's rows). Biases belong to the product (``I8MatMul``): ``act`` must have none."""
-    act = act or ops.ExpertAct.silu()
+    act = act or _SILU
     if act.gate_b is not None or act.up_b is not None or act.down_b is not None or act.pad:
         _fail("swiglu_i8: an activation with biases or padding")
     ld = _floats(g, "gate")
-    if _floats(u, "up", g.shape[1]) != ld or u.dtype != g.dtype or u.shape != g.shape:
+    if _floats(u, "up") != ld or u.dtype != g.dtype or u.shape != g.shape:
         _fail("gate %s %s and up %s %s differ in shape, type or stride", tuple(g.shape), g.dtype, tuple(u.shape), u.dtype)
     _same_device(g, u)
-    with _on(g):
-        r = _new_rows(g.shape[0], g.shape[1], g.device)
-        check(lib().cw_swiglu_i8(_DTYPES[g.dtype], ops._p(g), ops._p(u), ld, g.shape[0], g.shape[1], act.kind, act.alpha, act.limit,
-                                 ops._p(r.q), ops._p(r.scale), _stream(g)))
+    if _elsewhere(g):
+        with torch.cuda.device(g.device):
+            return swiglu_i8(g, u, act)
+    rows, k = g.shape
+    r = _new_rows(g, rows, k)
+    check(lib().cw_swiglu_i8(_DTYPES[g.dtype], g.data_ptr(), u.data_ptr(), ld, rows, k, act.kind, act.alpha, act.limit, r.q.data_ptr(),
+                             r.scale.data_ptr(), _stream(g)))
     return r
 
 
@@ -152,18 +168,22 @@ def rmsnorm_i8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Opti
     ldx = _floats(x, "x")
     rows, k = x.shape
     _vector(weight, k, "weight")
-    ldr = 0
+    ldr, total, y = 0, None, None
     if residual is not None:
-        ldr = _floats(residual, "residual", k)
+        ldr = _floats(residual, "residual")
         if residual.shape != x.shape or residual.dtype != x.dtype:
             _fail("residual %s %s for x %s %s", tuple(residual.shape), residual.dtype, tuple(x.shape), x.dtype)
     _same_device(x, weight, residual)
-    with _on(x):
-        r = _new_rows(rows, k, x.device)
-        total = None if residual is None else torch.empty((rows, k), dtype=x.dtype, device=x.device)
-        y = torch.empty((rows, k), dtype=torch.float32, device=x.device) if keep_y else None
-        check(lib().cw_rmsnorm_i8(_DTYPES[x.dtype], ops._p(x), ldx, ops._p(residual), ldr, ops._p(weight), eps, rows, k, ops._p(total),
-                                  ops._p(y), ops._p(r.q), ops._p(r.scale), _stream(x)))
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return rmsnorm_i8(x, weight, eps, residual, keep_y)
+    r = _new_rows(x, rows, k)
+    if residual is not None:
+        total = x.new_empty((rows, k))
+    if keep_y:
+        y = x.new_empty((rows, k), dtype=torch.float32)
+    check(lib().cw_rmsnorm_i8(_DTYPES[x.dtype], x.data_ptr(), ldx, _ptr(residual), ldr, weight.data_ptr(), eps, rows, k, _ptr(total), _ptr(y),
+                              r.q.data_ptr(), r.scale.data_ptr(), _stream(x)))
     return r, total, y
 
 
@@ -200,17 +220,19 @@ class I8MatMul:
         self.w, self.bias = matrix, bias
 
     def forward(self, xs: I8Rows, dtype=torch.float32) -> torch.Tensor:
-        n, k = self.w.shape
-        if xs.k != k:
-            _fail("rows of %d incompatible with (%d, %d)", xs.k, n, k)
+        w, q, k = self.w.q, xs.q, xs.k
+        if k != self.w.k:
+            _fail("rows of %d incompatible with %s", k, self.w.shape)
         if dtype not in _DTYPES:
             _fail("i8 matmul to %s", dtype)
-        _same_device(self.w.q, xs.q)
-        m = len(xs)
-        with _on(xs.q):
-            y = torch.empty((m, n), dtype=dtype, device=xs.q.device)
-            check(lib().cw_i8_matmul(ops._p(self.w.q), ops._p(self.w.scale), n, k, ops._p(xs.q), ops._p(xs.scale), m, ops._p(self.bias),
-                                     _DTYPES[dtype], ops._p(y), n, _stream(y)))
+        _same_device(w, q)
+        if _elsewhere(q):
+            with torch.cuda.device(q.device):
+                return self.forward(xs, dtype)
+        m, n = q.shape[0], w.shape[0]
+        y = q.new_empty((m, n), dtype=dtype)
+        check(lib().cw_i8_matmul(w.data_ptr(), self.w.scale.data_ptr(), n, k, q.data_ptr(), xs.scale.data_ptr(), m, _ptr(self.bias),
+                                 _DTYPES[dtype], y.data_ptr(), n, _stream(q)))
         return y
 
     __call__ = forward
@@ -288,17 +310,19 @@ class I8MoeLayer:
             _fail("rows of %d / logits %s do not fit the layer", xs.k, tuple(logits.shape))
         if dtype not in _DTYPES:
             _fail("i8 moe to %s", dtype)
-        device = xs.q.device
-        _same_device(self.banks[0].q, xs.q, logits)
+        q = xs.q
+        _same_device(self.banks[0].q, q, logits)
+        if _elsewhere(q):
+            with torch.cuda.device(q.device):
+                return self.forward(xs, logits, dtype)
         d = ctypes.byref(self.desc)
-        with _on(xs.q):
-            need = lib().cw_i8_moe_workspace_size(d, t)
-            if need == 0 and t > 0:
-                raise CwError(CW_EINVAL, lib().cw_last_error().decode(errors="replace"))
-            out = torch.empty((t, self.hidden), dtype=dtype, device=device)
-            ids = torch.empty((t, self.top_k), dtype=torch.int32, device=device)
-            w = torch.empty((t, self.top_k), dtype=torch.float32, device=device)
-            ws = torch.empty(need, dtype=torch.uint8, device=device)
-            check(lib().cw_i8_moe_layer(d, ops._p(xs.q), ops._p(xs.scale), ops._p(logits), t, _DTYPES[dtype], ops._p(out), ops._p(ids),
-                                        ops._p(w), ops._p(ws), need, _stream(out)))
+        need = lib().cw_i8_moe_workspace_size(d, t)
+        if need == 0 and t > 0:
+            raise CwError(CW_EINVAL, lib().cw_last_error().decode(errors="replace"))
+        out = q.new_empty((t, self.hidden), dtype=dtype)
+        ids = q.new_empty((t, self.top_k), dtype=torch.int32)
+        w = q.new_empty((t, self.top_k), dtype=torch.float32)
+        ws = q.new_empty(need)
+        check(lib().cw_i8_moe_layer(d, q.data_ptr(), xs.scale.data_ptr(), logits.data_ptr(), t, _DTYPES[dtype], out.data_ptr(), ids.data_ptr(),
+                                    w.data_ptr(), ws.data_ptr(), need, _stream(q)))
         return out, ids, w
