@@ -1,5 +1,6 @@
 // A MoE layer of 8-bit integer experts on 8-bit integer rows (gfx950): two kernels for a few tokens, grouped
 // matrix products for many.
+#include <math.h>
 #include <algorithm>
 
 #include "cw_i8.h"
@@ -43,35 +44,54 @@ __device__ __forceinline__ int wave_sum_i(int v) {
 
 // ------------------------------------------------------------------------------ a few tokens
 
-// Gate and up of one pick of a token: every wave routes the token itself (its logits are one load), then takes
-// R rows of both matrices, lane l the 16 bytes l, l + 64, ... of each row and of x.
+// Gate and up of one pick of a token, eight waves of R rows of both matrices each: lane l takes the 16 bytes l, l + 64,
+// ... of each row and of x. One wave routes the token for its block (every wave for itself: 16,384 times 2,500 cycles
+// for 8 tokens of 8 picks), no further than this pick; the last pick's first block, which goes all the way, stores the
+// routing.
+constexpr int I8_FEW_WAVES = 8;
 template <int PER, int NC, int R>
-__global__ __launch_bounds__(256) void k_i8_few_gateup(I8MoeArgs a) {
+__global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few_gateup(I8MoeArgs a) {
+    __shared__ uint32_t expert;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.z, j = blockIdx.y;
-    const int r0 = (blockIdx.x * 4 + wave) * R;
-    uint32_t id;
-    float wt;
-    wave_route<PER>(a.logits + (int64_t)t * a.E, a.E, a.K, a.norm, &id, &wt);
-    if (blockIdx.x == 0 && j == 0 && wave == 0 && lane < a.K) {
-        a.ids[(int64_t)t * a.K + lane] = id;
-        a.wt[(int64_t)t * a.K + lane] = wt;
+    const int r0 = (blockIdx.x * I8_FEW_WAVES + wave) * R;
+    if (wave == 0) {
+        uint32_t id;
+        float wt;
+        wave_route<PER>(a.logits + (int64_t)t * a.E, a.E, j + 1, a.norm, &id, &wt);
+        if (blockIdx.x == 0 && j == a.K - 1 && lane < a.K) {
+            a.ids[(int64_t)t * a.K + lane] = id;
+            a.wt[(int64_t)t * a.K + lane] = wt;
+        }
+        if (lane == j) expert = id;
     }
-    if (r0 >= a.I) return;
-    const int64_t e = __builtin_amdgcn_readlane((int)id, j);
     i32x4 x[NC], g[R][NC], u[R][NC];
+    int off[NC];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-        const int o = 16 * (lane + 64 * c), off = o < a.rbh ? o : 0;  // past the row: any valid bytes, times zeros
-        x[c] = load16(a.x + (int64_t)t * a.rbh + off);
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            const int64_t row = (int64_t)min(r0 + r, a.I - 1) * a.rbh + off;
-            g[r][c] = load16(a.w[0] + e * a.stride[0] + row);
-            u[r][c] = load16(a.w[1] + e * a.stride[1] + row);
-        }
+        const int o = 16 * (lane + 64 * c);
+        off[c] = o < a.rbh ? o : 0;  // past the row: any valid bytes, times zeros
+        x[c] = load16(a.x + (int64_t)t * a.rbh + off[c]);
         if (o >= a.rbh) x[c] = i32x4{0, 0, 0, 0};
     }
     const float sx = a.xs[t];
+    __syncthreads();
+    if (r0 >= a.I) return;
+    const int64_t e = __builtin_amdgcn_readfirstlane((int)expert);
+    float sw[2][R], b[2][R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int row = min(r0 + r, a.I - 1);
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            g[r][c] = load16(a.w[0] + e * a.stride[0] + (int64_t)row * a.rbh + off[c]);
+            u[r][c] = load16(a.w[1] + e * a.stride[1] + (int64_t)row * a.rbh + off[c]);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            sw[m][r] = a.ws[m][e * a.I + row];
+            b[m][r] = a.bias[m] ? a.bias[m][e * a.I + row] : 0.f;
+        }
+    }
 #pragma unroll
     for (int r = 0; r < R; r++) {
         int sg = 0, su = 0;
@@ -80,79 +100,176 @@ __global__ __launch_bounds__(256) void k_i8_few_gateup(I8MoeArgs a) {
             sg = dot16(g[r][c], x[c], sg);
             su = dot16(u[r][c], x[c], su);
         }
-        sg = wave_sum_i(sg);
-        su = wave_sum_i(su);
-        const int64_t n = e * a.I + min(r0 + r, a.I - 1);
-        const float gv = fmaf((float)sg, sx * a.ws[0][n], a.bias[0] ? a.bias[0][n] : 0.f);
-        const float uv = fmaf((float)su, sx * a.ws[1][n], a.bias[1] ? a.bias[1][n] : 0.f);
+        const float gv = fmaf((float)wave_sum_i(sg), sx * sw[0][r], b[0][r]), uv = fmaf((float)wave_sum_i(su), sx * sw[1][r], b[1][r]);
         if (lane == 0 && r0 + r < a.I) a.h[((int64_t)t * a.K + j) * a.ldh + r0 + r] = glu(gv, uv, a.act, a.alpha, a.limit);
     }
 }
 
 // Down and the weighted sum of a token: the block quantizes the token's K hidden rows into LDS (every block of
-// the token does), then each wave sums one output: lane l holds the 16 bytes l, l + 64, ... of the K rows' codes
-// laid end to end.
-constexpr int FEW_DOWN_WAVES = 8;
-template <class T, int NC>
-__global__ __launch_bounds__(64 * FEW_DOWN_WAVES) void k_i8_few_down(I8MoeArgs a) {
+// the token does, one, two, four or eight waves a row), then each wave sums R outputs: lane l holds the 16 bytes l,
+// l + 64, ... of the K rows' codes laid end to end. The hidden rows are asked for before the weights: loads return in
+// order, and the codes are made while the weights come in.
+template <class T, int NC, int R>
+__global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 ? 4 : 1) void k_i8_few_down(I8MoeArgs a) {
+    constexpr int NH = NC < 12 ? (NC + 1) / 2 : 6;  // pieces of a hidden row held in registers (the others are read twice)
     extern __shared__ __align__(16) uint8_t hq[];  // K rows of rbi codes
-    __shared__ float coef[32];
+    __shared__ float hs[32], coef[I8_FEW_WAVES * R][33];
+    __shared__ double top[I8_FEW_WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.y, cpr = a.rbi / 16;
-    const int row = blockIdx.x * FEW_DOWN_WAVES + wave, rowc = min(row, a.H - 1);
+    const int row0 = (blockIdx.x * I8_FEW_WAVES + wave) * R;
+    const int wpp = a.K > 4 ? 1 : a.K > 2 ? 2 : a.K > 1 ? 4 : 8, at0 = 4 * ((wave & (wpp - 1)) * 64 + lane), stride = 256 * wpp;
+    const float *h = a.h + (int64_t)t * a.K * a.ldh;
+    float hv[NH][4];
+    auto fetch_h = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NH; i++) load_row<4>(h + (int64_t)j * a.ldh + at0 + i * stride, a.I - at0 - i * stride, hv[i]);
+    };
+    fetch_h(min(wave / wpp, a.K - 1));
     const uint32_t *ids = a.ids + (int64_t)t * a.K;
-    i32x4 w[NC];
-    float sd[NC];
-    int pick[NC];
+    const float *wt = a.wt + (int64_t)t * a.K;
+    i32x4 w[R][NC];
+    uint32_t picks[(NC + 3) / 4] = {};  // of each chunk, a byte each
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-        const int i = min(lane + 64 * c, a.K * cpr - 1);
-        pick[c] = i / cpr;
-        const int64_t e = ids[pick[c]];
-        w[c] = load16(a.w[2] + e * a.stride[2] + (int64_t)rowc * a.rbi + 16 * (i - pick[c] * cpr));
-        sd[c] = a.ws[2][e * a.H + rowc];
+        const int i = min(lane + 64 * c, a.K * cpr - 1), pick = i / cpr;
+        picks[c / 4] |= (uint32_t)pick << (8 * (c % 4));
+        const uint8_t *p = a.w[2] + (int64_t)ids[pick] * a.stride[2] + 16 * (i - pick * cpr);
+#pragma unroll
+        for (int r = 0; r < R; r++) w[r][c] = load16(p + (int64_t)min(row0 + r, a.H - 1) * a.rbi);
     }
-    float b = 0.f;
-    if (a.bias[2] && lane < a.K) b = a.wt[(int64_t)t * a.K + lane] * a.bias[2][(int64_t)ids[lane] * a.H + rowc];
-    for (int j = wave; j < a.K; j += FEW_DOWN_WAVES) {
-        const float *h = a.h + ((int64_t)t * a.K + j) * a.ldh;
+    // lane j < K: the scale of the pick's output channel, and what its bias adds
+    float sd[R], b[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int j = min(lane, a.K - 1);
+        const int64_t n = (int64_t)ids[j] * a.H + min(row0 + r, a.H - 1);
+        sd[r] = wt[j] * a.ws[2][n];
+        b[r] = a.bias[2] && lane < a.K ? wt[j] * a.bias[2][n] : 0.f;
+    }
+    for (int j0 = 0; j0 < a.K; j0 += I8_FEW_WAVES / wpp) {
+        const int j = j0 + wave / wpp;
+        const float *row = h + (int64_t)min(j, a.K - 1) * a.ldh;
+        if (j0) fetch_h(min(j, a.K - 1));
         double m = 0.0;
-        for (int c = 4 * lane; c < a.I; c += 256) {
-            float v[4];
-            load_row<4>(h + c, a.I - c, v);
+        auto more = [&](const float (&v)[4]) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const double y = fabs((double)v[i]);
                 m = y <= m ? m : y < INFINITY ? y : INFINITY;
             }
+        };
+#pragma unroll
+        for (int i = 0; i < NH; i++) more(hv[i]);
+        for (int c = at0 + NH * stride; c < a.I; c += stride) {
+            float v[4];
+            load_row<4>(row + c, a.I - c, v);
+            more(v);
         }
         m = wave_max_d(m);
+        if (wpp > 1) {
+            if (lane == 0) top[wave] = m;
+            __syncthreads();
+            for (int o = 1; o < wpp; o++) m = fmax(m, top[wave ^ o]);
+            if (j0 + I8_FEW_WAVES / wpp < a.K) __syncthreads();
+        }
+        if (j >= a.K) continue;
         const bool some = m > 0.0 && m < INFINITY;
         const double inv = some ? 127.0 / m : 0.0;
-        for (int c = 4 * lane; c < a.rbi; c += 256) {
-            float v[4];
-            load_row<4>(h + c, a.I - c, v);
+        auto store = [&](int c, const float (&v)[4]) __attribute__((always_inline)) {
             *(uint32_t *)(hq + j * a.rbi + c) = some ? codes4(code(v[0], inv), code(v[1], inv), code(v[2], inv), code(v[3], inv)) : 0u;
+        };
+#pragma unroll
+        for (int i = 0; i < NH; i++)
+            if (at0 + i * stride < a.rbi) store(at0 + i * stride, hv[i]);
+        for (int c = at0 + NH * stride; c < a.rbi; c += stride) {
+            float v[4];
+            load_row<4>(row + c, a.I - c, v);
+            store(c, v);
         }
-        if (lane == 0) coef[j] = a.wt[(int64_t)t * a.K + j] * (m < INFINITY ? (float)(m / 127.0) : __int_as_float(0x7fc00000));
+        if (lane == 0 && (wave & (wpp - 1)) == 0) hs[j] = m < INFINITY ? (float)(m / 127.0) : __int_as_float(0x7fc00000);
     }
     __syncthreads();
-    if (row >= a.H) return;
-    float acc = b;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+        if (lane < a.K) coef[wave * R + r][lane] = sd[r] * hs[lane];  // (read by this wave alone)
+    if (row0 >= a.H) return;
+    float acc[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) acc[r] = b[r];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
         const int i = lane + 64 * c;
         if (i < a.K * cpr) {
-            const int d = dot16(w[c], *(const i32x4 *)(hq + 16 * i), 0);
-            acc = fmaf((float)d, coef[pick[c]] * sd[c], acc);
+            const i32x4 x = *(const i32x4 *)(hq + 16 * i);
+#pragma unroll
+            for (int r = 0; r < R; r++) acc[r] = fmaf((float)dot16(w[r][c], x, 0), coef[wave * R + r][(picks[c / 4] >> (8 * (c % 4))) & 0xFF], acc[r]);
         }
     }
-    acc = wave_sum(acc);
-    if (lane == 0) ((T *)a.out)[(int64_t)t * a.H + row] = from_f32<T>(acc);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const float v = wave_sum(acc[r]);
+        if (lane == 0 && row0 + r < a.H) ((T *)a.out)[(int64_t)t * a.H + row0 + r] = from_f32<T>(v);
+    }
 }
 
 // ------------------------------------------------------------------------------ many tokens
 
 constexpr int I8_TILE = 128;  // picks of a tile
+
+// The routing of up to I8_PLAN_TOKENS tokens and their piles in one launch of one block: each wave routes every 16th
+// token, then the picks are counted by expert in LDS, the experts' places and tiles come from a scan, and the picks
+// are dealt out (their order within a pile does not matter: each pick's outputs are computed by themselves). Against
+// the router's and the piles' own launches, whose routing runs on as many CUs as there are tokens: 9 tokens over 256
+// experts 9.8 -> 7 us.
+constexpr int I8_PLAN_TOKENS = 64;
+template <int PER>
+__global__ __launch_bounds__(1024) void k_i8_plan(I8MoeArgs a, int *pile_pick, int *pile_tok, MfTile *tiles, int *n_tiles) {
+    __shared__ int cnt[1024], place[1024], sums[2][16];
+    __shared__ uint16_t expert[I8_PLAN_TOKENS * 32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, picks = a.T * a.K;
+    cnt[tid] = 0;
+    for (int t = wave; t < a.T; t += 16) {
+        uint32_t id;
+        float w;
+        wave_route<PER>(a.logits + (int64_t)t * a.E, a.E, a.K, a.norm, &id, &w);
+        if (lane < a.K) {
+            a.ids[t * a.K + lane] = id;
+            a.wt[t * a.K + lane] = w;
+            expert[t * a.K + lane] = (uint16_t)id;
+        }
+    }
+    __syncthreads();
+    for (int p = tid; p < picks; p += 1024) atomicAdd(&cnt[expert[p]], 1);
+    __syncthreads();
+    const int c = cnt[tid], tc = (c + I8_TILE - 1) / I8_TILE;
+    int ic = c, it = tc;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int uc = __shfl_up(ic, d), ut = __shfl_up(it, d);
+        if (lane >= d) {
+            ic += uc;
+            it += ut;
+        }
+    }
+    if (lane == 63) {
+        sums[0][wave] = ic;
+        sums[1][wave] = it;
+    }
+    __syncthreads();
+    for (int w = 0; w < wave; w++) {
+        ic += sums[0][w];
+        it += sums[1][w];
+    }
+    place[tid] = ic - c;
+    for (int q = 0; q < tc; q++) tiles[it - tc + q] = MfTile{tid, ic - c + q * I8_TILE, min(I8_TILE, c - q * I8_TILE), tid};
+    if (tid == 1023) *n_tiles = it;
+    __syncthreads();
+    for (int p = tid; p < picks; p += 1024) {
+        const int at = atomicAdd(&place[expert[p]], 1);
+        pile_pick[at] = p;
+        pile_tok[at] = p / a.K;
+    }
+}
 
 // Gate and up of a tile: a wave holds 16 rows of each. Hidden rows in pile order, f32.
 template <int MB>
@@ -295,8 +412,17 @@ struct I8MoeLayout {
     bool few;
 };
 
+// Two launches read an expert once per pick, the grouped ones once per tile: about 15 us more for their launches, but
+// each byte once. The picks' reads beyond the distinct experts', E (1 - (1 - K / E)^T) on average, come in part from the
+// caches. Measured, two launches / grouped, and those bytes: 256 experts of 512 x 2,048, top-8, 16 tokens 69 / 96 us
+// (85 MB), 32 tokens 120 / 135 (299); 128 of 2,880 x 2,880, top-4, 6 tokens 124 / 133 (53), 8 tokens 157 / 165 (91),
+// 16 tokens 291 / 249 (330); 8 of 2,048 x 4,096, top-2, 6 tokens 47 / 49 (137), 8 tokens 55 / 51 (222); 512 of 512 x
+// 2,048, top-10, 32 tokens 182 / 182 (250).
 static bool few_path(const cw_i8_moe_desc *d, int T) {
-    return T <= 8 && i8_row_bytes(d->hidden) <= 4 * 1024 && d->top_k * i8_row_bytes(d->inter) <= 16 * 1024;
+    const int64_t rbh = i8_row_bytes(d->hidden), rbi = i8_row_bytes(d->inter);
+    if (rbh > 4 * 1024 || d->top_k * rbi > 16 * 1024 || T > 1024) return false;
+    const double K = d->top_k, E = d->n_experts, picks = T * K, distinct = E * (1 - pow(1 - K / E, T));
+    return (picks - distinct) * (2.0 * d->inter * rbh + (double)d->hidden * rbi) <= 200e6;
 }
 
 static I8MoeLayout layout(const cw_i8_moe_desc *d, int T) {
@@ -341,28 +467,49 @@ static int check_desc(const cw_i8_moe_desc *d, int T) {
     return CW_OK;
 }
 
+// Rows a wave: more where that still leaves every CU four blocks (the routing and the rows' codes are made once a
+// block).
+template <class T, int NC>
+static int few_down(const I8MoeArgs &a, hipStream_t s) {
+    constexpr int MORE = NC <= 4 ? 4 : NC <= 8 ? 2 : 1;
+    const int64_t rows = (a.H + I8_FEW_WAVES - 1) / I8_FEW_WAVES, cus = resident_blocks(1);
+    auto go = [&](auto kernel, int r) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + r - 1) / r), a.T), dim3(64 * I8_FEW_WAVES), a.K * a.rbi, s, a);
+        return check_launch("k_i8_few_down");
+    };
+    if (MORE == 4 && rows * a.T >= 16 * cus) return go(k_i8_few_down<T, NC, MORE>, MORE);
+    if (MORE >= 2 && rows * a.T >= 8 * cus) return go(k_i8_few_down<T, NC, MORE < 2 ? 1 : 2>, 2);
+    return go(k_i8_few_down<T, NC, 1>, 1);
+}
 template <class T>
 static int few_down(const I8MoeArgs &a, hipStream_t s) {
     const int chunks = a.K * (a.rbi / 16);
-    const dim3 grid((a.H + FEW_DOWN_WAVES - 1) / FEW_DOWN_WAVES, a.T);
-#define CW_DOWN(N) \
-    if (chunks <= 64 * N) { \
-        hipLaunchKernelGGL((k_i8_few_down<T, N>), grid, dim3(64 * FEW_DOWN_WAVES), a.K * a.rbi, s, a); \
-        return check_launch("k_i8_few_down"); \
-    }
-    CW_DOWN(2) CW_DOWN(4) CW_DOWN(8) CW_DOWN(12) CW_DOWN(16)
-#undef CW_DOWN
+    if (chunks <= 64 * 1) return few_down<T, 1>(a, s);
+    if (chunks <= 64 * 2) return few_down<T, 2>(a, s);
+    if (chunks <= 64 * 4) return few_down<T, 4>(a, s);
+    if (chunks <= 64 * 8) return few_down<T, 8>(a, s);
+    if (chunks <= 64 * 12) return few_down<T, 12>(a, s);
+    if (chunks <= 64 * 16) return few_down<T, 16>(a, s);
     return set_error(CW_ENOTSUP, "i8 moe: %d picks' rows of %d", a.K, a.I);
+}
+template <int PER, int NC>
+static int few_gateup(const I8MoeArgs &a, hipStream_t s) {
+    constexpr int MORE = NC <= 2 ? 4 : 2;
+    const int64_t rows = (a.I + I8_FEW_WAVES - 1) / I8_FEW_WAVES, cus = resident_blocks(1);
+    auto go = [&](auto kernel, int r) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + r - 1) / r), a.K, a.T), dim3(64 * I8_FEW_WAVES), 0, s, a);
+        return check_launch("k_i8_few_gateup");
+    };
+    if (MORE == 4 && rows * a.T * a.K >= 16 * cus) return go(k_i8_few_gateup<PER, NC, MORE>, MORE);
+    if (rows * a.T * a.K >= 2 * cus) return go(k_i8_few_gateup<PER, NC, 2>, 2);
+    return go(k_i8_few_gateup<PER, NC, 1>, 1);
 }
 template <int PER>
 static int few_gateup(const I8MoeArgs &a, hipStream_t s) {
-#define CW_GU(N, R) \
-    if (a.rbh <= 1024 * N) { \
-        hipLaunchKernelGGL((k_i8_few_gateup<PER, N, R>), dim3((a.I + 4 * R - 1) / (4 * R), a.K, a.T), dim3(256), 0, s, a); \
-        return check_launch("k_i8_few_gateup"); \
-    }
-    CW_GU(1, 4) CW_GU(2, 2) CW_GU(3, 2) CW_GU(4, 2)
-#undef CW_GU
+    if (a.rbh <= 1024) return few_gateup<PER, 1>(a, s);
+    if (a.rbh <= 2048) return few_gateup<PER, 2>(a, s);
+    if (a.rbh <= 1024 * 3) return few_gateup<PER, 3>(a, s);
+    if (a.rbh <= 4096) return few_gateup<PER, 4>(a, s);
     return set_error(CW_ENOTSUP, "i8 moe: rows of %d", a.H);
 }
 
@@ -374,10 +521,17 @@ static int moe_layer(const cw_i8_moe_desc *d, I8MoeArgs a, int ydtype, const I8M
         return ydtype == CW_F16 ? few_down<_Float16>(a, s) : ydtype == CW_BF16 ? few_down<bf16_t>(a, s) : few_down<float>(a, s);
     }
     const int TK = a.T * a.K, tmax = max_tiles(TK, a.E, I8_TILE);
-    if ((rc = cw_route_topk(a.logits, a.T, a.E, a.K, a.norm, a.ids, a.wt, s))) return rc;
     int *pile_pick = (int *)(base + L.pile_pick), *pile_tok = (int *)(base + L.pile_tok), *n_tiles = (int *)(base + L.n_tiles);
     MfTile *tiles = (MfTile *)(base + L.tiles);
-    if ((rc = mfma_piles(a.ids, nullptr, TK, a.K, a.E, 0, pile_pick, pile_tok, tiles, n_tiles, s, I8_TILE))) return rc;
+    if (a.T <= I8_PLAN_TOKENS) {
+        if (a.E <= 256) hipLaunchKernelGGL(k_i8_plan<4>, dim3(1), dim3(1024), 0, s, a, pile_pick, pile_tok, tiles, n_tiles);
+        else if (a.E <= 512) hipLaunchKernelGGL(k_i8_plan<8>, dim3(1), dim3(1024), 0, s, a, pile_pick, pile_tok, tiles, n_tiles);
+        else hipLaunchKernelGGL(k_i8_plan<16>, dim3(1), dim3(1024), 0, s, a, pile_pick, pile_tok, tiles, n_tiles);
+        if ((rc = check_launch("k_i8_plan"))) return rc;
+    } else {
+        if ((rc = cw_route_topk(a.logits, a.T, a.E, a.K, a.norm, a.ids, a.wt, s))) return rc;
+        if ((rc = mfma_piles(a.ids, nullptr, TK, a.K, a.E, 0, pile_pick, pile_tok, tiles, n_tiles, s, I8_TILE))) return rc;
+    }
     int8_t *hq = (int8_t *)(base + L.hq);
     float *hs = (float *)(base + L.hs);
     a.tiles = tiles;
