@@ -9,6 +9,12 @@
 
 namespace cw {
 
+// A tile: m picks of one expert from pile position pos0; the expert has `of` tiles, the first of them tile `first`.
+struct I8Tile {
+    int expert, pos0, m, first, of;
+};
+constexpr int I8_TILE = 128;  // picks of a tile, at most
+
 struct I8MoeArgs {
     const uint8_t *w[3];
     int64_t stride[3];
@@ -22,7 +28,7 @@ struct I8MoeArgs {
     float *wt, *h;
     void *out;
     // many tokens
-    const MfTile *tiles;
+    const I8Tile *tiles;
     const int *n_tiles, *pile_pick, *pile_tok;
     const uint8_t *hq;
     const float *hs;
@@ -214,32 +220,47 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 ? 4 : 1) void k_i8_few_d
 
 // ------------------------------------------------------------------------------ many tokens
 
-constexpr int I8_TILE = 128;  // picks of a tile
 
-// The routing of up to I8_PLAN_TOKENS tokens and their piles in one launch of one block: each wave routes every 16th
-// token, then the picks are counted by expert in LDS, the experts' places and tiles come from a scan, and the picks
-// are dealt out (their order within a pile does not matter: each pick's outputs are computed by themselves). Against
-// the router's and the piles' own launches, whose routing runs on as many CUs as there are tokens: 9 tokens over 256
-// experts 9.8 -> 7 us.
-constexpr int I8_PLAN_TOKENS = 64;
-template <int PER>
-__global__ __launch_bounds__(1024) void k_i8_plan(I8MoeArgs a, int *pile_pick, int *pile_tok, MfTile *tiles, int *n_tiles) {
-    __shared__ int cnt[1024], place[1024], sums[2][16];
-    __shared__ uint16_t expert[I8_PLAN_TOKENS * 32];
+// One block: the picks counted by expert in LDS, the experts' places and tiles from a scan, and the picks dealt out
+// (their order within a pile does not matter: each pick's outputs are computed by themselves), through LDS up to
+// I8_STAGED picks (scattered 4-byte stores from one CU cost a memory transaction each). ROUTE: of up to I8_PLAN_TOKENS
+// tokens, which its waves route first, every 16th token each: one launch less (9 tokens over 256 experts 9.8 -> 7 us; with
+// more tokens the routing of a CU to each is faster).
+constexpr int I8_PLAN_TOKENS = 64, I8_STAGED = 12288;
+template <bool ROUTE, int PER>
+__global__ __launch_bounds__(1024) void k_i8_plan(I8MoeArgs a, int *pile_pick, int *pile_tok, I8Tile *tiles, int *n_tiles) {
+    __shared__ int cnt[1024], place[1024], sums[2][16], staged[I8_STAGED];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, picks = a.T * a.K;
     cnt[tid] = 0;
-    for (int t = wave; t < a.T; t += 16) {
-        uint32_t id;
-        float w;
-        wave_route<PER>(a.logits + (int64_t)t * a.E, a.E, a.K, a.norm, &id, &w);
-        if (lane < a.K) {
-            a.ids[t * a.K + lane] = id;
-            a.wt[t * a.K + lane] = w;
-            expert[t * a.K + lane] = (uint16_t)id;
+    if constexpr (ROUTE) {
+        int *expert = staged;  // (staged[] is filled after the last read of these)
+        for (int t = wave; t < a.T; t += 16) {
+            uint32_t id;
+            float w;
+            wave_route<PER>(a.logits + (int64_t)t * a.E, a.E, a.K, a.norm, &id, &w);
+            if (lane < a.K) {
+                a.ids[t * a.K + lane] = id;
+                a.wt[t * a.K + lane] = w;
+                expert[t * a.K + lane] = (int)id;
+            }
         }
     }
     __syncthreads();
-    for (int p = tid; p < picks; p += 1024) atomicAdd(&cnt[expert[p]], 1);
+    constexpr int U = ROUTE ? 2 : 8;  // a thread's picks at a time (ROUTE: all of them)
+    int e[U];
+    auto load = [&](int p0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int p = min(p0 + 1024 * u + tid, picks - 1);
+            e[u] = ROUTE ? staged[p] : (int)a.ids[p];
+        }
+    };
+    for (int p0 = 0; p0 < picks; p0 += 1024 * U) {
+        load(p0);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (p0 + 1024 * u + tid < picks) atomicAdd(&cnt[e[u]], 1);
+    }
     __syncthreads();
     const int c = cnt[tid], tc = (c + I8_TILE - 1) / I8_TILE;
     int ic = c, it = tc;
@@ -261,31 +282,41 @@ __global__ __launch_bounds__(1024) void k_i8_plan(I8MoeArgs a, int *pile_pick, i
         it += sums[1][w];
     }
     place[tid] = ic - c;
-    for (int q = 0; q < tc; q++) tiles[it - tc + q] = MfTile{tid, ic - c + q * I8_TILE, min(I8_TILE, c - q * I8_TILE), tid};
+    // (an expert's picks spread over its tiles evenly, in whole 16s)
+    const int rows = tc ? ((c + tc - 1) / tc + 15) / 16 * 16 : 0;
+    for (int q = 0; q < tc; q++) tiles[it - tc + q] = I8Tile{tid, ic - c + q * rows, min(rows, c - q * rows), it - tc, tc};
     if (tid == 1023) *n_tiles = it;
     __syncthreads();
-    for (int p = tid; p < picks; p += 1024) {
-        const int at = atomicAdd(&place[expert[p]], 1);
+    for (int p0 = 0; p0 < picks; p0 += 1024 * U) {
+        if (!ROUTE && picks > 1024 * U) load(p0);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int p = p0 + 1024 * u + tid;
+            if (p >= picks) continue;
+            const int at = atomicAdd(&place[e[u]], 1);
+            if (picks <= I8_STAGED) {
+                staged[at] = p;
+            } else {
+                pile_pick[at] = p;
+                pile_tok[at] = p / a.K;
+            }
+        }
+    }
+    if (picks > I8_STAGED) return;
+    __syncthreads();
+    for (int at = tid; at < picks; at += 1024) {
+        const int p = staged[at];
         pile_pick[at] = p;
         pile_tok[at] = p / a.K;
     }
 }
-
-// Gate and up of a tile: a wave holds 16 rows of each. Hidden rows in pile order, f32.
-template <int MB>
-__device__ __forceinline__ void gateup_tile(const I8MoeArgs &a, const MfTile &tl, int n0, uint8_t *lds) {
-    constexpr int NB = 1;
+// A wave's sums of gate (acc[i][j], j < NB) and up (acc[i][NB + j]): rows r0 + 16 i of the tile's picks, columns n0 + 16 j
+// of the hidden row, which is stored in pile order, f32. (All loads before the bounds checks, from clamped places: inside
+// them each would be waited for in turn.)
+template <int MB, int NB>
+__device__ __forceinline__ void finish_gateup(const I8MoeArgs &a, const I8Tile &tl, int r0, int n0, const i32x4 (&acc)[MB][2 * NB]) {
     const int lane = threadIdx.x & 63;
-    const uint8_t *w0[2];
-    uint32_t wrow[2 * NB];
-#pragma unroll
-    for (int j = 0; j < 2; j++) w0[j] = a.w[j] + (int64_t)tl.expert * a.stride[j];
-#pragma unroll
-    for (int j = 0; j < 2 * NB; j++) wrow[j] = min(n0 + 16 * (j % NB) + (lane & 15), a.I - 1) * a.rbh + 16 * (lane >> 4);
-    i32x4 acc[MB][2 * NB];
-    i8_loop<MB, 2 * NB, 2>(lds, a.x, [&](int r) { return (uint32_t)a.pile_tok[tl.pos0 + min(r, tl.m - 1)] * (uint32_t)a.rbh; }, w0, wrow,
-                              a.rbh, acc);
-    float sw[2 * NB][4], b[2 * NB][4];
+    float sw[2 * NB][4], b[2 * NB][4], sx[MB];
 #pragma unroll
     for (int j = 0; j < 2 * NB; j++)
 #pragma unroll
@@ -294,16 +325,12 @@ __device__ __forceinline__ void gateup_tile(const I8MoeArgs &a, const MfTile &tl
             sw[j][i] = a.ws[j / NB][n];
             b[j][i] = a.bias[j / NB] ? a.bias[j / NB][n] : 0.f;
         }
-    // (all loads before the bounds checks, from clamped places: inside them each would be waited for in turn)
-    float sxs[MB];
 #pragma unroll
-    for (int mb = 0; mb < MB; mb++) sxs[mb] = a.xs[a.pile_tok[tl.pos0 + min(16 * mb + (lane & 15), tl.m - 1)]];
+    for (int mb = 0; mb < MB; mb++) sx[mb] = a.xs[a.pile_tok[tl.pos0 + min(r0 + 16 * mb + (lane & 15), tl.m - 1)]];
 #pragma unroll
     for (int mb = 0; mb < MB; mb++) {
-        const int r = 16 * mb + (lane & 15);
+        const int r = r0 + 16 * mb + (lane & 15);
         if (r >= tl.m) continue;
-        const int p = tl.pos0 + r;
-        const float sx = sxs[mb];
 #pragma unroll
         for (int j = 0; j < NB; j++) {
             const int n = n0 + 16 * j + 4 * (lane >> 4);
@@ -311,41 +338,31 @@ __device__ __forceinline__ void gateup_tile(const I8MoeArgs &a, const MfTile &tl
             float h[4];
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                h[i] = glu(fmaf((float)acc[mb][j][i], sx * sw[j][i], b[j][i]), fmaf((float)acc[mb][NB + j][i], sx * sw[NB + j][i], b[NB + j][i]),
+                h[i] = glu(fmaf((float)acc[mb][j][i], sx[mb] * sw[j][i], b[j][i]), fmaf((float)acc[mb][NB + j][i], sx[mb] * sw[NB + j][i], b[NB + j][i]),
                            a.act, a.alpha, a.limit);
-            store_row<4>(a.h + (int64_t)p * a.ldh + n, a.I - n, h);
+            store_row<4>(a.h + (int64_t)(tl.pos0 + r) * a.ldh + n, a.I - n, h);
         }
     }
 }
-// Down of a tile: a wave holds 32 rows. One row of H per pick, f32, in pick order.
-template <int MB>
-__device__ __forceinline__ void down_tile(const I8MoeArgs &a, const MfTile &tl, int n0, uint8_t *lds) {
-    constexpr int NW = 2;
+// The same of down: one row of H per pick, f32, in pick order.
+template <int MB, int NW>
+__device__ __forceinline__ void finish_down(const I8MoeArgs &a, const I8Tile &tl, int r0, int n0, const i32x4 (&acc)[MB][NW]) {
     const int lane = threadIdx.x & 63;
-    const uint8_t *w0[1] = {a.w[2] + (int64_t)tl.expert * a.stride[2]};
-    uint32_t wrow[NW];
-#pragma unroll
-    for (int j = 0; j < NW; j++) wrow[j] = min(n0 + 16 * j + (lane & 15), a.H - 1) * a.rbi + 16 * (lane >> 4);
-    i32x4 acc[MB][NW];
-    i8_loop<MB, NW, 1>(lds, a.hq + (int64_t)tl.pos0 * a.rbi, [&](int r) { return (uint32_t)(min(r, tl.m - 1) * a.rbi); }, w0, wrow,
-                          a.rbi, acc);
-    float sw[NW][4];
+    float sw[NW][4], sx[MB];
+    int picks[MB];
 #pragma unroll
     for (int j = 0; j < NW; j++)
 #pragma unroll
         for (int i = 0; i < 4; i++) sw[j][i] = a.ws[2][(int64_t)tl.expert * a.H + min(n0 + 16 * j + 4 * (lane >> 4) + i, a.H - 1)];
-    float sxs[MB];
-    int picks[MB];
 #pragma unroll
     for (int mb = 0; mb < MB; mb++) {
-        const int p = tl.pos0 + min(16 * mb + (lane & 15), tl.m - 1);
-        sxs[mb] = a.hs[p];
+        const int p = tl.pos0 + min(r0 + 16 * mb + (lane & 15), tl.m - 1);
+        sx[mb] = a.hs[p];
         picks[mb] = a.pile_pick[p];
     }
 #pragma unroll
     for (int mb = 0; mb < MB; mb++) {
-        if (16 * mb + (lane & 15) >= tl.m) continue;
-        const float sx = sxs[mb];
+        if (r0 + 16 * mb + (lane & 15) >= tl.m) continue;
         float *d = a.dn + (int64_t)picks[mb] * a.H;
 #pragma unroll
         for (int j = 0; j < NW; j++) {
@@ -353,35 +370,61 @@ __device__ __forceinline__ void down_tile(const I8MoeArgs &a, const MfTile &tl, 
             if (n >= a.H) continue;
             float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = (float)acc[mb][j][i] * (sx * sw[j][i]);
+            for (int i = 0; i < 4; i++) v[i] = (float)acc[mb][j][i] * (sx[mb] * sw[j][i]);
             store_row<4>(d + n, a.H - n, v);
         }
     }
 }
 
-// Blocks go to the eight dies in turn; each die takes a contiguous range of the items (a tile's blocks of W one after
-// the other), so that a tile's picks are read by one die and not by all (2,048 tokens over 128 experts of 2,880 x 2,880:
-// 2.4 GB fetched for gate and up instead of 2.1).
-template <bool DOWN>
-__global__ __launch_bounds__(256, 2) void k_i8_moe_tiles(I8MoeArgs a, int n_blocks) {
-    extern __shared__ __align__(1024) uint8_t lds[];
+// The item of a block: blocks go to the eight dies in turn; each die takes a contiguous range of the items, an expert's
+// blocks of W one after the other and its tiles side by side for each, so that an expert's picks and weights are read by
+// one die and not by all, the weights once for all its tiles (2,048 tokens over 128 experts of 2,880 x 2,880: 2.4 GB
+// fetched for gate and up instead of 2.2 with the tiles in block order).
+__device__ __forceinline__ bool item_of_block(const I8MoeArgs &a, int n_blocks, I8Tile &tl, int &nb) {
     const int total = *a.n_tiles * n_blocks, die = blockIdx.x & 7, at = blockIdx.x >> 3, per = total >> 3, rest = total & 7;
-    if (at >= per + (die < rest)) return;
-    const int item = __builtin_amdgcn_readfirstlane(die * per + min(die, rest) + at), tile = item / n_blocks, nb = item % n_blocks;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const MfTile tl = a.tiles[tile];
-    const int n0 = DOWN ? 128 * nb + 32 * wave : 64 * nb + 16 * wave;
-    auto run = [&](auto mb) __attribute__((always_inline)) {
-        if constexpr (DOWN) down_tile<decltype(mb)::value>(a, tl, n0, lds);
-        else gateup_tile<decltype(mb)::value>(a, tl, n0, lds);
-    };
-    if (tl.m <= 16) run(Ic<1>{});
-    else if (tl.m <= 32) run(Ic<2>{});
-    else if (tl.m <= 48) run(Ic<3>{});
-    else if (tl.m <= 64) run(Ic<4>{});
-    else if (tl.m <= 80) run(Ic<5>{});
-    else if (tl.m <= 96) run(Ic<6>{});
-    else run(Ic<8>{});
+    if (at >= per + (die < rest)) return false;
+    const int item = die * per + min(die, rest) + at;
+    const I8Tile any = a.tiles[__builtin_amdgcn_readfirstlane(item / n_blocks)];  // a tile of the item's expert
+    const int in = item - any.first * n_blocks;
+    nb = __builtin_amdgcn_readfirstlane(in / any.of);
+    tl = a.tiles[__builtin_amdgcn_readfirstlane(any.first + in - nb * any.of)];
+    return true;
+}
+
+// A wave streams 16 rows of gate and of up, or 32 of down, for a tile's picks.
+template <bool DOWN, int MB>
+__device__ __forceinline__ void stream_tile(const I8MoeArgs &a, const I8Tile &tl, int n0, uint8_t *lds) {
+    const int lane = threadIdx.x & 63, rb = DOWN ? a.rbi : a.rbh;
+    uint32_t wrow[2];
+    i32x4 acc[MB][2];
+    if constexpr (DOWN) {
+        const uint8_t *w0[1] = {a.w[2] + (int64_t)tl.expert * a.stride[2]};
+#pragma unroll
+        for (int j = 0; j < 2; j++) wrow[j] = (uint32_t)min(n0 + 16 * j + (lane & 15), a.H - 1) * (uint32_t)rb + 16 * (lane >> 4);
+        i8_loop<MB, 2, 1>(lds, a.hq + (int64_t)tl.pos0 * rb, [&](int r) { return (uint32_t)(min(r, tl.m - 1) * rb); }, w0, wrow, rb, acc);
+        finish_down<MB, 2>(a, tl, 0, n0, acc);
+    } else {
+        const uint8_t *w0[2] = {a.w[0] + (int64_t)tl.expert * a.stride[0], a.w[1] + (int64_t)tl.expert * a.stride[1]};
+        wrow[0] = wrow[1] = (uint32_t)min(n0 + (lane & 15), a.I - 1) * (uint32_t)rb + 16 * (lane >> 4);
+        i8_loop<MB, 2, 2>(lds, a.x, [&](int r) { return (uint32_t)a.pile_tok[tl.pos0 + min(r, tl.m - 1)] * (uint32_t)rb; }, w0, wrow, rb, acc);
+        finish_gateup<MB, 1>(a, tl, 0, n0, acc);
+    }
+}
+constexpr int I8_GU_COLS = 64, I8_DN_COLS = 128;  // of a block
+template <bool DOWN>
+__global__ __launch_bounds__(256, 2) void k_i8_moe_stream(I8MoeArgs a, int n_blocks) {
+    extern __shared__ __align__(1024) uint8_t lds[];
+    I8Tile tl;
+    int nb;
+    if (!item_of_block(a, n_blocks, tl, nb)) return;
+    const int n0 = (DOWN ? 32 : 16) * (4 * nb + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    if (tl.m <= 16) stream_tile<DOWN, 1>(a, tl, n0, lds);
+    else if (tl.m <= 32) stream_tile<DOWN, 2>(a, tl, n0, lds);
+    else if (tl.m <= 48) stream_tile<DOWN, 3>(a, tl, n0, lds);
+    else if (tl.m <= 64) stream_tile<DOWN, 4>(a, tl, n0, lds);
+    else if (tl.m <= 80) stream_tile<DOWN, 5>(a, tl, n0, lds);
+    else if (tl.m <= 96) stream_tile<DOWN, 6>(a, tl, n0, lds);
+    else stream_tile<DOWN, 8>(a, tl, n0, lds);
 }
 
 // out[t] = sum_j w_j (dn_j + bias), in pick order; a thread per four columns
@@ -425,6 +468,8 @@ static bool few_path(const cw_i8_moe_desc *d, int T) {
     return (picks - distinct) * (2.0 * d->inter * rbh + (double)d->hidden * rbi) <= 200e6;
 }
 
+static int64_t i8_max_tiles(int64_t picks, int experts) { return (picks + I8_TILE - 1) / I8_TILE + std::min<int64_t>(experts, picks); }
+
 static I8MoeLayout layout(const cw_i8_moe_desc *d, int T) {
     I8MoeLayout L = {};
     size_t off = 0;
@@ -435,7 +480,7 @@ static I8MoeLayout layout(const cw_i8_moe_desc *d, int T) {
     take(L.w, TK * 4);
     take(L.h, TK * ((d->inter + 3) & ~3) * 4);
     if (!L.few) {
-        take(L.tiles, (size_t)max_tiles((int)TK, d->n_experts, I8_TILE) * sizeof(MfTile));
+        take(L.tiles, (size_t)i8_max_tiles(TK, d->n_experts) * sizeof(I8Tile));
         take(L.n_tiles, 4);
         take(L.pile_pick, TK * 4);
         take(L.pile_tok, TK * 4);
@@ -456,7 +501,10 @@ static int check_desc(const cw_i8_moe_desc *d, int T) {
     if (d->hidden > CW_I8_MAX_K || d->inter > CW_I8_MAX_K)
         return set_error(CW_ENOTSUP, "i8 moe: hidden %d, inter %d above %d", d->hidden, d->inter, CW_I8_MAX_K);
     CW_REQUIRE(d->act == CW_ACT_SILU || d->act == CW_ACT_CLAMPED_SWIGLU, "i8 moe: unknown activation %d", d->act);
-    CW_REQUIRE((int64_t)T * d->top_k < (1ll << 28), "i8 moe: %lld picks", (long long)T * d->top_k);
+    // (a launch holds fewer than 2^32 threads; offsets of rows of x from its start are 32 bits)
+    const int64_t blocks = i8_max_tiles((int64_t)T * d->top_k, d->n_experts) * std::max((d->inter + I8_GU_COLS - 1) / I8_GU_COLS, (d->hidden + I8_DN_COLS - 1) / I8_DN_COLS);
+    if ((int64_t)T * d->top_k >= 1 << 28 || blocks >= 1 << 23 || (int64_t)T * i8_row_bytes(d->hidden) >= 1ll << 32)
+        return set_error(CW_ENOTSUP, "i8 moe: %d tokens of %d picks, hidden %d, inter %d", T, d->top_k, d->hidden, d->inter);
     for (int m = 0; m < 3; m++) {
         const int64_t need = (m == 2 ? d->hidden : d->inter) * i8_row_bytes(m == 2 ? d->inter : d->hidden);
         CW_REQUIRE(d->w[m] && d->scale[m], "i8 moe: matrix %d is null", m);
@@ -520,18 +568,20 @@ static int moe_layer(const cw_i8_moe_desc *d, I8MoeArgs a, int ydtype, const I8M
         if (rc) return rc;
         return ydtype == CW_F16 ? few_down<_Float16>(a, s) : ydtype == CW_BF16 ? few_down<bf16_t>(a, s) : few_down<float>(a, s);
     }
-    const int TK = a.T * a.K, tmax = max_tiles(TK, a.E, I8_TILE);
+    const int TK = a.T * a.K, tmax = (int)i8_max_tiles(TK, a.E);
     int *pile_pick = (int *)(base + L.pile_pick), *pile_tok = (int *)(base + L.pile_tok), *n_tiles = (int *)(base + L.n_tiles);
-    MfTile *tiles = (MfTile *)(base + L.tiles);
+    I8Tile *tiles = (I8Tile *)(base + L.tiles);
+    auto plan = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), 0, s, a, pile_pick, pile_tok, tiles, n_tiles);
+        return check_launch("k_i8_plan");
+    };
     if (a.T <= I8_PLAN_TOKENS) {
-        if (a.E <= 256) hipLaunchKernelGGL(k_i8_plan<4>, dim3(1), dim3(1024), 0, s, a, pile_pick, pile_tok, tiles, n_tiles);
-        else if (a.E <= 512) hipLaunchKernelGGL(k_i8_plan<8>, dim3(1), dim3(1024), 0, s, a, pile_pick, pile_tok, tiles, n_tiles);
-        else hipLaunchKernelGGL(k_i8_plan<16>, dim3(1), dim3(1024), 0, s, a, pile_pick, pile_tok, tiles, n_tiles);
-        if ((rc = check_launch("k_i8_plan"))) return rc;
+        rc = a.E <= 256 ? plan(k_i8_plan<true, 4>) : a.E <= 512 ? plan(k_i8_plan<true, 8>) : plan(k_i8_plan<true, 16>);
     } else {
         if ((rc = cw_route_topk(a.logits, a.T, a.E, a.K, a.norm, a.ids, a.wt, s))) return rc;
-        if ((rc = mfma_piles(a.ids, nullptr, TK, a.K, a.E, 0, pile_pick, pile_tok, tiles, n_tiles, s, I8_TILE))) return rc;
+        rc = plan(k_i8_plan<false, 4>);
     }
+    if (rc) return rc;
     int8_t *hq = (int8_t *)(base + L.hq);
     float *hs = (float *)(base + L.hs);
     a.tiles = tiles;
@@ -541,12 +591,14 @@ static int moe_layer(const cw_i8_moe_desc *d, I8MoeArgs a, int ydtype, const I8M
     a.hq = (const uint8_t *)hq;
     a.hs = hs;
     a.dn = (float *)(base + L.dn);
-    const int lds = I8Stage<I8_TILE / 16>::LDS, gu = (a.I + 63) / 64, dn = (a.H + 127) / 128;
-    hipLaunchKernelGGL(k_i8_moe_tiles<false>, dim3((unsigned)((tmax * gu + 7) / 8 * 8)), dim3(256), lds, s, a, gu);
-    if ((rc = check_launch("k_i8_moe_tiles"))) return rc;
+    auto product = [&](auto kernel, int n, int cols) {
+        const int blocks = (n + cols - 1) / cols;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((tmax * blocks + 7) / 8 * 8)), dim3(256), I8Stage<I8_TILE / 16>::LDS, s, a, blocks);
+        return check_launch("k_i8_moe_stream");
+    };
+    if ((rc = product(k_i8_moe_stream<false>, a.I, I8_GU_COLS))) return rc;
     if ((rc = i8_quantize_f32(a.h, TK, a.I, a.ldh, hq, hs, s))) return rc;
-    hipLaunchKernelGGL(k_i8_moe_tiles<true>, dim3((unsigned)((tmax * dn + 7) / 8 * 8)), dim3(256), lds, s, a, dn);
-    if ((rc = check_launch("k_i8_moe_tiles"))) return rc;
+    if ((rc = product(k_i8_moe_stream<true>, a.H, I8_DN_COLS))) return rc;
     const int64_t n = (int64_t)a.T * ((a.H + 3) / 4);
     const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 16));
     if (ydtype == CW_F16) hipLaunchKernelGGL(k_i8_combine<_Float16>, grid, dim3(256), 0, s, a);

@@ -92,7 +92,7 @@ def test_layer_refuses_bad_calls():
             getattr(d, field)[m] = v
             assert layer(d) == CW_EINVAL, (m, field, v)
     d = desc()
-    assert layer(d, T=-1) == CW_EINVAL and layer(d, T=1 << 27) == CW_EINVAL
+    assert layer(d, T=-1) == CW_EINVAL and layer(d, T=1 << 27) == CW_ENOTSUP
     assert layer(d, dtype=F.MXFP4) == CW_ENOTSUP
     for bad in ({"x": None}, {"x": Q}, {"xs": None}, {"logits": None}, {"out": None}, {"ws": None}, {"ws": Q}):
         assert layer(d, **bad) == CW_EINVAL, bad
