@@ -391,40 +391,41 @@ __device__ __forceinline__ bool item_of_block(const I8MoeArgs &a, int n_blocks, 
     return true;
 }
 
-// A wave streams 16 rows of gate and of up, or 32 of down, for a tile's picks.
-template <bool DOWN, int MB>
+// A wave multiplies a tile's picks with 8 NW rows of gate and of up, or 16 NW of down.
+template <bool DOWN, int MB, int NW>
 __device__ __forceinline__ void stream_tile(const I8MoeArgs &a, const I8Tile &tl, int n0, uint8_t *lds) {
+    constexpr int NB = NW / 2;
     const int lane = threadIdx.x & 63, rb = DOWN ? a.rbi : a.rbh;
-    uint32_t wrow[2];
-    i32x4 acc[MB][2];
+    uint32_t wrow[NW];
+    i32x4 acc[MB][NW];
     if constexpr (DOWN) {
         const uint8_t *w0[1] = {a.w[2] + (int64_t)tl.expert * a.stride[2]};
 #pragma unroll
-        for (int j = 0; j < 2; j++) wrow[j] = (uint32_t)min(n0 + 16 * j + (lane & 15), a.H - 1) * (uint32_t)rb + 16 * (lane >> 4);
-        i8_loop<MB, 2, 1>(lds, a.hq + (int64_t)tl.pos0 * rb, [&](int r) { return (uint32_t)(min(r, tl.m - 1) * rb); }, w0, wrow, rb, acc);
-        finish_down<MB, 2>(a, tl, 0, n0, acc);
+        for (int j = 0; j < NW; j++) wrow[j] = (uint32_t)min(n0 + 16 * j + (lane & 15), a.H - 1) * (uint32_t)rb + 16 * (lane >> 4);
+        i8_loop<MB, NW, 1>(lds, a.hq + (int64_t)tl.pos0 * rb, [&](int r) { return (uint32_t)(min(r, tl.m - 1) * rb); }, w0, wrow, rb, acc);
+        finish_down<MB, NW>(a, tl, 0, n0, acc);
     } else {
         const uint8_t *w0[2] = {a.w[0] + (int64_t)tl.expert * a.stride[0], a.w[1] + (int64_t)tl.expert * a.stride[1]};
-        wrow[0] = wrow[1] = (uint32_t)min(n0 + (lane & 15), a.I - 1) * (uint32_t)rb + 16 * (lane >> 4);
-        i8_loop<MB, 2, 2>(lds, a.x, [&](int r) { return (uint32_t)a.pile_tok[tl.pos0 + min(r, tl.m - 1)] * (uint32_t)rb; }, w0, wrow, rb, acc);
-        finish_gateup<MB, 1>(a, tl, 0, n0, acc);
+#pragma unroll
+        for (int j = 0; j < NW; j++) wrow[j] = (uint32_t)min(n0 + 16 * (j % NB) + (lane & 15), a.I - 1) * (uint32_t)rb + 16 * (lane >> 4);
+        i8_loop<MB, NW, 2>(lds, a.x, [&](int r) { return (uint32_t)a.pile_tok[tl.pos0 + min(r, tl.m - 1)] * (uint32_t)rb; }, w0, wrow, rb, acc);
+        finish_gateup<MB, NB>(a, tl, 0, n0, acc);
     }
 }
-constexpr int I8_GU_COLS = 64, I8_DN_COLS = 128;  // of a block
-template <bool DOWN>
+template <bool DOWN, int NW>
 __global__ __launch_bounds__(256, 2) void k_i8_moe_stream(I8MoeArgs a, int n_blocks) {
     extern __shared__ __align__(1024) uint8_t lds[];
     I8Tile tl;
     int nb;
     if (!item_of_block(a, n_blocks, tl, nb)) return;
-    const int n0 = (DOWN ? 32 : 16) * (4 * nb + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
-    if (tl.m <= 16) stream_tile<DOWN, 1>(a, tl, n0, lds);
-    else if (tl.m <= 32) stream_tile<DOWN, 2>(a, tl, n0, lds);
-    else if (tl.m <= 48) stream_tile<DOWN, 3>(a, tl, n0, lds);
-    else if (tl.m <= 64) stream_tile<DOWN, 4>(a, tl, n0, lds);
-    else if (tl.m <= 80) stream_tile<DOWN, 5>(a, tl, n0, lds);
-    else if (tl.m <= 96) stream_tile<DOWN, 6>(a, tl, n0, lds);
-    else stream_tile<DOWN, 8>(a, tl, n0, lds);
+    const int n0 = (DOWN ? 16 : 8) * NW * (4 * nb + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    if (tl.m <= 16) stream_tile<DOWN, 1, NW>(a, tl, n0, lds);
+    else if (tl.m <= 32) stream_tile<DOWN, 2, NW>(a, tl, n0, lds);
+    else if (tl.m <= 48) stream_tile<DOWN, 3, NW>(a, tl, n0, lds);
+    else if (tl.m <= 64) stream_tile<DOWN, 4, NW>(a, tl, n0, lds);
+    else if (tl.m <= 80) stream_tile<DOWN, 5, NW>(a, tl, n0, lds);
+    else if (tl.m <= 96) stream_tile<DOWN, 6, NW>(a, tl, n0, lds);
+    else stream_tile<DOWN, 8, NW>(a, tl, n0, lds);
 }
 
 // out[t] = sum_j w_j (dn_j + bias), in pick order; a thread per four columns
@@ -502,7 +503,7 @@ static int check_desc(const cw_i8_moe_desc *d, int T) {
         return set_error(CW_ENOTSUP, "i8 moe: hidden %d, inter %d above %d", d->hidden, d->inter, CW_I8_MAX_K);
     CW_REQUIRE(d->act == CW_ACT_SILU || d->act == CW_ACT_CLAMPED_SWIGLU, "i8 moe: unknown activation %d", d->act);
     // (a launch holds fewer than 2^32 threads; offsets of rows of x from its start are 32 bits)
-    const int64_t blocks = i8_max_tiles((int64_t)T * d->top_k, d->n_experts) * std::max((d->inter + I8_GU_COLS - 1) / I8_GU_COLS, (d->hidden + I8_DN_COLS - 1) / I8_DN_COLS);
+    const int64_t blocks = i8_max_tiles((int64_t)T * d->top_k, d->n_experts) * std::max((d->inter + 63) / 64, (d->hidden + 127) / 128);
     if ((int64_t)T * d->top_k >= 1 << 28 || blocks >= 1 << 23 || (int64_t)T * i8_row_bytes(d->hidden) >= 1ll << 32)
         return set_error(CW_ENOTSUP, "i8 moe: %d tokens of %d picks, hidden %d, inter %d", T, d->top_k, d->hidden, d->inter);
     for (int m = 0; m < 3; m++) {
@@ -561,6 +562,16 @@ static int few_gateup(const I8MoeArgs &a, hipStream_t s) {
     return set_error(CW_ENOTSUP, "i8 moe: rows of %d", a.H);
 }
 
+// Four groups of weight rows a wave instead of two, where the picks share the weights and there are blocks for every CU
+// twice. Measured, two / four groups: 128 experts of 2,880 x 2,880, top-4, 64 tokens (2 picks an expert) 525 / 544 us,
+// 512 tokens (16) 662 / 660, 2,048 tokens (64) 823 / 803; 256 of 512 x 2,048, top-8, 512 tokens (16) 213 / 204; 64 of
+// 1,408 x 2,048, top-6, 2,048 tokens (192) 316 / 281; 16 of 2,880 x 4,096, top-2, 512 tokens (64, 368 blocks) 160 / 165,
+// 2,048 tokens (256, 736 blocks) 360 / 318.
+static bool many_picks(const I8MoeArgs &a) {
+    const double picks = (double)a.T * a.K, avg = picks / a.E;
+    return avg >= 12 && a.E * ceil(avg / I8_TILE) * ((a.I + 127) / 128) >= 2 * resident_blocks(1);
+}
+
 static int moe_layer(const cw_i8_moe_desc *d, I8MoeArgs a, int ydtype, const I8MoeLayout &L, uint8_t *base, hipStream_t s) {
     int rc;
     if (L.few) {
@@ -591,14 +602,18 @@ static int moe_layer(const cw_i8_moe_desc *d, I8MoeArgs a, int ydtype, const I8M
     a.hq = (const uint8_t *)hq;
     a.hs = hs;
     a.dn = (float *)(base + L.dn);
-    auto product = [&](auto kernel, int n, int cols) {
-        const int blocks = (n + cols - 1) / cols;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((tmax * blocks + 7) / 8 * 8)), dim3(256), I8Stage<I8_TILE / 16>::LDS, s, a, blocks);
+    constexpr int LDS = I8Stage<I8_TILE / 16, 2>::LDS;
+    auto product = [&](auto kernel, int nw, bool down) {
+        const int cols = (down ? 64 : 32) * nw, blocks = ((down ? a.H : a.I) + cols - 1) / cols;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((tmax * blocks + 7) / 8 * 8)), dim3(256), LDS, s, a, blocks);
         return check_launch("k_i8_moe_stream");
     };
-    if ((rc = product(k_i8_moe_stream<false>, a.I, I8_GU_COLS))) return rc;
+    const bool many = many_picks(a);
+    rc = many ? product(k_i8_moe_stream<false, 4>, 4, false) : product(k_i8_moe_stream<false, 2>, 2, false);
+    if (rc) return rc;
     if ((rc = i8_quantize_f32(a.h, TK, a.I, a.ldh, hq, hs, s))) return rc;
-    if ((rc = product(k_i8_moe_stream<true>, a.H, I8_DN_COLS))) return rc;
+    rc = many ? product(k_i8_moe_stream<true, 4>, 4, true) : product(k_i8_moe_stream<true, 2>, 2, true);
+    if (rc) return rc;
     const int64_t n = (int64_t)a.T * ((a.H + 3) / 4);
     const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 16));
     if (ydtype == CW_F16) hipLaunchKernelGGL(k_i8_combine<_Float16>, grid, dim3(256), 0, s, a);
