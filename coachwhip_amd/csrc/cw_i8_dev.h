@@ -89,13 +89,27 @@ __device__ __forceinline__ uint32_t code(double y, double inv) {
 }
 __device__ __forceinline__ uint32_t codes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return a | b << 8 | c << 16 | d << 24; }
 
-// h = act(g, u): silu(g) u, or the clamped form of gpt-oss (cw_clamped_swiglu, without its biases)
+// h = act(g, u): silu(g) u, or the clamped form of gpt-oss (cw_clamped_swiglu, without its biases), with the hardware's
+// 2^x and 1 / x, an ulp each: 11 operations, where the library's exp and a correctly rounded division take about 40
+// (8,192 rows of 2,880 to codes 44 -> 31 us).
 __device__ __forceinline__ float glu(float g, float u, int act, float alpha, float limit) {
-    if (act == CW_ACT_SILU) return g / (1.0f + expf(-g)) * u;
+    constexpr float LOG2E = 1.4426950408889634f;
+    if (act == CW_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -LOG2E)) * u;
     // (comparisons rather than fminf: a NaN stays one)
     g = g > limit ? limit : g;
     u = u > limit ? limit : u < -limit ? -limit : u;
-    return (u + 1.0f) * (g * (1.0f / (1.0f + expf(-(g * alpha)))));
+    return (u + 1.0f) * (g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * (alpha * -LOG2E))));
+}
+
+// the larger of m and |v|'s bits: ordered as the magnitudes are, infinities and NaNs above all finite ones
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, float v) { return max(m, __float_as_uint(v) & 0x7FFFFFFFu); }
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+    v = max(v, dpp_u<0xB1>(v));
+    v = max(v, dpp_u<0x4E>(v));
+    v = max(v, dpp_u<0x141>(v));
+    v = max(v, dpp_u<0x140>(v));
+    return max(max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16)),
+               max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
 }
 
 }  // namespace cw

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 ? 4 : 1) void k_i8_few_d
     constexpr int NH = NC < 12 ? (NC + 1) / 2 : 6;  // pieces of a hidden row held in registers (the others are read twice)
     extern __shared__ __align__(16) uint8_t hq[];  // K rows of rbi codes
     __shared__ float hs[32], coef[I8_FEW_WAVES * R][33];
-    __shared__ double top[I8_FEW_WAVES];
+    __shared__ uint32_t top[I8_FEW_WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.y, cpr = a.rbi / 16;
     const int row0 = (blockIdx.x * I8_FEW_WAVES + wave) * R;
     const int wpp = a.K > 4 ? 1 : a.K > 2 ? 2 : a.K > 1 ? 4 : 8, at0 = 4 * ((wave & (wpp - 1)) * 64 + lane), stride = 256 * wpp;
@@ -156,13 +156,10 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 ? 4 : 1) void k_i8_few_d
         const int j = j0 + wave / wpp;
         const float *row = h + (int64_t)min(j, a.K - 1) * a.ldh;
         if (j0) fetch_h(min(j, a.K - 1));
-        double m = 0.0;
+        uint32_t bits = 0;
         auto more = [&](const float (&v)[4]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const double y = fabs((double)v[i]);
-                m = y <= m ? m : y < INFINITY ? y : INFINITY;
-            }
+            for (int i = 0; i < 4; i++) bits = max_bits(bits, v[i]);
         };
 #pragma unroll
         for (int i = 0; i < NH; i++) more(hv[i]);
@@ -171,16 +168,16 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 ? 4 : 1) void k_i8_few_d
             load_row<4>(row + c, a.I - c, v);
             more(v);
         }
-        m = wave_max_d(m);
+        bits = wave_max_u(bits);
         if (wpp > 1) {
-            if (lane == 0) top[wave] = m;
+            if (lane == 0) top[wave] = bits;
             __syncthreads();
-            for (int o = 1; o < wpp; o++) m = fmax(m, top[wave ^ o]);
+            for (int o = 1; o < wpp; o++) bits = max(bits, top[wave ^ o]);
             if (j0 + I8_FEW_WAVES / wpp < a.K) __syncthreads();
         }
         if (j >= a.K) continue;
-        const bool some = m > 0.0 && m < INFINITY;
-        const double inv = some ? 127.0 / m : 0.0;
+        const bool fine = bits < 0x7F800000u, some = fine && bits;
+        const double m = __uint_as_float(bits), inv = some ? 127.0 / m : 0.0;
         auto store = [&](int c, const float (&v)[4]) __attribute__((always_inline)) {
             *(uint32_t *)(hq + j * a.rbi + c) = some ? codes4(code(v[0], inv), code(v[1], inv), code(v[2], inv), code(v[3], inv)) : 0u;
         };
@@ -192,7 +189,7 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 ? 4 : 1) void k_i8_few_d
             load_row<4>(row + c, a.I - c, v);
             store(c, v);
         }
-        if (lane == 0 && (wave & (wpp - 1)) == 0) hs[j] = m < INFINITY ? (float)(m / 127.0) : __int_as_float(0x7fc00000);
+        if (lane == 0 && (wave & (wpp - 1)) == 0) hs[j] = fine ? (float)(m / 127.0) : __int_as_float(0x7fc00000);
     }
     __syncthreads();
 #pragma unroll

@@ -152,9 +152,9 @@ def test_rmsnorm_rows_not_finite_stay_alone():
     assert not zero.scale.any() and not zero.q.any()
 
 
-# h in f32: exp within an ulp (2 U) of its argument's value, whose own rounding is 8 * 1.702 U at |g| <= 8; the two sums, the
-# division, the products a U each
-GLU_REL = (2 + 14 + 6) * U
+# h in f32: 2^x within an ulp (2 U) of its argument's value, whose own rounding and that of the constant in it are 2 U of at most
+# 8 * 1.702 (as a power of e); 1 / x within an ulp; the two sums and the products a U each
+GLU_REL = (2 + 2 * 8 * 1.702 + 2 + 6) * U
 
 
 def glu64(g, u, act):
@@ -299,7 +299,7 @@ class Experts:
             # d h: the factors' slopes (|silu'| <= 1.1, of the clamped form 1.1 as well) times their errors, and the activation's own
             dg, du = 4 * U * (pg.abs() + g.abs()), 4 * U * (pu.abs() + u.abs())
             gate = (g * torch.sigmoid(act.alpha * g)).abs() if act.kind else (g * torch.sigmoid(g)).abs()
-            rel = GLU_REL + (act.alpha if act.kind else 1) * g.abs() * 2 * U
+            rel = GLU_REL + (act.alpha if act.kind else 1) * g.abs() * 2 * U  # (of arguments past 8 * 1.702)
             dh = 1.2 * dg * (u.abs() + act.kind) + du * gate + rel * h.abs()
             a = h.abs().amax(1, keepdim=True)
             da = dh.amax(1, keepdim=True)
