@@ -223,7 +223,7 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 ? 4 : 1) void k_i8_few_d
 // I8_STAGED picks (scattered 4-byte stores from one CU cost a memory transaction each). ROUTE: of up to I8_PLAN_TOKENS
 // tokens, which its waves route first, every 16th token each: one launch less (9 tokens over 256 experts 9.8 -> 7 us; with
 // more tokens the routing of a CU to each is faster).
-constexpr int I8_PLAN_TOKENS = 64, I8_STAGED = 12288;
+constexpr int I8_PLAN_TOKENS = 32, I8_STAGED = 12288;
 template <bool ROUTE, int PER>
 __global__ __launch_bounds__(1024) void k_i8_plan(I8MoeArgs a, int *pile_pick, int *pile_tok, I8Tile *tiles, int *n_tiles) {
     __shared__ int cnt[1024], place[1024], sums[2][16], staged[I8_STAGED];
@@ -384,7 +384,8 @@ __device__ __forceinline__ bool item_of_block(const I8MoeArgs &a, int n_blocks, 
     const I8Tile any = a.tiles[__builtin_amdgcn_readfirstlane(item / n_blocks)];  // a tile of the item's expert
     const int in = item - any.first * n_blocks;
     nb = __builtin_amdgcn_readfirstlane(in / any.of);
-    tl = a.tiles[__builtin_amdgcn_readfirstlane(any.first + in - nb * any.of)];
+    if (any.of == 1) tl = any;
+    else tl = a.tiles[__builtin_amdgcn_readfirstlane(any.first + in - nb * any.of)];
     return true;
 }
 

@@ -90,11 +90,10 @@ enum { K_NATURAL = 0, K_PAIRS = 1, K_OCTETS = 2 };
 inline int k_order(int dtype) {
     return dtype == CW_MXFP4 ? K_PAIRS : dtype == CW_Q8_0 || dtype == CW_IQ4_XS ? K_NATURAL : K_OCTETS;
 }
-// one block: piles of the picks by slot, or by expert where n_experts is not 0, and the list of their tiles of
-// up to tile_rows picks
+// one block: piles of the picks by slot, or by expert where n_experts is not 0, and the tile list
 int mfma_piles(const uint32_t *slots, const uint32_t *ids, int TK, int K, int n_slots, int n_experts, int *pile_pick, int *pile_tok,
-               MfTile *tiles, int *n_tiles, hipStream_t s, int tile_rows = MF_MT);
-int max_tiles(int TK, int n_piles, int tile_rows = MF_MT);
+               MfTile *tiles, int *n_tiles, hipStream_t s);
+int max_tiles(int TK, int n_piles);
 // rows x k f32 -> fp16 rows (ld = k, K order as given) with per-row power-of-two scales
 int pack_rows_f16(const float *x, int rows, int k, int ldx, uint16_t *a16, float *ascale, hipStream_t s,
                   const PackExtra *extra = nullptr, int order = K_NATURAL);

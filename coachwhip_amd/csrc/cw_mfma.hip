@@ -571,7 +571,7 @@ __device__ __forceinline__ int wave_incl_scan(int v, int lane) {
 constexpr int PILE_PER = 16, PILE_LDS = 12288;
 template <bool BY_EXPERT>
 __global__ __launch_bounds__(1024) void k_piles(const uint32_t *slots, const uint32_t *ids, int TK, int K, int n_slots, int n_keys,
-                                                 int mt, int *pile_pick, int *pile_tok, MfTile *tiles, int *n_tiles) {
+                                                 int *pile_pick, int *pile_tok, MfTile *tiles, int *n_tiles) {
     __shared__ int cnt[1024], off[1024], cur[1024], rep[1024], wtot[16], wttot[16], wftot[16];
     __shared__ int staged[PILE_LDS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -604,10 +604,10 @@ __global__ __launch_bounds__(1024) void k_piles(const uint32_t *slots, const uin
     __syncthreads();
     // exclusive scans of the counts, the tile counts and the first tiles: per wave, then over the
     // 16 wave totals. The tile list holds every slot's first tile, then the later tiles of the
-    // slots with more than mt picks (a tile's rows): the GEMMs hand out work items in list order, so the last
+    // slots with more than MF_MT picks: the GEMMs hand out work items in list order, so the last
     // round of items, which only some blocks run, takes the (smaller) remainder tiles.
     const int c = tid < n_keys ? cnt[tid] : 0;
-    const int tc = (c + mt - 1) / mt, fc = c > 0 ? 1 : 0;
+    const int tc = (c + MF_MT - 1) / MF_MT, fc = c > 0 ? 1 : 0;
     const int ic = wave_incl_scan(c, lane), itc = wave_incl_scan(tc, lane), ifc = wave_incl_scan(fc, lane);
     if (lane == 63) {
         wtot[wave] = ic;
@@ -630,7 +630,7 @@ __global__ __launch_bounds__(1024) void k_piles(const uint32_t *slots, const uin
     if (tid < n_keys) {
         const int ex = !BY_EXPERT && ids && c > 0 ? (int)ids[rep[tid]] : tid, sl = BY_EXPERT && c > 0 ? (int)slots[rep[tid]] : tid;
         for (int q = 0; q < tc; q++)
-            tiles[q == 0 ? my_f : nf + (my_toff - my_f) + q - 1] = MfTile{sl, my_off + q * mt, min(mt, c - q * mt), ex};
+            tiles[q == 0 ? my_f : nf + (my_toff - my_f) + q - 1] = MfTile{sl, my_off + q * MF_MT, min(MF_MT, c - q * MF_MT), ex};
     }
     __syncthreads();
     for (int c0 = 0; c0 < TK; c0 += 1024 * PILE_PER) {
@@ -774,13 +774,13 @@ bool mfma_supported(int dtype) {
            dtype == CW_Q2_K || dtype == CW_IQ3_XXS || dtype == CW_IQ4_XS || dtype == CW_MXFP4_R16;
 }
 
-int max_tiles(int TK, int n_piles, int tile_rows) { return (TK + tile_rows - 1) / tile_rows + (n_piles < TK ? n_piles : TK); }
+int max_tiles(int TK, int n_piles) { return (TK + MF_MT - 1) / MF_MT + (n_piles < TK ? n_piles : TK); }
 
 int mfma_piles(const uint32_t *slots, const uint32_t *ids, int TK, int K, int n_slots, int n_experts, int *pile_pick, int *pile_tok,
-               MfTile *tiles, int *n_tiles, hipStream_t s, int tile_rows) {
+               MfTile *tiles, int *n_tiles, hipStream_t s) {
     if (n_slots > 1024 || n_experts > 1024) return set_error(CW_ENOTSUP, "mfma: %d slots, %d experts (1024 max)", n_slots, n_experts);
-    if (n_experts) hipLaunchKernelGGL(k_piles<true>, dim3(1), dim3(1024), 0, s, slots, ids, TK, K, n_slots, n_experts, tile_rows, pile_pick, pile_tok, tiles, n_tiles);
-    else hipLaunchKernelGGL(k_piles<false>, dim3(1), dim3(1024), 0, s, slots, ids, TK, K, n_slots, n_slots, tile_rows, pile_pick, pile_tok, tiles, n_tiles);
+    if (n_experts) hipLaunchKernelGGL(k_piles<true>, dim3(1), dim3(1024), 0, s, slots, ids, TK, K, n_slots, n_experts, pile_pick, pile_tok, tiles, n_tiles);
+    else hipLaunchKernelGGL(k_piles<false>, dim3(1), dim3(1024), 0, s, slots, ids, TK, K, n_slots, n_slots, pile_pick, pile_tok, tiles, n_tiles);
     return check_launch("k_piles");
 }
 

@@ -208,7 +208,8 @@ class I8Matrix:
 
     @classmethod
     def from_qtensor(cls, w: ops.QTensor):
-        return cls.from_float(w.dequantize())
+        with torch.cuda.device(w.data.device):
+            return cls.from_float(w.dequantize())
 
 
 class I8MatMul:
@@ -268,10 +269,11 @@ class I8ExpertBank:
         q = torch.empty((e, n, row_bytes(k)), dtype=torch.int8, device=bank.data.device)
         scale = torch.empty((e, n), dtype=torch.float32, device=bank.data.device)
         size = F.matrix_bytes(bank.dtype, n, k)
-        for s in range(e):
-            raw = bank.data[s * bank.slot_stride:s * bank.slot_stride + size]
-            r = quantize_i8(ops.dequantize(bank.dtype, raw, n * k).view(n, k))
-            q[s], scale[s] = r.q, r.scale
+        with torch.cuda.device(bank.data.device):
+            for s in range(e):
+                raw = bank.data[s * bank.slot_stride:s * bank.slot_stride + size]
+                r = quantize_i8(ops.dequantize(bank.dtype, raw, n * k).view(n, k))
+                q[s], scale[s] = r.q, r.scale
         return cls(q, scale, k)
 
 

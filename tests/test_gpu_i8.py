@@ -193,7 +193,10 @@ def check_matmul(x, w, bias, dtype, y):
 
 MM_SHAPES = [(1, 1, 1), (1, 2048, 2048), (2, 17, 100), (1, 513, 4097), (3, 4001, 2880), (15, 64, 128), (16, 4096, 4096), (17, 70, 640), (33, 1000, 257),
              (77, 4001, 2880), (64, 512, 8192), (100, 33, 32768), (128, 256, 384), (129, 255, 896), (130, 2048, 200), (200, 1024, 1024), (300, 777, 1536),
-             (513, 513, 513), (1025, 300, 128), (700, 4096, 640)]
+             (513, 513, 513), (1025, 300, 128), (700, 4096, 640),
+             # a step or a few in a ring of eight, tiles of 64 x 128, of 128 x 128, of 256 x 256
+             (200, 300, 64), (200, 300, 384), (90, 500, 1025), (20, 9000, 2000), (512, 4001, 1500), (400, 4096, 300), (900, 3000, 2500), (3600, 4500, 128),
+             (8200, 8200, 100), (4096, 4000, 512), (5000, 3001, 897), (2500, 6001, 300), (5000, 4000, 2000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
