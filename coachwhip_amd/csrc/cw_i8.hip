@@ -27,7 +27,8 @@ struct RowsArgs {
 // y * 127 / a to the nearest. The norm's mean, factor and products and every code are computed in 64 bits,
 // whose vector rate here is half that of 32: a code does not depend on the order of a sum, and the kernel
 // stays bound by its bytes. A row with a value that is not finite gets the scale NaN and zero codes; a row
-// of zeros the scale 0.
+// of zeros the scale 0. 8,192 rows, bf16: norm of 4,096 50 us (4.7 TB/s), SwiGLU of 2,880 29 (4.0; about 30 vector
+// operations a value beside the loads).
 template <class T, int MODE, int TPR, int NCH>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_rows_i8(RowsArgs a) {
     constexpr int NT = TPR == 64 ? 256 : TPR, RPB = NT / TPR, WPR = TPR / 64;

@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256, 1) void k_i8_big(I8MatArgs a, int tiles_m, int
 }
 
 // Fewer rows than fill the device with such tiles: tiles of 32 FM x 32 FN, eight waves: two groups of four (16 FM x
-// 16 FN each), one for each half of a step. A ring of LDS stages keeps 80 to 112 KB of loads in flight on a CU, whose
+// 16 FN each), one for each half of a step. A ring of LDS stages keeps 96 to 128 KB of loads in flight on a CU, whose
 // share of L2 bounds these tiles; the groups' integer sums meet in LDS.
 template <int FM, int FN>
 struct I8Ring {

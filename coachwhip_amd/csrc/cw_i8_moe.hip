@@ -375,8 +375,8 @@ __device__ __forceinline__ void finish_down(const I8MoeArgs &a, const I8Tile &tl
 
 // The item of a block: blocks go to the eight dies in turn; each die takes a contiguous range of the items, an expert's
 // blocks of W one after the other and its tiles side by side for each, so that an expert's picks and weights are read by
-// one die and not by all, the weights once for all its tiles (2,048 tokens over 128 experts of 2,880 x 2,880: 2.4 GB
-// fetched for gate and up instead of 2.2 with the tiles in block order).
+// one die and not by all, the weights once for all its tiles (2,048 tokens over 128 experts of 2,880 x 2,880: 2.2 GB
+// fetched for gate and up, 2.4 with the tiles in block order).
 __device__ __forceinline__ bool item_of_block(const I8MoeArgs &a, int n_blocks, I8Tile &tl, int &nb) {
     const int total = *a.n_tiles * n_blocks, die = blockIdx.x & 7, at = blockIdx.x >> 3, per = total >> 3, rest = total & 7;
     if (at >= per + (die < rest)) return false;
@@ -389,7 +389,9 @@ __device__ __forceinline__ bool item_of_block(const I8MoeArgs &a, int n_blocks, 
     return true;
 }
 
-// A wave multiplies a tile's picks with 8 NW rows of gate and of up, or 16 NW of down.
+// A wave multiplies a tile's picks with 8 NW rows of gate and of up, or 16 NW of down. 2,048 tokens over 128 experts of
+// 2,880 x 2,880: gate and up 491 us, down 257, 4.35 TB/s of weights, which bound it, beside the f32 rows it writes (gate
+// and up without their stores: 411).
 template <bool DOWN, int MB, int NW>
 __device__ __forceinline__ void stream_tile(const I8MoeArgs &a, const I8Tile &tl, int n0, uint8_t *lds) {
     constexpr int NB = NW / 2;
@@ -426,7 +428,8 @@ __global__ __launch_bounds__(256, 2) void k_i8_moe_stream(I8MoeArgs a, int n_blo
     else stream_tile<DOWN, 8, NW>(a, tl, n0, lds);
 }
 
-// out[t] = sum_j w_j (dn_j + bias), in pick order; a thread per four columns
+// out[t] = sum_j w_j (dn_j + bias), in pick order; a thread per four columns (2,048 tokens of 4 picks, 2,880 columns:
+// 106 MB in 23 us, 4.6 TB/s)
 template <class T>
 __global__ __launch_bounds__(256) void k_i8_combine(I8MoeArgs a) {
     const int per = (a.H + 3) / 4;

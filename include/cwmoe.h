@@ -330,7 +330,8 @@ int cw_dequantize_i8(const int8_t *q, const float *scale, int64_t rows, int64_t 
                      cw_stream_t stream);
 
 /* y[r][c] = x_scale[r] * w_scale[c] * sum_k x[r][k] w[c][k] (+ bias[c], f32, may be NULL), rounded
- * once to ydtype; W is n rows of k codes, x m rows; rows of y are ldy elements apart. */
+ * once to ydtype; W is n rows of k codes, x m rows; rows of y are ldy elements apart. CW_ENOTSUP
+ * for n above 2^26 and for products of 2^22 tiles (256 x 256 at most, about 2.7e11 outputs). */
 int cw_i8_matmul(const int8_t *w, const float *w_scale, int64_t n, int64_t k, const int8_t *x, const float *x_scale,
                  int64_t m, const float *bias, int ydtype, void *y, int64_t ldy, cw_stream_t stream);
 
@@ -353,7 +354,9 @@ typedef struct cw_i8_moe_desc {
  * and up of the picked experts, the activation in f32, the hidden row of each pick quantized as
  * cw_quantize_i8 does, down, the weighted sum in f32, rounded once to ydtype. ids_out / w_out
  * (T x K, may be NULL) receive the routing. A few tokens run as two launches. ws: 256-byte aligned,
- * of cw_i8_moe_workspace_size bytes, any contents; calls that overlap in time need distinct ones. */
+ * of cw_i8_moe_workspace_size bytes, any contents; calls that overlap in time need distinct ones.
+ * CW_ENOTSUP where T x top_k reaches 2^28, where the T rows of x reach 4 GiB, and where a launch
+ * would exceed the grid. */
 size_t cw_i8_moe_workspace_size(const cw_i8_moe_desc *desc, int T);
 int cw_i8_moe_layer(const cw_i8_moe_desc *desc, const int8_t *x, const float *x_scale, const float *logits, int T, int ydtype,
                     void *out, uint32_t *ids_out, float *w_out, void *ws, size_t ws_bytes, cw_stream_t stream);

@@ -62,7 +62,7 @@ def rand_rows(g, n, k):
 
 # ------------------------------------------------------------------------------ rows to codes
 
-ROW_SHAPES = [(1, 1), (3, 7), (1, 128), (2, 129), (5, 512), (4, 1000), (1, 2048), (7, 2880), (3, 4097), (2, 8192), (2, 9001), (1, 32768), (1030, 66)]
+ROW_SHAPES = [(1, 1), (3, 7), (1, 128), (2, 129), (5, 512), (4, 1000), (1, 2048), (7, 2880), (3, 4097), (2, 8192), (2, 9001), (1, 32768), (1030, 66), (2053, 2881)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
