@@ -339,7 +339,7 @@ def test_layer_matches_64_bits(E, K, H, I, act, bias, T):
         ex.check(x, logits, K, norm, out, ids, w)
 
 
-@pytest.mark.parametrize("T", [129, 600])
+@pytest.mark.parametrize("T", [129, 600, 1100])
 def test_layer_with_every_token_on_one_expert(T):
     ex = Experts(6, 256, 200, "silu", False, 1)
     x, logits = ex.inputs(T)
@@ -349,7 +349,7 @@ def test_layer_with_every_token_on_one_expert(T):
     ex.check(x, logits, 2, True, out, ids, w)
 
 
-@pytest.mark.parametrize("T", [2, 30])
+@pytest.mark.parametrize("T", [2, 30, 1030])  # (the last grouped)
 def test_layer_rows_not_finite_or_zero_stay_alone(T):
     ex = Experts(8, 256, 96, "clamped", True, 2)
     x, logits = ex.inputs(T)
@@ -361,6 +361,31 @@ def test_layer_rows_not_finite_or_zero_stay_alone(T):
     x[1][1] = 0
     out, ids, w = layer.forward(i8.I8Rows(*x, 256), logits)
     ex.check(x, logits, 2, True, out, ids, w)
+
+
+@pytest.mark.parametrize("T", [5, 1030])  # (in two launches, and grouped)
+def test_layer_logits_not_finite_stay_alone(T):
+    """The routing is ``ops.route``'s, whatever the logits: picks are experts that exist, each once; a row with a NaN or
+    +inf among its logits, or with -inf alone, has NaN results, -inf beside enough finite logits masks an expert, and so does
+    a NaN with its sign set, which that order puts below every other value (renormalised weights sum the picks alone)."""
+    ex = Experts(70, 256, 96, "clamped", True, 3)
+    x, logits = ex.inputs(T)
+    layer = ex.layer(4)
+    clean = layer.forward(i8.I8Rows(*x, 256), logits)
+    bad = logits.clone()
+    bad[0, 69] = float("nan")
+    bad[1, ::2] = torch.tensor([-1], dtype=torch.int32, device="cuda").view(torch.float32)  # a negative NaN, all bits set
+    bad[2] = -float("inf")
+    bad[3, 7] = float("inf")
+    bad[4, 4:] = -float("inf")
+    out, ids, w = layer.forward(i8.I8Rows(*x, 256), bad)
+    assert ((0 <= ids) & (ids < 70)).all() and all(len(set(row)) == 4 for row in ids.tolist())
+    want_ids, want_w = ops.route(bad, 4, True)
+    assert torch.equal(ids, want_ids.to(ids.dtype)) and torch.allclose(w, want_w, rtol=0, atol=0, equal_nan=True)
+    assert torch.isnan(out[[0, 2, 3]]).all() and torch.isfinite(out[1]).all() and (ids[1] % 2 == 1).all()
+    assert sorted(ids[4].tolist()) == [0, 1, 2, 3] and torch.isfinite(out[4]).all()
+    for a, b in zip((out, ids, w), clean):
+        assert torch.equal(a[5:], b[5:])
 
 
 @pytest.mark.parametrize("T", [1, 8, 50])
