@@ -12,8 +12,7 @@ struct RowsArgs {
     int64_t ldx, ldr;         // elements between rows
     int64_t rows, row0;       // this launch: rows row0 .. rows - 1
     int k;
-    int act;                  // GLU
-    float alpha, limit;
+    Glu glu;
     const float *w;           // norm
     double eps;
     void *sum;                // norm: x + r (or NULL), rows of k
@@ -49,7 +48,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_rows_i8(RowsArgs a) {
             float u[8];
             load_row<8>(r + e, valid, u);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = i < valid ? glu(v[i], u[i], a.act, a.alpha, a.limit) : 0.f;
+            for (int i = 0; i < 8; i++) v[i] = i < valid ? glu(v[i], u[i], a.glu) : 0.f;
         }
         if constexpr (MODE == ROWS_NORM) {
             if (a.r) {
@@ -237,9 +236,7 @@ int cw_swiglu_i8(int dtype, const void *g, const void *u, int64_t ld, int64_t ro
     a.ldx = a.ldr = ld;
     a.rows = rows;
     a.k = (int)width;
-    a.act = act;
-    a.alpha = alpha;
-    a.limit = limit;
+    a.glu = glu_of(act, alpha, limit);
     a.q = (uint8_t *)q;
     a.scale = scale;
     return rows_i8<ROWS_GLU>(dtype, a, (hipStream_t)stream);

@@ -89,16 +89,34 @@ __device__ __forceinline__ uint32_t code(double y, double inv) {
 }
 __device__ __forceinline__ uint32_t codes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return a | b << 8 | c << 16 | d << 24; }
 
-// h = act(g, u): silu(g) u, or the clamped form of gpt-oss (cw_clamped_swiglu, without its biases), with the hardware's
-// 2^x and 1 / x, an ulp each: 11 operations, where the library's exp and a correctly rounded division take about 40
-// (8,192 rows of 2,880 to codes took 44 us with those, 31 with these, all else alike).
-__device__ __forceinline__ float glu(float g, float u, int act, float alpha, float limit) {
-    constexpr float LOG2E = 1.4426950408889634f;
-    if (act == CW_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -LOG2E)) * u;
+// The activation's constants: c1 + c2 = -alpha log2(e) in two f32 terms (alpha 1: silu).
+struct Glu {
+    int act;
+    float limit, c1, c2;
+};
+inline Glu glu_of(int act, float alpha, float limit) {
+    const double c = -1.4426950408889634 * (act == CW_ACT_SILU ? 1.0 : (double)alpha);
+    const float c1 = (float)c;
+    return Glu{act, limit, c1, (float)(c - (double)c1)};
+}
+// 1 / (1 + e^(-alpha g)) = 1 / (1 + 2^p), p = g (c1 + c2), with the hardware's 2^x and 1 / x, an ulp each. What p lost when it was
+// rounded to f32, lo (up to 2^-17 of a power of two, 30 half steps of the result), comes back to first order, sigma(p + lo) =
+// s - s (1 - s) ln2 lo, whose next term is below 2^-35: 6 half steps of f32 at most, whatever g is.
+// 12 operations, 6 of them for lo (8,192 rows of 2,880 to codes with the values read back, in a graph: 38.6 us without them, 40.9
+// with); the library's exp and a correctly rounded division are about 40. (lo is not finite where g c1 overflows; s is 0 or 1
+// there, and the product 0.)
+__device__ __forceinline__ float sigmoid(float g, const Glu &a) {
+    const float p = g * a.c1, lo = __builtin_amdgcn_fmed3f(fmaf(g, a.c2, fmaf(g, a.c1, -p)), -1.0f, 1.0f);
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(p));
+    return fmaf(fmaf(-s, s, s) * lo, -0.6931471805599453f, s);
+}
+// h = act(g, u): silu(g) u, or the clamped form of gpt-oss (cw_clamped_swiglu, without its biases)
+__device__ __forceinline__ float glu(float g, float u, const Glu &a) {
+    if (a.act == CW_ACT_SILU) return g * sigmoid(g, a) * u;
     // (comparisons rather than fminf: a NaN stays one)
-    g = g > limit ? limit : g;
-    u = u > limit ? limit : u < -limit ? -limit : u;
-    return (u + 1.0f) * (g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * (alpha * -LOG2E))));
+    g = g > a.limit ? a.limit : g;
+    u = u > a.limit ? a.limit : u < -a.limit ? -a.limit : u;
+    return (u + 1.0f) * (g * sigmoid(g, a));
 }
 
 // the larger of m and |v|'s bits: ordered as the magnitudes are, infinities and NaNs above all finite ones

@@ -21,8 +21,8 @@ struct I8MoeArgs {
     const float *ws[3], *bias[3];
     const uint8_t *x;
     const float *xs, *logits;
-    int E, K, H, I, T, norm, act;
-    float alpha, limit;
+    int E, K, H, I, T, norm;
+    Glu glu;
     int rbh, rbi, ldh;  // bytes of a row of H and of I codes, floats of a hidden row
     uint32_t *ids;
     float *wt, *h;
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few_gateup(I8MoeArgs a
             su = dot16(u[r][c], x[c], su);
         }
         const float gv = fmaf((float)wave_sum_i(sg), sx * sw[0][r], b[0][r]), uv = fmaf((float)wave_sum_i(su), sx * sw[1][r], b[1][r]);
-        if (lane == 0 && r0 + r < a.I) a.h[((int64_t)t * a.K + j) * a.ldh + r0 + r] = glu(gv, uv, a.act, a.alpha, a.limit);
+        if (lane == 0 && r0 + r < a.I) a.h[((int64_t)t * a.K + j) * a.ldh + r0 + r] = glu(gv, uv, a.glu);
     }
 }
 
@@ -335,8 +335,7 @@ __device__ __forceinline__ void finish_gateup(const I8MoeArgs &a, const I8Tile &
             float h[4];
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                h[i] = glu(fmaf((float)acc[mb][j][i], sx[mb] * sw[j][i], b[j][i]), fmaf((float)acc[mb][NB + j][i], sx[mb] * sw[NB + j][i], b[NB + j][i]),
-                           a.act, a.alpha, a.limit);
+                h[i] = glu(fmaf((float)acc[mb][j][i], sx[mb] * sw[j][i], b[j][i]), fmaf((float)acc[mb][NB + j][i], sx[mb] * sw[NB + j][i], b[NB + j][i]), a.glu);
             store_row<4>(a.h + (int64_t)(tl.pos0 + r) * a.ldh + n, a.I - n, h);
         }
     }
@@ -661,9 +660,7 @@ int cw_i8_moe_layer(const cw_i8_moe_desc *d, const int8_t *x, const float *x_sca
     a.I = d->inter;
     a.T = T;
     a.norm = d->norm;
-    a.act = d->act;
-    a.alpha = d->alpha;
-    a.limit = d->limit;
+    a.glu = glu_of(d->act, d->alpha, d->limit);
     a.rbh = (int)i8_row_bytes(a.H);
     a.rbi = (int)i8_row_bytes(a.I);
     a.ldh = (a.I + 3) & ~3;

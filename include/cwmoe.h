@@ -314,7 +314,8 @@ int cw_quantize_i8(int dtype, const void *x, int64_t ldx, int64_t rows, int64_t 
 
 /* The same of h = silu(g) * u, or of the clamped SwiGLU of cw_clamped_swiglu (without its biases,
  * which cw_i8_matmul adds): g and u are rows of width values, ld elements apart (the two halves of
- * one product's rows, or two matrices). h is computed in f32. */
+ * one product's rows, or two matrices). h is computed in f32, to 9 half steps of it (2^-24 each) while
+ * alpha |g| is below 87. */
 int cw_swiglu_i8(int dtype, const void *g, const void *u, int64_t ld, int64_t rows, int64_t width, int act, float alpha,
                  float limit, int8_t *q, float *scale, cw_stream_t stream);
 
