@@ -89,6 +89,11 @@ __device__ __forceinline__ uint32_t code(double y, double inv) {
 }
 __device__ __forceinline__ uint32_t codes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return a | b << 8 | c << 16 | d << 24; }
 
+// An integer sum times its two scales (sx sw: their product in 64 bits, exact), plus b. In 64 bits: a product of two f32 scales
+// leaves f32's normal range where the result does not (rows with a largest value of 2^-118 and weights' scales of 5e-4: four
+// digits lost; 0 * inf between large ones), in either order. Rounded once, to f32.
+__device__ __forceinline__ float scaled(int sum, double sxsw, float b) { return (float)fma((double)sum, sxsw, (double)b); }
+
 // The activation's constants: c1 + c2 = -alpha log2(e) in two f32 terms (alpha 1: silu).
 struct Glu {
     int act;

@@ -79,11 +79,18 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few_gateup(I8MoeArgs a
         x[c] = load16(a.x + (int64_t)t * a.rbh + off[c]);
         if (o >= a.rbh) x[c] = i32x4{0, 0, 0, 0};
     }
-    const float sx = a.xs[t];
+    const double sx = a.xs[t];
     __syncthreads();
     if (r0 >= a.I) return;
     const int64_t e = __builtin_amdgcn_readfirstlane((int)expert);
-    float sw[2][R], b[2][R];
+    // lane r < R scales row r0 + r
+    const int64_t mine = e * a.I + min(r0 + (lane & (R - 1)), a.I - 1);
+    float sw[2], b[2];
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+        sw[m] = a.ws[m][mine];
+        b[m] = a.bias[m] ? a.bias[m][mine] : 0.f;
+    }
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const int row = min(r0 + r, a.I - 1);
@@ -92,12 +99,8 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few_gateup(I8MoeArgs a
             g[r][c] = load16(a.w[0] + e * a.stride[0] + (int64_t)row * a.rbh + off[c]);
             u[r][c] = load16(a.w[1] + e * a.stride[1] + (int64_t)row * a.rbh + off[c]);
         }
-#pragma unroll
-        for (int m = 0; m < 2; m++) {
-            sw[m][r] = a.ws[m][e * a.I + row];
-            b[m][r] = a.bias[m] ? a.bias[m][e * a.I + row] : 0.f;
-        }
     }
+    int sum[2] = {0, 0};
 #pragma unroll
     for (int r = 0; r < R; r++) {
         int sg = 0, su = 0;
@@ -106,9 +109,13 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few_gateup(I8MoeArgs a
             sg = dot16(g[r][c], x[c], sg);
             su = dot16(u[r][c], x[c], su);
         }
-        const float gv = fmaf((float)wave_sum_i(sg), sx * sw[0][r], b[0][r]), uv = fmaf((float)wave_sum_i(su), sx * sw[1][r], b[1][r]);
-        if (lane == 0 && r0 + r < a.I) a.h[((int64_t)t * a.K + j) * a.ldh + r0 + r] = glu(gv, uv, a.glu);
+        sg = wave_sum_i(sg);
+        su = wave_sum_i(su);
+        sum[0] = lane == r ? sg : sum[0];
+        sum[1] = lane == r ? su : sum[1];
     }
+    const float h = glu(scaled(sum[0], sx * sw[0], b[0]), scaled(sum[1], sx * sw[1], b[1]), a.glu);
+    if (lane < R && r0 + lane < a.I) a.h[((int64_t)t * a.K + j) * a.ldh + r0 + lane] = h;
 }
 
 // Down and the weighted sum of a token: the block quantizes the token's K hidden rows into LDS (every block of
@@ -116,10 +123,11 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few_gateup(I8MoeArgs a
 // l + 64, ... of the K rows' codes laid end to end. The hidden rows are asked for before the weights: loads return in
 // order, and the codes are made while the weights come in.
 template <class T, int NC, int R>
-__global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 ? 4 : 1) void k_i8_few_down(I8MoeArgs a) {
+__global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 || R == 4 ? 4 : NC == 4 ? 6 : 8) void k_i8_few_down(I8MoeArgs a) {
     constexpr int NH = NC < 12 ? (NC + 1) / 2 : 6;  // pieces of a hidden row held in registers (the others are read twice)
     extern __shared__ __align__(16) uint8_t hq[];  // K rows of rbi codes
-    __shared__ float hs[32], coef[I8_FEW_WAVES * R][33];
+    __shared__ float hs[32];
+    __shared__ double coef[I8_FEW_WAVES * R][33];
     __shared__ uint32_t top[I8_FEW_WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.y, cpr = a.rbi / 16;
     const int row0 = (blockIdx.x * I8_FEW_WAVES + wave) * R;
@@ -143,14 +151,15 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 ? 4 : 1) void k_i8_few_d
 #pragma unroll
         for (int r = 0; r < R; r++) w[r][c] = load16(p + (int64_t)min(row0 + r, a.H - 1) * a.rbi);
     }
-    // lane j < K: the scale of the pick's output channel, and what its bias adds
+    // lane j < K: the pick's weight, the scale of its output channel and its bias
+    const int mine = min(lane, a.K - 1);
+    const float wj = wt[mine];
     float sd[R], b[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        const int j = min(lane, a.K - 1);
-        const int64_t n = (int64_t)ids[j] * a.H + min(row0 + r, a.H - 1);
-        sd[r] = wt[j] * a.ws[2][n];
-        b[r] = a.bias[2] && lane < a.K ? wt[j] * a.bias[2][n] : 0.f;
+        const int64_t n = (int64_t)ids[mine] * a.H + min(row0 + r, a.H - 1);
+        sd[r] = a.ws[2][n];
+        b[r] = a.bias[2] && lane < a.K ? a.bias[2][n] : 0.f;
     }
     for (int j0 = 0; j0 < a.K; j0 += I8_FEW_WAVES / wpp) {
         const int j = j0 + wave / wpp;
@@ -194,23 +203,23 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 ? 4 : 1) void k_i8_few_d
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < R; r++)
-        if (lane < a.K) coef[wave * R + r][lane] = sd[r] * hs[lane];  // (read by this wave alone)
+        if (lane < a.K) coef[wave * R + r][lane] = (double)wj * sd[r] * hs[lane];  // (read by this wave alone; in 64 bits as in scaled())
     if (row0 >= a.H) return;
-    float acc[R];
+    double acc[R];
 #pragma unroll
-    for (int r = 0; r < R; r++) acc[r] = b[r];
+    for (int r = 0; r < R; r++) acc[r] = (double)wj * b[r];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
         const int i = lane + 64 * c;
         if (i < a.K * cpr) {
             const i32x4 x = *(const i32x4 *)(hq + 16 * i);
 #pragma unroll
-            for (int r = 0; r < R; r++) acc[r] = fmaf((float)dot16(w[r][c], x, 0), coef[wave * R + r][(picks[c / 4] >> (8 * (c % 4))) & 0xFF], acc[r]);
+            for (int r = 0; r < R; r++) acc[r] = fma((double)dot16(w[r][c], x, 0), coef[wave * R + r][(picks[c / 4] >> (8 * (c % 4))) & 0xFF], acc[r]);
         }
     }
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        const float v = wave_sum(acc[r]);
+        const float v = (float)wave_sum_d(acc[r]);
         if (lane == 0 && row0 + r < a.H) ((T *)a.out)[(int64_t)t * a.H + row0 + r] = from_f32<T>(v);
     }
 }
@@ -335,7 +344,8 @@ __device__ __forceinline__ void finish_gateup(const I8MoeArgs &a, const I8Tile &
             float h[4];
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                h[i] = glu(fmaf((float)acc[mb][j][i], sx[mb] * sw[j][i], b[j][i]), fmaf((float)acc[mb][NB + j][i], sx[mb] * sw[NB + j][i], b[NB + j][i]), a.glu);
+                h[i] = glu(scaled(acc[mb][j][i], (double)sx[mb] * sw[j][i], b[j][i]),
+                           scaled(acc[mb][NB + j][i], (double)sx[mb] * sw[NB + j][i], b[NB + j][i]), a.glu);
             store_row<4>(a.h + (int64_t)(tl.pos0 + r) * a.ldh + n, a.I - n, h);
         }
     }
@@ -366,7 +376,7 @@ __device__ __forceinline__ void finish_down(const I8MoeArgs &a, const I8Tile &tl
             if (n >= a.H) continue;
             float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = (float)acc[mb][j][i] * (sx[mb] * sw[j][i]);
+            for (int i = 0; i < 4; i++) v[i] = scaled(acc[mb][j][i], (double)sx[mb] * sw[j][i], 0.f);
             store_row<4>(d + n, a.H - n, v);
         }
     }

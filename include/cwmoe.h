@@ -330,9 +330,10 @@ int cw_rmsnorm_i8(int dtype, const void *x, int64_t ldx, const void *residual, i
 int cw_dequantize_i8(const int8_t *q, const float *scale, int64_t rows, int64_t k, int dtype, void *out,
                      cw_stream_t stream);
 
-/* y[r][c] = x_scale[r] * w_scale[c] * sum_k x[r][k] w[c][k] (+ bias[c], f32, may be NULL), rounded
- * once to ydtype; W is n rows of k codes, x m rows; rows of y are ldy elements apart. CW_ENOTSUP
- * for n above 2^26 and for products of 2^22 tiles (256 x 256 at most, about 2.7e11 outputs). */
+/* y[r][c] = x_scale[r] * w_scale[c] * sum_k x[r][k] w[c][k] (+ bias[c], f32, may be NULL),
+ * exact but for three roundings to f32 and the one to ydtype, whatever the scales' exponents; W is n
+ * rows of k codes, x m rows; rows of y are ldy elements apart. CW_ENOTSUP for n above 2^26 and for
+ * products of 2^22 tiles (256 x 256 at most, about 2.7e11 outputs). */
 int cw_i8_matmul(const int8_t *w, const float *w_scale, int64_t n, int64_t k, const int8_t *x, const float *x_scale,
                  int64_t m, const float *bias, int ydtype, void *y, int64_t ldy, cw_stream_t stream);
 
@@ -353,7 +354,7 @@ typedef struct cw_i8_moe_desc {
 
 /* out[T][hidden] = cw_moe_layer's contract on 8-bit rows: route the logits (cw_route_topk), gate
  * and up of the picked experts, the activation in f32, the hidden row of each pick quantized as
- * cw_quantize_i8 does, down, the weighted sum in f32, rounded once to ydtype. ids_out / w_out
+ * cw_quantize_i8 does, down, the weighted sum in f32 or more, rounded once to ydtype. ids_out / w_out
  * (T x K, may be NULL) receive the routing. A few tokens run as two launches. ws: 256-byte aligned,
  * of cw_i8_moe_workspace_size bytes, any contents; calls that overlap in time need distinct ones.
  * CW_ENOTSUP where T x top_k reaches 2^28, where the T rows of x reach 4 GiB, and where a launch
