@@ -315,19 +315,28 @@ struct I8TileTime {
     double some_b, some_s, all_b, all_s;
 };
 constexpr I8TileTime I8_TILES[4] = {{64, 64, 2.4, 1.45, 3.0, 1.6}, {64, 128, 3.4, 2.15, 4.0, 2.4}, {128, 128, 4.2, 3.2, 5.5, 4.3}, {256, 256, 12, 8, 15, 11.9}};
+constexpr int64_t I8_MAX_TILES = 1 << 22;  // (a launch holds fewer than 2^32 threads, 512 of a tile at most)
+// (-1: every tile's count exceeds the launch)
 static int i8_pick_tile(int64_t m, int64_t n, int rb, int cus) {
-    int best = 0;
+    int best = -1;
     double least = 0;
     for (int i = 0; i < 4; i++) {
         const I8TileTime &t = I8_TILES[i];
         const int64_t blocks = (m + t.tm - 1) / t.tm * ((n + t.tn - 1) / t.tn);
+        if (blocks >= I8_MAX_TILES) continue;
         const double k = rb / 1024.0, us = (double)(blocks / cus) * (t.all_b + t.all_s * k) + (blocks % cus ? t.some_b + t.some_s * k : 0.0);
-        if (i == 0 || us < least) {
+        if (best < 0 || us < least) {
             best = i;
             least = us;
         }
     }
     return best;
+}
+// Groups of 16 rows of x that k_i8_few takes (0: tiles). Measured, few rows / 64 x 64 tiles: 16 rows of 4096 x 4096 6.3 / 9.8 us,
+// of 8192 x 8192 21.0 / 22.1; 32 rows 8.8 / 10.3 and 30.8 / 23.9 (each block reads all of x); 64 rows of 1024 x 1024 4.8 / 5.3, of
+// 2048 x 2048 7.3 / 6.9.
+static int i8_few_groups(int64_t m, int64_t n, int rb) {
+    return m <= 16 ? 1 : m <= 32 && n * rb <= 1 << 24 ? 2 : m <= 64 && n * rb <= 1 << 21 ? 4 : 0;
 }
 
 // dynamic LDS above 64 KB, opted into once per kernel and device
@@ -343,28 +352,24 @@ static int i8_allow_lds(const void *kernel, int i, int lds) {
 }
 
 template <class T>
-static int i8_matmul(const I8MatArgs &a, hipStream_t s) {
+static int i8_matmul(const I8MatArgs &a, int few_groups, int tile_of, hipStream_t s) {
     auto few = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)((a.n + 15) / 16)), dim3(64 * I8_FEW_WAVES), 0, s, a);
         return check_launch("k_i8_few");
     };
-    auto tile = [&](auto kernel, int i, int threads, int lds) {
-        const int64_t tm = (a.m + I8_TILES[i].tm - 1) / I8_TILES[i].tm, tn = (a.n + I8_TILES[i].tn - 1) / I8_TILES[i].tn;
-        if (tm * tn >= 1 << 22) return set_error(CW_ENOTSUP, "i8_matmul: %lld x %lld outputs", (long long)a.m, (long long)a.n);
-        if (int rc = i8_allow_lds<T>((const void *)kernel, i, lds)) return rc;
+    auto tile = [&](auto kernel, int threads, int lds) {
+        const I8TileTime &t = I8_TILES[tile_of];
+        const int64_t tm = (a.m + t.tm - 1) / t.tm, tn = (a.n + t.tn - 1) / t.tn;
+        if (int rc = i8_allow_lds<T>((const void *)kernel, tile_of, lds)) return rc;
         hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(threads), lds, s, a, (int)tm, (int)tn);
         return check_launch("k_i8_tile");
     };
-    // Measured, few rows / 64 x 64 tiles: 16 rows of 4096 x 4096 6.3 / 9.8 us, of 8192 x 8192 21.0 / 22.1; 32 rows 8.8 / 10.3
-    // and 30.8 / 23.9 (each block reads all of x); 64 rows of 1024 x 1024 4.8 / 5.3, of 2048 x 2048 7.3 / 6.9.
-    if (a.m <= 16) return few(k_i8_few<T, 1>);
-    if (a.m <= 32 && a.n * a.rb <= 1 << 24) return few(k_i8_few<T, 2>);
-    if (a.m <= 64 && a.n * a.rb <= 1 << 21) return few(k_i8_few<T, 4>);
-    switch (i8_pick_tile(a.m, a.n, a.rb, (int)resident_blocks(1))) {
-    case 0: return tile(k_i8_ring<T, 2, 2>, 0, 512, I8Ring<2, 2>::LDS);
-    case 1: return tile(k_i8_ring<T, 2, 4>, 1, 512, I8Ring<2, 4>::LDS);
-    case 2: return tile(k_i8_ring<T, 4, 4>, 2, 512, I8Ring<4, 4>::LDS);
-    default: return tile(k_i8_big<T>, 3, 256, 2 * I8_BIG_STAGE);
+    if (few_groups) return few_groups == 1 ? few(k_i8_few<T, 1>) : few_groups == 2 ? few(k_i8_few<T, 2>) : few(k_i8_few<T, 4>);
+    switch (tile_of) {
+    case 0: return tile(k_i8_ring<T, 2, 2>, 512, I8Ring<2, 2>::LDS);
+    case 1: return tile(k_i8_ring<T, 2, 4>, 512, I8Ring<2, 4>::LDS);
+    case 2: return tile(k_i8_ring<T, 4, 4>, 512, I8Ring<4, 4>::LDS);
+    default: return tile(k_i8_big<T>, 256, 2 * I8_BIG_STAGE);
     }
 }
 
@@ -383,6 +388,8 @@ int cw_i8_matmul(const int8_t *w, const float *w_scale, int64_t n, int64_t k, co
     if (n > 1 << 26) return set_error(CW_ENOTSUP, "i8_matmul: %lld rows of w above %d", (long long)n, 1 << 26);
     CW_REQUIRE(ldy >= n, "i8_matmul: rows of y of %lld %lld apart", (long long)n, (long long)ldy);
     if (m == 0) return CW_OK;
+    const int rb = (int)i8_row_bytes(k), few_groups = i8_few_groups(m, n, rb), tile = few_groups ? 0 : i8_pick_tile(m, n, rb, (int)resident_blocks(1));
+    if (tile < 0) return set_error(CW_ENOTSUP, "i8_matmul: %lld x %lld outputs", (long long)m, (long long)n);
     CW_REQUIRE(w && w_scale && x && x_scale && y, "i8_matmul: null pointer");
     CW_REQUIRE(i8_aligned(w, 16) && i8_aligned(x, 16), "i8_matmul: codes must be 16-byte aligned");
     I8MatArgs a = {};
@@ -393,13 +400,13 @@ int cw_i8_matmul(const int8_t *w, const float *w_scale, int64_t n, int64_t k, co
     a.bias = bias;
     a.n = n;
     a.m = m;
-    a.rb = (int)i8_row_bytes(k);
+    a.rb = rb;
     a.y = y;
     a.ldy = ldy;
     hipStream_t s = (hipStream_t)stream;
-    if (ydtype == CW_F16) return i8_matmul<_Float16>(a, s);
-    if (ydtype == CW_BF16) return i8_matmul<bf16_t>(a, s);
-    return i8_matmul<float>(a, s);
+    if (ydtype == CW_F16) return i8_matmul<_Float16>(a, few_groups, tile, s);
+    if (ydtype == CW_BF16) return i8_matmul<bf16_t>(a, few_groups, tile, s);
+    return i8_matmul<float>(a, few_groups, tile, s);
 }
 
 }  // extern "C"
