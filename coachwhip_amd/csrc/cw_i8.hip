@@ -25,8 +25,8 @@ struct RowsArgs {
 // 8 (t + c TPR)..): one pass over the inputs. a = max|y|, scale = a / 127 rounded to f32, code =
 // y * 127 / a to the nearest. The norm's mean, factor and products and every code are computed in 64 bits,
 // whose vector rate here is half that of 32: a code does not depend on the order of a sum, and the kernel
-// stays bound by its bytes. A row with a value that is not finite gets the scale NaN and zero codes; a row
-// of zeros the scale 0. 8,192 rows, bf16: norm of 4,096 50 us (4.7 TB/s), SwiGLU of 2,880 29 (4.0; about 30 vector
+// stays bound by its bytes. A row with a value that is not finite, or whose scale would not be, gets the scale NaN and
+// zero codes; a row of zeros the scale 0. 8,192 rows, bf16: norm of 4,096 50 us (4.7 TB/s), SwiGLU of 2,880 29 (4.0; about 30 vector
 // operations a value beside the loads).
 template <class T, int MODE, int TPR, int NCH>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_rows_i8(RowsArgs a) {
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_rows_i8(RowsArgs a) {
 #pragma unroll
         for (int w = 0; w < WPR; w++) m = fmax(m, red[1][w]);
     }
-    const bool codes = m > 0.0 && m < INFINITY;
+    const bool fine = m <= 127.0 * (double)__FLT_MAX__, codes = fine && m > 0.0;  // (a norm's values may pass f32's, and so the scale)
     const double inv = codes ? 127.0 / m : 0.0;
     const int rb = (a.k + 127) / 128 * 128;
 #pragma unroll
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_rows_i8(RowsArgs a) {
         for (int i = 0; i < 8; i++) q[i] = codes ? code(y[c][i], inv) : 0u;
         *(uint2 *)(a.q + row * rb + e) = make_uint2(codes4(q[0], q[1], q[2], q[3]), codes4(q[4], q[5], q[6], q[7]));
     }
-    if (tid == 0) a.scale[row] = m < INFINITY ? (float)(m / 127.0) : __int_as_float(0x7fc00000);
+    if (tid == 0) a.scale[row] = fine ? (float)(m / 127.0) : __int_as_float(0x7fc00000);
 }
 
 template <class T, int MODE>

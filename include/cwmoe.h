@@ -320,7 +320,8 @@ int cw_swiglu_i8(int dtype, const void *g, const void *u, int64_t ld, int64_t ro
                  float limit, int8_t *q, float *scale, cw_stream_t stream);
 
 /* The same of y = h * weight / sqrt(mean(h^2) + eps), h = x + residual rounded to dtype (h = x
- * without a residual), in 64 bits: the codes do not depend on the order of a sum. sum (rows of k,
+ * without a residual), in 64 bits: the codes do not depend on the order of a sum. A row
+ * with a value above 127 times f32's largest gets the scale NaN and zero codes too. sum (rows of k,
  * may be NULL, and may be x or residual themselves where their rows are k apart) receives h,
  * y (f32, rows of k, may be NULL) the values before quantizing, which cw_router_logits reads. */
 int cw_rmsnorm_i8(int dtype, const void *x, int64_t ldx, const void *residual, int64_t ldr, const float *weight, float eps,
