@@ -167,6 +167,8 @@ def rmsnorm_i8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Opti
     (``ops.router_logits`` reads them)."""
     ldx = _floats(x, "x")
     rows, k = x.shape
+    if weight is None:
+        _fail("rmsnorm_i8: a weight of %d values", k)
     _vector(weight, k, "weight")
     ldr, total, y = 0, None, None
     if residual is not None:
