@@ -149,8 +149,10 @@ static int rows_launch(RowsArgs a, hipStream_t s) {
     // 5.6; 8,192 of 4,096 256 threads 48.5 / 34.9 / 19.2, 128 53.3 / 39.1 / 21.5, 512 57.3 / 39.1 / 21.8; one row of 2,048 256
     // threads 2.9 / 2.9 / 2.4, 64 4.8 / 5.6 / 2.8. Rows of 257 to 384 pieces, for which 256 threads take two pieces each: 8,192 of
     // 2,880 128 threads 35.2 / 29.4 / 15.0, 256 40.6 / 31.3 / 14.6; 301 of them 5.9 / 5.6 / 3.4 and 5.1 / 4.7 / 3.1.
-    if (MODE != ROWS_PLAIN && a.rows >= 2048 && chunks > 256) {
-        CW_ROWS(128, 3)
+    if constexpr (MODE != ROWS_PLAIN) {
+        if (a.rows >= 2048 && chunks > 256) {
+            CW_ROWS(128, 3)
+        }
     }
     CW_ROWS(64, 1) CW_ROWS(64, 2) CW_ROWS(256, 1) CW_ROWS(256, 2) CW_ROWS(256, 4) CW_ROWS(1024, 2) CW_ROWS(1024, 4)
 #undef CW_ROWS

@@ -229,12 +229,13 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 || R == 4 ? 4 : NC == 4 
 
 // One block: the picks counted by expert in LDS, the experts' places and tiles from a scan, and the picks dealt out
 // (their order within a pile does not matter: each pick's outputs are computed by themselves), through LDS up to
-// I8_STAGED picks (scattered 4-byte stores from one CU cost a memory transaction each). ROUTE: of up to I8_PLAN_TOKENS
-// tokens, which its waves route first, every 16th token each: one launch less (9 tokens over 256 experts 9.8 -> 7 us; with
+// I8_STAGED picks (scattered 4-byte stores from one CU cost a memory transaction each). PER (a lane's logits) not 0: of up to
+// I8_PLAN_TOKENS tokens, which its waves route first, every 16th token each: one launch less (9 tokens over 256 experts 9.8 -> 7 us; with
 // more tokens the routing of a CU to each is faster).
 constexpr int I8_PLAN_TOKENS = 32, I8_STAGED = 12288;
-template <bool ROUTE, int PER>
+template <int PER>
 __global__ __launch_bounds__(1024) void k_i8_plan(I8MoeArgs a, int *pile_pick, int *pile_tok, I8Tile *tiles, int *n_tiles) {
+    constexpr bool ROUTE = PER > 0;
     __shared__ int cnt[1024], place[1024], sums[2][16], staged[I8_STAGED];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, picks = a.T * a.K;
     cnt[tid] = 0;
@@ -597,10 +598,10 @@ static int moe_layer(const cw_i8_moe_desc *d, I8MoeArgs a, int ydtype, const I8M
         return check_launch("k_i8_plan");
     };
     if (a.T <= I8_PLAN_TOKENS) {
-        rc = a.E <= 256 ? plan(k_i8_plan<true, 4>) : a.E <= 512 ? plan(k_i8_plan<true, 8>) : plan(k_i8_plan<true, 16>);
+        rc = a.E <= 256 ? plan(k_i8_plan<4>) : a.E <= 512 ? plan(k_i8_plan<8>) : plan(k_i8_plan<16>);
     } else {
         if ((rc = cw_route_topk(a.logits, a.T, a.E, a.K, a.norm, a.ids, a.wt, s))) return rc;
-        rc = plan(k_i8_plan<false, 4>);
+        rc = plan(k_i8_plan<0>);
     }
     if (rc) return rc;
     int8_t *hq = (int8_t *)(base + L.hq);
