@@ -2,6 +2,7 @@
 #include <atomic>
 
 #include "cw_i8.h"
+#include "cw_i8_rules.h"
 #include "cw_i8_tile.h"
 #include "cw_mfma.h"
 
@@ -257,7 +258,6 @@ __global__ __launch_bounds__(512, 2) void k_i8_ring(I8MatArgs a, int tiles_m, in
 // waves' sums meet in LDS: integers, so in any order the same. One row of 8192 x 8192: 15.0 us, 4.5 TB/s (16 waves, or
 // two to four steps' loads at a time: 15.0 to 18.8, fewer blocks fit a CU); 2048 x 2048: 3.4 us, of which the launch
 // and one round trip are most.
-constexpr int I8_FEW_WAVES = 8;
 template <class T, int MB>
 __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few(I8MatArgs a) {
     __shared__ i32x4 part[I8_FEW_WAVES][MB][64];
@@ -302,41 +302,6 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few(I8MatArgs a) {
 #pragma unroll
     for (int o = 1; o < I8_FEW_WAVES; o++) v += part[o][wave][lane];
     i8_store4<T>(a, m, n, v, sx, sw, b);
-}
-
-// The tile whose estimated time is the least. A CU runs one block of any of them; a round of blocks on every CU takes
-// b + s k / 1024 us, more than one on some of them (whose share of L2 and of the fabric is larger). Measured (4096 x
-// 4096; launch 2.5 us included), estimate / measured: 64 x 64 at 128 rows 10.7 / 10.7, 256 rows (every CU) 11.9 / 11.3,
-// 512 rows 21.3 / 21.5; 64 x 128 at 256 rows 14.5 / 14.6, 512 rows 16.1 / 16.1, 1,024 rows 29.7 / 32.2; 128 x 128 at
-// 512 rows 19.5 / 21.4, 1,024 rows 25.2 / 25.1, 2,048 rows 47.9 / 48.1; 256 x 256 at 2,048 rows 46.5 / 51.1, 4,096 rows
-// 65.1 / 65.1, 8,192 rows 128 / 131.
-struct I8TileTime {
-    int tm, tn;
-    double some_b, some_s, all_b, all_s;
-};
-constexpr I8TileTime I8_TILES[4] = {{64, 64, 2.4, 1.45, 3.0, 1.6}, {64, 128, 3.4, 2.15, 4.0, 2.4}, {128, 128, 4.2, 3.2, 5.5, 4.3}, {256, 256, 12, 8, 15, 11.9}};
-constexpr int64_t I8_MAX_TILES = 1 << 22;  // (a launch holds fewer than 2^32 threads, 512 of a tile at most)
-// (-1: every tile's count exceeds the launch)
-static int i8_pick_tile(int64_t m, int64_t n, int rb, int cus) {
-    int best = -1;
-    double least = 0;
-    for (int i = 0; i < 4; i++) {
-        const I8TileTime &t = I8_TILES[i];
-        const int64_t blocks = (m + t.tm - 1) / t.tm * ((n + t.tn - 1) / t.tn);
-        if (blocks >= I8_MAX_TILES) continue;
-        const double k = rb / 1024.0, us = (double)(blocks / cus) * (t.all_b + t.all_s * k) + (blocks % cus ? t.some_b + t.some_s * k : 0.0);
-        if (best < 0 || us < least) {
-            best = i;
-            least = us;
-        }
-    }
-    return best;
-}
-// Groups of 16 rows of x that k_i8_few takes (0: tiles). Measured, few rows / 64 x 64 tiles: 16 rows of 4096 x 4096 6.3 / 9.8 us,
-// of 8192 x 8192 21.0 / 22.1; 32 rows 8.8 / 10.3 and 30.8 / 23.9 (each block reads all of x); 64 rows of 1024 x 1024 4.8 / 5.3, of
-// 2048 x 2048 7.3 / 6.9.
-static int i8_few_groups(int64_t m, int64_t n, int rb) {
-    return m <= 16 ? 1 : m <= 32 && n * rb <= 1 << 24 ? 2 : m <= 64 && n * rb <= 1 << 21 ? 4 : 0;
 }
 
 // dynamic LDS above 64 KB, opted into once per kernel and device

@@ -1,9 +1,9 @@
 // A MoE layer of 8-bit integer experts on 8-bit integer rows (gfx950): two kernels for a few tokens, grouped
 // matrix products for many.
-#include <math.h>
 #include <algorithm>
 
 #include "cw_i8.h"
+#include "cw_i8_rules.h"
 #include "cw_i8_tile.h"
 #include "cw_mfma.h"
 
@@ -13,7 +13,6 @@ namespace cw {
 struct I8Tile {
     int expert, pos0, m, first, of;
 };
-constexpr int I8_TILE = 128;  // picks of a tile, at most
 
 struct I8MoeArgs {
     const uint8_t *w[3];
@@ -54,7 +53,6 @@ __device__ __forceinline__ int wave_sum_i(int v) {
 // ... of each row and of x. One wave routes the token for its block (every wave for itself: 16,384 times 2,500 cycles
 // for 8 tokens of 8 picks), no further than this pick; the last pick's first block, which goes all the way, stores the
 // routing.
-constexpr int I8_FEW_WAVES = 8;
 template <int PER, int NC, int R>
 __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few_gateup(I8MoeArgs a) {
     __shared__ uint32_t expert;
@@ -232,7 +230,7 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 || R == 4 ? 4 : NC == 4 
 // I8_STAGED picks (scattered 4-byte stores from one CU cost a memory transaction each). PER (a lane's logits) not 0: of up to
 // I8_PLAN_TOKENS tokens, which its waves route first, every 16th token each: one launch less (9 tokens over 256 experts 9.8 -> 7 us; with
 // more tokens the routing of a CU to each is faster).
-constexpr int I8_PLAN_TOKENS = 32, I8_STAGED = 12288;
+constexpr int I8_STAGED = 12288;
 template <int PER>
 __global__ __launch_bounds__(1024) void k_i8_plan(I8MoeArgs a, int *pile_pick, int *pile_tok, I8Tile *tiles, int *n_tiles) {
     constexpr bool ROUTE = PER > 0;
@@ -467,27 +465,12 @@ struct I8MoeLayout {
     bool few;
 };
 
-// Two launches read an expert once per pick, the grouped ones once per tile: about 15 us more for their launches, but
-// each byte once. The picks' reads beyond the distinct experts', E (1 - (1 - K / E)^T) on average, come in part from the
-// caches. Measured, two launches / grouped, and those bytes: 256 experts of 512 x 2,048, top-8, 16 tokens 69 / 96 us
-// (85 MB), 32 tokens 120 / 135 (299); 128 of 2,880 x 2,880, top-4, 6 tokens 124 / 133 (53), 8 tokens 157 / 165 (91),
-// 16 tokens 291 / 249 (330); 8 of 2,048 x 4,096, top-2, 6 tokens 47 / 49 (137), 8 tokens 55 / 51 (222); 512 of 512 x
-// 2,048, top-10, 32 tokens 182 / 182 (250).
-static bool few_path(const cw_i8_moe_desc *d, int T) {
-    const int64_t rbh = i8_row_bytes(d->hidden), rbi = i8_row_bytes(d->inter);
-    if (rbh > 4 * 1024 || d->top_k * rbi > 16 * 1024 || T > 1024) return false;
-    const double K = d->top_k, E = d->n_experts, picks = T * K, distinct = E * (1 - pow(1 - K / E, T));
-    return (picks - distinct) * (2.0 * d->inter * rbh + (double)d->hidden * rbi) <= 200e6;
-}
-
-static int64_t i8_max_tiles(int64_t picks, int experts) { return (picks + I8_TILE - 1) / I8_TILE + std::min<int64_t>(experts, picks); }
-
 static I8MoeLayout layout(const cw_i8_moe_desc *d, int T) {
     I8MoeLayout L = {};
     size_t off = 0;
     auto take = [&](size_t &at, size_t bytes) { at = off; off = (off + bytes + 255) & ~(size_t)255; };
     const size_t TK = (size_t)T * d->top_k;
-    L.few = few_path(d, T);
+    L.few = i8_few_tokens(d->n_experts, d->top_k, d->hidden, d->inter, T);
     take(L.ids, TK * 4);
     take(L.w, TK * 4);
     take(L.h, TK * ((d->inter + 3) & ~3) * 4);
@@ -527,66 +510,58 @@ static int check_desc(const cw_i8_moe_desc *d, int T) {
     return CW_OK;
 }
 
-// Rows a wave: more where that still leaves every CU four blocks (the routing and the rows' codes are made once a
-// block).
 template <class T, int NC>
 static int few_down(const I8MoeArgs &a, hipStream_t s) {
-    constexpr int MORE = NC <= 4 ? 4 : NC <= 8 ? 2 : 1;
-    const int64_t rows = (a.H + I8_FEW_WAVES - 1) / I8_FEW_WAVES, cus = resident_blocks(1);
-    auto go = [&](auto kernel, int r) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + r - 1) / r), a.T), dim3(64 * I8_FEW_WAVES), a.K * a.rbi, s, a);
+    const int r = i8_down_rows(NC, a.H, a.T, (int)resident_blocks(1));
+    auto go = [&](auto kernel) {
+        const int per = I8_FEW_WAVES * r;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.H + per - 1) / per), a.T), dim3(64 * I8_FEW_WAVES), a.K * a.rbi, s, a);
         return check_launch("k_i8_few_down");
     };
-    if (MORE == 4 && rows * a.T >= 16 * cus) return go(k_i8_few_down<T, NC, MORE>, MORE);
-    if (MORE >= 2 && rows * a.T >= 8 * cus) return go(k_i8_few_down<T, NC, MORE < 2 ? 1 : 2>, 2);
-    return go(k_i8_few_down<T, NC, 1>, 1);
+    if constexpr (NC <= 4)
+        if (r == 4) return go(k_i8_few_down<T, NC, 4>);
+    if constexpr (NC <= 8)
+        if (r == 2) return go(k_i8_few_down<T, NC, 2>);
+    return go(k_i8_few_down<T, NC, 1>);
 }
 template <class T>
 static int few_down(const I8MoeArgs &a, hipStream_t s) {
-    const int chunks = a.K * (a.rbi / 16);
-    if (chunks <= 64 * 1) return few_down<T, 1>(a, s);
-    if (chunks <= 64 * 2) return few_down<T, 2>(a, s);
-    if (chunks <= 64 * 4) return few_down<T, 4>(a, s);
-    if (chunks <= 64 * 8) return few_down<T, 8>(a, s);
-    if (chunks <= 64 * 12) return few_down<T, 12>(a, s);
-    if (chunks <= 64 * 16) return few_down<T, 16>(a, s);
-    return set_error(CW_ENOTSUP, "i8 moe: %d picks' rows of %d", a.K, a.I);
+    switch (i8_down_pieces(a.K, a.rbi)) {
+    case 1: return few_down<T, 1>(a, s);
+    case 2: return few_down<T, 2>(a, s);
+    case 4: return few_down<T, 4>(a, s);
+    case 8: return few_down<T, 8>(a, s);
+    case 12: return few_down<T, 12>(a, s);
+    default: return few_down<T, 16>(a, s);
+    }
 }
 template <int PER, int NC>
 static int few_gateup(const I8MoeArgs &a, hipStream_t s) {
-    constexpr int MORE = NC <= 2 ? 4 : 2;
-    const int64_t rows = (a.I + I8_FEW_WAVES - 1) / I8_FEW_WAVES, cus = resident_blocks(1);
-    auto go = [&](auto kernel, int r) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + r - 1) / r), a.K, a.T), dim3(64 * I8_FEW_WAVES), 0, s, a);
+    const int r = i8_gateup_rows(NC, a.I, a.T * a.K, (int)resident_blocks(1));
+    auto go = [&](auto kernel) {
+        const int per = I8_FEW_WAVES * r;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.I + per - 1) / per), a.K, a.T), dim3(64 * I8_FEW_WAVES), 0, s, a);
         return check_launch("k_i8_few_gateup");
     };
-    if (MORE == 4 && rows * a.T * a.K >= 16 * cus) return go(k_i8_few_gateup<PER, NC, MORE>, MORE);
-    if (rows * a.T * a.K >= 2 * cus) return go(k_i8_few_gateup<PER, NC, 2>, 2);
-    return go(k_i8_few_gateup<PER, NC, 1>, 1);
+    if constexpr (NC <= 2)
+        if (r == 4) return go(k_i8_few_gateup<PER, NC, 4>);
+    return r == 2 ? go(k_i8_few_gateup<PER, NC, 2>) : go(k_i8_few_gateup<PER, NC, 1>);
 }
 template <int PER>
 static int few_gateup(const I8MoeArgs &a, hipStream_t s) {
-    if (a.rbh <= 1024) return few_gateup<PER, 1>(a, s);
-    if (a.rbh <= 2048) return few_gateup<PER, 2>(a, s);
-    if (a.rbh <= 1024 * 3) return few_gateup<PER, 3>(a, s);
-    if (a.rbh <= 4096) return few_gateup<PER, 4>(a, s);
-    return set_error(CW_ENOTSUP, "i8 moe: rows of %d", a.H);
-}
-
-// Four groups of weight rows a wave instead of two, where the picks share the weights and there are blocks for every CU
-// twice. Measured, two / four groups: 128 experts of 2,880 x 2,880, top-4, 64 tokens (2 picks an expert) 525 / 544 us,
-// 512 tokens (16) 662 / 660, 2,048 tokens (64) 823 / 803; 256 of 512 x 2,048, top-8, 512 tokens (16) 213 / 204; 64 of
-// 1,408 x 2,048, top-6, 2,048 tokens (192) 316 / 281; 16 of 2,880 x 4,096, top-2, 512 tokens (64, 368 blocks) 160 / 165,
-// 2,048 tokens (256, 736 blocks) 360 / 318.
-static bool many_picks(const I8MoeArgs &a) {
-    const double picks = (double)a.T * a.K, avg = picks / a.E;
-    return avg >= 12 && a.E * ceil(avg / I8_TILE) * ((a.I + 127) / 128) >= 2 * resident_blocks(1);
+    switch (i8_gateup_pieces(a.rbh)) {
+    case 1: return few_gateup<PER, 1>(a, s);
+    case 2: return few_gateup<PER, 2>(a, s);
+    case 3: return few_gateup<PER, 3>(a, s);
+    default: return few_gateup<PER, 4>(a, s);
+    }
 }
 
 static int moe_layer(const cw_i8_moe_desc *d, I8MoeArgs a, int ydtype, const I8MoeLayout &L, uint8_t *base, hipStream_t s) {
     int rc;
     if (L.few) {
-        rc = a.E <= 256 ? few_gateup<4>(a, s) : a.E <= 512 ? few_gateup<8>(a, s) : few_gateup<16>(a, s);
+        const int per = i8_route_width(a.E);
+        rc = per == 4 ? few_gateup<4>(a, s) : per == 8 ? few_gateup<8>(a, s) : few_gateup<16>(a, s);
         if (rc) return rc;
         return ydtype == CW_F16 ? few_down<_Float16>(a, s) : ydtype == CW_BF16 ? few_down<bf16_t>(a, s) : few_down<float>(a, s);
     }
@@ -598,7 +573,8 @@ static int moe_layer(const cw_i8_moe_desc *d, I8MoeArgs a, int ydtype, const I8M
         return check_launch("k_i8_plan");
     };
     if (a.T <= I8_PLAN_TOKENS) {
-        rc = a.E <= 256 ? plan(k_i8_plan<4>) : a.E <= 512 ? plan(k_i8_plan<8>) : plan(k_i8_plan<16>);
+        const int per = i8_route_width(a.E);
+        rc = per == 4 ? plan(k_i8_plan<4>) : per == 8 ? plan(k_i8_plan<8>) : plan(k_i8_plan<16>);
     } else {
         if ((rc = cw_route_topk(a.logits, a.T, a.E, a.K, a.norm, a.ids, a.wt, s))) return rc;
         rc = plan(k_i8_plan<0>);
@@ -619,7 +595,7 @@ static int moe_layer(const cw_i8_moe_desc *d, I8MoeArgs a, int ydtype, const I8M
         hipLaunchKernelGGL(kernel, dim3((unsigned)((tmax * blocks + 7) / 8 * 8)), dim3(256), LDS, s, a, blocks);
         return check_launch("k_i8_moe_stream");
     };
-    const bool many = many_picks(a);
+    const bool many = i8_many_picks(a.E, a.K, a.I, a.T, (int)resident_blocks(1));
     rc = many ? product(k_i8_moe_stream<false, 4>, 4, false) : product(k_i8_moe_stream<false, 2>, 2, false);
     if (rc) return rc;
     if ((rc = i8_quantize_f32(a.h, TK, a.I, a.ldh, hq, hs, s))) return rc;

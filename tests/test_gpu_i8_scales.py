@@ -10,7 +10,8 @@ from .test_gpu_i8 import DTYPES, U, gen, half, rand_rows, randn, say
 pytestmark = pytest.mark.gpu
 
 # every kernel of the products: few rows (16, 32, 64), the rings (64 x 64, 64 x 128, 128 x 128) and 256 x 256
-SHAPES = [(1, 100, 300), (3, 40, 1000), (20, 300, 640), (50, 300, 640), (129, 255, 896), (300, 1500, 1500), (512, 4001, 1500), (5000, 3001, 897), (8200, 8200, 100)]
+SHAPES = [(1, 100, 300), (3, 40, 1000), (20, 300, 640), (50, 300, 640), (129, 255, 896), (300, 1500, 1500), (512, 4001, 1500), (700, 4096, 640), (5000, 3001, 897),
+          (8200, 8200, 100)]
 
 
 def check(y, p, bias, dtype):
