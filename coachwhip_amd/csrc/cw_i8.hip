@@ -26,8 +26,8 @@ struct RowsArgs {
 // y * 127 / a to the nearest. The norm's mean, factor and products and every code are computed in 64 bits,
 // whose vector rate here is half that of 32: a code does not depend on the order of a sum, and the kernel
 // stays bound by its bytes. A row with a value that is not finite, or whose scale would not be, gets the scale NaN and
-// zero codes; a row of zeros the scale 0. 8,192 rows, bf16: norm of 4,096 50 us (4.7 TB/s), SwiGLU of 2,880 29 (4.0; about 30 vector
-// operations a value beside the loads).
+// zero codes; a row of zeros the scale 0. 8,192 rows, bf16: norm of 4,096 50 us (4.7 TB/s), SwiGLU of 2,880 30 (3.9; about 38 vector
+// operations a value).
 template <class T, int MODE, int TPR, int NCH>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_rows_i8(RowsArgs a) {
     constexpr int NT = TPR == 64 ? 256 : TPR, RPB = NT / TPR, WPR = TPR / 64;
@@ -147,8 +147,11 @@ static int rows_launch(RowsArgs a, hipStream_t s) {
     }
     // Threads a row, measured with bf16, norm / SwiGLU / plain, us: 8,192 rows of 512 64 threads 8.9 / 7.5 / 4.6, 128 12.6 / 8.6 /
     // 5.6; 8,192 of 4,096 256 threads 48.5 / 34.9 / 19.2, 128 53.3 / 39.1 / 21.5, 512 57.3 / 39.1 / 21.8; one row of 2,048 256
-    // threads 2.9 / 2.9 / 2.4, 64 4.8 / 5.6 / 2.8. Rows of 257 to 384 pieces, for which 256 threads take two pieces each: 8,192 of
-    // 2,880 128 threads 35.2 / 29.4 / 15.0, 256 40.6 / 31.3 / 14.6; 301 of them 5.9 / 5.6 / 3.4 and 5.1 / 4.7 / 3.1.
+    // threads 2.9 / 2.9 / 2.4, 64 4.8 / 5.6 / 2.8. Rows of 257 to 384 pieces, for which 256 threads take two pieces each and leave
+    // up to half of them empty, norm / SwiGLU with 128 threads and with 256, bf16: 2,176 columns 8,192 rows 30.5 / 26.4 and 35.0 /
+    // 28.6, 2,048 rows 10.3 / 9.3 and 12.4 / 10.2, 1,024 rows 7.2 / 7.6 and 7.3 / 6.8, 301 rows 6.1 / 6.2 and 5.2 / 5.0; 3,040 columns
+    // 37.3 / 31.6 and 41.1 / 33.3, 11.3 / 10.1 and 13.4 / 11.3, 7.9 / 7.9 and 8.0 / 7.4, 6.0 / 5.9 and 5.2 / 5.0; 2,560 and 2,880 and f16
+    // alike. f32 is bound by its bytes: within 3 % either way from 4,096 rows, 128 threads 7 to 11 % faster (norm) at 2,048.
     if constexpr (MODE != ROWS_PLAIN) {
         if (a.rows >= 2048 && chunks > 256) {
             CW_ROWS(128, 3)

@@ -227,9 +227,9 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 || R == 4 ? 4 : NC == 4 
 
 // One block: the picks counted by expert in LDS, the experts' places and tiles from a scan, and the picks dealt out
 // (their order within a pile does not matter: each pick's outputs are computed by themselves), through LDS up to
-// I8_STAGED picks (scattered 4-byte stores from one CU cost a memory transaction each). PER (a lane's logits) not 0: of up to
-// I8_PLAN_TOKENS tokens, which its waves route first, every 16th token each: one launch less (9 tokens over 256 experts 9.8 -> 7 us; with
-// more tokens the routing of a CU to each is faster).
+// I8_STAGED picks (scattered 4-byte stores from one CU cost a memory transaction each). 8,192 picks 6.2 us, 12,288 8.2, 12,800
+// 17.1, 16,384 20.7. PER (a lane's logits) not 0: of up to I8_PLAN_TOKENS tokens, which its waves route first, every 16th token
+// each: one launch less (9 tokens over 256 experts 9.8 -> 7 us; with more tokens the routing of a CU to each is faster).
 constexpr int I8_STAGED = 12288;
 template <int PER>
 __global__ __launch_bounds__(1024) void k_i8_plan(I8MoeArgs a, int *pile_pick, int *pile_tok, I8Tile *tiles, int *n_tiles) {
@@ -398,8 +398,9 @@ __device__ __forceinline__ bool item_of_block(const I8MoeArgs &a, int n_blocks, 
 }
 
 // A wave multiplies a tile's picks with 8 NW rows of gate and of up, or 16 NW of down. 2,048 tokens over 128 experts of
-// 2,880 x 2,880: gate and up 491 us, down 257, 4.35 TB/s of weights, which bound it, beside the f32 rows it writes (gate
-// and up without their stores: 411).
+// 2,880 x 2,880: gate and up 489 us, down 258, 4.35 TB/s of weights, beside the f32 rows it writes (gate and up without
+// their stores: 411). With many picks an expert its waves wait to issue: 61 % of their cycles over 8 experts of 2,048 x 4,096, at 42 %
+// of the integer rate, L2 read at 6.7 TB/s.
 template <bool DOWN, int MB, int NW>
 __device__ __forceinline__ void stream_tile(const I8MoeArgs &a, const I8Tile &tl, int n0, uint8_t *lds) {
     constexpr int NB = NW / 2;

@@ -12,11 +12,12 @@ namespace cw {
 constexpr int I8_FEW_WAVES = 8;  // waves of a block of the kernels for few rows and few tokens
 
 // The tile whose estimated time is the least. A CU runs one block of any of them; a round of blocks on every CU takes
-// b + s k / 1024 us, more than one on some of them (whose share of L2 and of the fabric is larger). Measured (4096 x
-// 4096; launch 2.5 us included), estimate / measured: 64 x 64 at 128 rows 10.7 / 10.7, 256 rows (every CU) 11.9 / 11.3,
-// 512 rows 21.3 / 21.5; 64 x 128 at 256 rows 14.5 / 14.6, 512 rows 16.1 / 16.1, 1,024 rows 29.7 / 32.2; 128 x 128 at
-// 512 rows 19.5 / 21.4, 1,024 rows 25.2 / 25.1, 2,048 rows 47.9 / 48.1; 256 x 256 at 2,048 rows 46.5 / 51.1, 4,096 rows
-// 65.1 / 65.1, 8,192 rows 128 / 131.
+// b + s k / 1024 us, more than one on some of them (whose share of L2 and of the fabric is larger). Measured in a graph (4096 x
+// 4096 in bf16; launch 2.5 us included), estimate / measured: 64 x 64 at 128 rows 10.7 / 11.3, 256 rows (every CU) 11.9 / 11.8,
+// 512 rows 21.3 / 23.0; 64 x 128 at 256 rows 14.5 / 15.3, 512 rows 16.1 / 16.4, 1,024 rows 29.7 / 29.7; 128 x 128 at
+// 512 rows 19.5 / 22.2, 1,024 rows 25.2 / 23.6, 2,048 rows 47.9 / 46.5, 4,096 rows 93.3 / 89.3; 256 x 256 at 2,048 rows 46.5 /
+// 52.0, 4,096 rows 65.1 / 60.3, 8,192 rows 128 / 120. So the estimates are off by up to a tenth, and at 2,048 rows of that
+// matrix the slower tile is taken (52.0 instead of 46.5).
 struct I8TileTime {
     int tm, tn;
     double some_b, some_s, all_b, all_s;
@@ -39,9 +40,9 @@ inline int i8_pick_tile(int64_t m, int64_t n, int rb, int cus) {
     }
     return best;
 }
-// Groups of 16 rows of x that k_i8_few takes (0: tiles). Measured, few rows / 64 x 64 tiles: 16 rows of 4096 x 4096 6.3 / 9.8 us,
-// of 8192 x 8192 21.0 / 22.1; 32 rows 8.8 / 10.3 and 30.8 / 23.9 (each block reads all of x); 64 rows of 1024 x 1024 4.8 / 5.3, of
-// 2048 x 2048 7.3 / 6.9.
+// Groups of 16 rows of x that k_i8_few takes (0: tiles). Measured in a graph, few rows / 64 x 64 tiles: 16 rows of 4096 x 4096
+// 6.6 / 10.1 us, of 8192 x 8192 18.9 / 17.9; 32 rows 8.8 / 10.8 and 26.3 / 20.2 (each block reads all of x); 64 rows of 1024 x 1024
+// 4.9 / 5.7, of 2048 x 2048 7.2 / 7.2.
 inline int i8_few_groups(int64_t m, int64_t n, int rb) {
     return m <= 16 ? 1 : m <= 32 && n * rb <= 1 << 24 ? 2 : m <= 64 && n * rb <= 1 << 21 ? 4 : 0;
 }
@@ -57,10 +58,12 @@ inline int i8_route_width(int E) { return E <= 256 ? 4 : E <= 512 ? 8 : 16; }
 
 // Two launches read an expert once per pick, the grouped ones once per tile: about 15 us more for their launches, but
 // each byte once. The picks' reads beyond the distinct experts', E (1 - (1 - K / E)^T) on average, come in part from the
-// caches. Measured, two launches / grouped, and those bytes: 256 experts of 512 x 2,048, top-8, 16 tokens 69 / 96 us
-// (85 MB), 32 tokens 120 / 135 (299); 128 of 2,880 x 2,880, top-4, 6 tokens 124 / 133 (53), 8 tokens 157 / 165 (91),
-// 16 tokens 291 / 249 (330); 8 of 2,048 x 4,096, top-2, 6 tokens 47 / 49 (137), 8 tokens 55 / 51 (222); 512 of 512 x
-// 2,048, top-10, 32 tokens 182 / 182 (250).
+// caches. Measured in a graph, two launches / grouped, and those bytes: 256 experts of 512 x 2,048, top-8, 16 tokens 69 / 97 us
+// (82 MB), 32 tokens 121 / 136 (292); 128 of 2,880 x 2,880, top-4, 6 tokens 123 / 137 (46), 8 tokens 157 / 175 (84),
+// 16 tokens 290 / 264 (331); 8 of 2,048 x 4,096, top-2, 6 tokens 42 / 46 (137), 8 tokens 52 / 51 (222); 512 of 512 x
+// 2,048, top-10, 32 tokens 180 / 182 (253). Bytes alone do not decide: 32 tokens over the 256 small experts take the slower form.
+// The two launches hold a row of x in four pieces a lane and the K hidden rows in 16 KB: layers beyond that (hidden above 4,096;
+// top-2 with an inter of 14,336 and hidden 4,096: 118 us for one token, of 69 for its bytes) are grouped for any number of tokens.
 inline bool i8_few_tokens(int E_, int K_, int H, int I, int T) {
     const int64_t rbh = (H + 127) / 128 * 128, rbi = (I + 127) / 128 * 128;
     if (rbh > 4 * 1024 || K_ * rbi > 16 * 1024 || T > 1024) return false;
@@ -86,10 +89,10 @@ inline int i8_down_rows(int pieces, int H, int64_t T, int cus) {
 }
 
 // Four groups of weight rows a wave instead of two, where the picks share the weights and there are blocks for every CU
-// twice. Measured, two / four groups: 128 experts of 2,880 x 2,880, top-4, 64 tokens (2 picks an expert) 525 / 544 us,
-// 512 tokens (16) 662 / 660, 2,048 tokens (64) 823 / 803; 256 of 512 x 2,048, top-8, 512 tokens (16) 213 / 204; 64 of
-// 1,408 x 2,048, top-6, 2,048 tokens (192) 316 / 281; 16 of 2,880 x 4,096, top-2, 512 tokens (64, 368 blocks) 160 / 165,
-// 2,048 tokens (256, 736 blocks) 360 / 318.
+// twice. Measured in a graph, two / four groups: 128 experts of 2,880 x 2,880, top-4, 64 tokens (2 picks an expert) 533 / 551 us,
+// 512 tokens (16) 670 / 667, 2,048 tokens (64) 821 / 788; 256 of 512 x 2,048, top-8, 512 tokens (16) 212 / 200; 64 of
+// 1,408 x 2,048, top-6, 2,048 tokens (192) 306 / 273; 16 of 2,880 x 4,096, top-2, 512 tokens (64, 368 blocks) 168 / 177,
+// 2,048 tokens (256, 736 blocks) 346 / 312.
 inline bool i8_many_picks(int E, int K, int I, int T, int cus) {
     const double avg = (double)T * K / E;
     return avg >= 12 && E * ceil(avg / I8_TILE) * ((I + 127) / 128) >= 2 * cus;
