@@ -17,23 +17,38 @@ struct I8MatArgs {
     int64_t ldy;
 };
 
-// four outputs of row m from column n: sum * (sx sw) + bias. USUAL: in f32, where the product of the scales is a normal number
-template <class T, bool USUAL = false>
-__device__ __forceinline__ void i8_store4(const I8MatArgs &a, int64_t m, int64_t n, i32x4 v, double sx, const float (&sw)[4], const float (&b)[4]) {
+// The formula of an output, the same in every kernel, so that a row's results do not depend on the rows beside it, whose number
+// picks the kernel: in f32, fma(sum, sx sw, bias), where both scales are usual ones, zero or from 2^-63 to 2^63 (their product is
+// zero or a normal number), else in 64 bits. (For all in 64 bits 8,192 rows of 4096 x 4096 took 135 us in a graph instead of 126.)
+struct ScaleRange {
+    uint32_t least = ~0u, most = 0;
+    __device__ __forceinline__ void add(float s) {
+        const uint32_t u = __float_as_uint(s) & 0x7FFFFFFFu;
+        least = min(least, u - 1);  // (zero: the largest)
+        most = max(most, u);
+    }
+    __device__ __forceinline__ bool usual() const { return least >= (64u << 23) - 1 && most <= 190u << 23; }
+};
+// four outputs of row m from column n. USUAL: all their scales are
+template <class T, bool USUAL>
+__device__ __forceinline__ void i8_store4(const I8MatArgs &a, int64_t m, int64_t n, i32x4 v, float sx, const float (&sw)[4], const float (&b)[4]) {
     float f[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) f[i] = USUAL ? fmaf((float)v[i], (float)sx * sw[i], b[i]) : scaled(v[i], sx * sw[i], b[i]);
+    for (int i = 0; i < 4; i++) {
+        f[i] = fmaf((float)v[i], sx * sw[i], b[i]);
+        if constexpr (!USUAL) {
+            ScaleRange r;
+            r.add(sx);
+            r.add(sw[i]);
+            if (!r.usual()) f[i] = scaled(v[i], (double)sx * sw[i], b[i]);
+        }
+        asm("" : "+v"(f[i]));  // (in f32: some kernels would fuse the fma with f16's conversion, others not)
+    }
     store_row<4>((T *)a.y + m * a.ldy + n, a.n - n < 4 ? (int)(a.n - n) : 4, f);
-}
-// a scale from 2^-63 to 2^63, or zero: two of them have a product that f32 holds (zero, or from 2^-126 to 2^126)
-__device__ __forceinline__ bool usual_scale(float s) {
-    const float m = fabsf(s);
-    return s == 0.f || (m >= 0x1p-63f && m <= 0x1p63f);
 }
 
 // A wave's sums scaled and stored: rows of x from m0, of W from n0. All scales are loaded first, from clamped
-// places: loads inside the bounds checks would be waited for one after the other (32 us a tile of 256 x 256). In 64 bits; many
-// of them in f32 where all the wave's scales are usual ones (8,192 rows of 4096 x 4096 in a graph: 126 us, 135 with 64 bits).
+// places: loads inside the bounds checks would be waited for one after the other (32 us a tile of 256 x 256).
 template <class T, int MB, int NW>
 __device__ __forceinline__ void i8_finish(const I8MatArgs &a, int64_t m0, int64_t n0, const i32x4 (&acc)[MB][NW]) {
     const int lane = threadIdx.x & 63;
@@ -71,17 +86,15 @@ __device__ __forceinline__ void i8_finish(const I8MatArgs &a, int64_t m0, int64_
                 if (n + 16 * j < a.n) i8_store4<T, usual.value>(a, m + 16 * i, n + 16 * j, acc[i][j], sx[i], sw[j], b[j]);
         }
     };
-    if constexpr (MB * NW >= 64) {
-        bool usual = true;
+    ScaleRange r;
 #pragma unroll
-        for (int i = 0; i < MB; i++) usual &= usual_scale(sx[i]);
+    for (int i = 0; i < MB; i++) r.add(sx[i]);
 #pragma unroll
-        for (int j = 0; j < NW; j++)
+    for (int j = 0; j < NW; j++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) usual &= usual_scale(sw[j][c]);
-        if (__all(usual)) return store(std::true_type{});
-    }
-    store(std::false_type{});
+        for (int c = 0; c < 4; c++) r.add(sw[j][c]);
+    if (__all(r.usual())) store(std::true_type{});
+    else store(std::false_type{});
 }
 
 // Blocks go to the eight dies in turn: each die gets a contiguous range of tiles, in panels of four tiles of W, so that
@@ -287,7 +300,7 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few(I8MatArgs a) {
             for (int i = 0; i < MB; i++) acc[i] = mfma_i8(w[kk], x[i][kk], acc[i]);
     }
     const int64_t m = 16 * (wave % MB) + (lane & 15), n = n0 + 4 * (lane >> 4);
-    const double sx = a.xs[min(m, a.m - 1)];
+    const float sx = a.xs[min(m, a.m - 1)];
     float sw[4], b[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -301,7 +314,12 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few(I8MatArgs a) {
     i32x4 v = part[0][wave][lane];
 #pragma unroll
     for (int o = 1; o < I8_FEW_WAVES; o++) v += part[o][wave][lane];
-    i8_store4<T>(a, m, n, v, sx, sw, b);
+    ScaleRange r;
+    r.add(sx);
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.add(sw[i]);
+    if (__all(r.usual())) i8_store4<T, true>(a, m, n, v, sx, sw, b);
+    else i8_store4<T, false>(a, m, n, v, sx, sw, b);
 }
 
 // dynamic LDS above 64 KB, opted into once per kernel and device

@@ -332,9 +332,10 @@ int cw_dequantize_i8(const int8_t *q, const float *scale, int64_t rows, int64_t 
                      cw_stream_t stream);
 
 /* y[r][c] = x_scale[r] * w_scale[c] * sum_k x[r][k] w[c][k] (+ bias[c], f32, may be NULL),
- * exact but for three roundings to f32 and the one to ydtype, whatever the scales' exponents; W is n
- * rows of k codes, x m rows; rows of y are ldy elements apart. CW_ENOTSUP for n above 2^26 and for
- * results of 2^22 tiles of 256 x 256 or more (about 2.7e11 outputs). */
+ * exact but for three roundings to f32 and the one to ydtype, whatever the scales' exponents; a row's
+ * results do not depend on the other rows or on their number. W is n rows of k codes, x m rows; rows
+ * of y are ldy elements apart. CW_ENOTSUP for n above 2^26 and for results of 2^22 tiles of 256 x 256
+ * or more (about 2.7e11 outputs). */
 int cw_i8_matmul(const int8_t *w, const float *w_scale, int64_t n, int64_t k, const int8_t *x, const float *x_scale,
                  int64_t m, const float *bias, int ydtype, void *y, int64_t ldy, cw_stream_t stream);
 

@@ -9,6 +9,7 @@ from coachwhip_amd._lib import CW_EINVAL, CW_ENOTSUP
 
 from . import i8_rules as rules
 from .test_gpu_i8 import MM_SHAPES
+from .test_gpu_i8_batch import BATCHES, K, N
 from .test_gpu_i8_instances import DOWN, GATEUP, GROUPED, all_counts
 from .test_gpu_i8_scales import SHAPES as SCALE_SHAPES
 
@@ -60,3 +61,8 @@ def test_every_kernel_of_many_tokens_is_tested():
     ((1 << 28) + 1, 64, 512, ("tile", 128, 128)), ((1 << 30) - 256, 64, 64, ("tile", 256, 256)), (1 << 30, 256, 64, None)])
 def test_tiles_beyond_a_launch_are_no_candidates(m, n, k, want):
     assert rules.product(m, n, k) == want
+
+
+def test_batches_of_rows_take_every_product_kernel():
+    assert {rules.product(m, N, K) for m in BATCHES + [5000]} | {rules.product(50, 300, K)} >= {("few", g) for g in (1, 2, 4)} | {
+        ("tile", *t) for t in ((64, 64), (64, 128), (128, 128), (256, 256))}
