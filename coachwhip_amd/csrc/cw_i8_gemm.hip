@@ -191,7 +191,7 @@ __global__ __launch_bounds__(256, 1) void k_i8_big(I8MatArgs a, int tiles_m, int
 
 // Fewer rows than fill the device with such tiles: tiles of 32 FM x 32 FN, eight waves: two groups of four (16 FM x
 // 16 FN each), one for each half of a step. A ring of LDS stages keeps 96 to 128 KB of loads in flight on a CU, for which
-// these tiles wait (52 % of the waves' cycles at 77 rows of 4001 x 2880); the groups' integer sums meet in LDS.
+// these tiles wait (51 % of the waves' cycles at 77 rows of 4001 x 2880); the groups' integer sums meet in LDS.
 template <int FM, int FN>
 struct I8Ring {
     static constexpr int TM = 32 * FM, TN = 32 * FN, STAGE = (TM + TN) * I8_STEP, STAGES = 163840 / STAGE < 8 ? 163840 / STAGE : 8;
@@ -268,8 +268,8 @@ __global__ __launch_bounds__(512, 2) void k_i8_ring(I8MatArgs a, int tiles_m, in
 
 // Few rows of x: a block takes 16 rows of W and up to 16 MB of x over all of k, its waves the steps of 128 codes in
 // turn, both operands straight from memory into registers (no byte of either is used by two waves of a block). The
-// waves' sums meet in LDS: integers, so in any order the same. One row of 8192 x 8192: 13.8 us, 4.9 TB/s (16 waves, or
-// two to four steps' loads at a time, when it took 15.0: 15.0 to 18.8, fewer blocks fit a CU); 2048 x 2048: 3.9 us, of which the
+// waves' sums meet in LDS: integers, so in any order the same. One row of 8192 x 8192: 14 us, 4.8 TB/s (16 waves, or
+// two to four steps' loads at a time, when it took 15.0: 15.0 to 18.8, fewer blocks fit a CU); 2048 x 2048: 3.8 us, of which the
 // launch and one round trip are most.
 template <class T, int MB>
 __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_i8_few(I8MatArgs a) {
