@@ -398,7 +398,7 @@ __device__ __forceinline__ bool item_of_block(const I8MoeArgs &a, int n_blocks, 
 }
 
 // A wave multiplies a tile's picks with 8 NW rows of gate and of up, or 16 NW of down. 2,048 tokens over 128 experts of
-// 2,880 x 2,880: gate and up 489 us, down 258, 4.35 TB/s of weights, beside the f32 rows it writes (gate and up without
+// 2,880 x 2,880: gate and up 492 us, down 257, 4.35 TB/s of weights, beside the f32 rows it writes (gate and up without
 // their stores: 411). With many picks an expert its waves wait to issue: 61 % of their cycles over 8 experts of 2,048 x 4,096, at 42 %
 // of the integer rate, L2 read at 6.7 TB/s.
 template <bool DOWN, int MB, int NW>
