@@ -15,6 +15,8 @@ NO_SLOT = 0xFFFFFFFF
 CW_MOE_STATE_BYTES, CW_MOE_STATUS_OFFSET = 8448, 8320
 # include/cwmoe.h: the most codes in a row of the 8-bit integer path
 CW_I8_MAX_K = 32768
+# include/cwmoe.h: the most codes in a row of the 8-bit float path
+CW_F8_MAX_K = 32768
 
 
 class CwError(RuntimeError):
@@ -51,6 +53,11 @@ class I8MoeDesc(ctypes.Structure):
     _fields_ = [("n_experts", _I), ("top_k", _I), ("hidden", _I), ("inter", _I), ("norm", _I), ("act", _I),
                 ("alpha", ctypes.c_float), ("limit", ctypes.c_float), ("w", _P * 3), ("slot_stride", _L * 3),
                 ("scale", _P * 3), ("bias", _P * 3)]
+
+
+class F8MoeDesc(ctypes.Structure):
+    """struct cw_f8_moe_desc (include/cwmoe.h)."""
+    _fields_ = I8MoeDesc._fields_
 
 
 class BankSource(ctypes.Structure):
@@ -98,6 +105,21 @@ SIGNATURES = {
     "cw_i8_matmul": ([_P, _P, _L, _L, _P, _P, _L, _P, _I, _P, _L, _P], _I),
     "cw_i8_moe_workspace_size": ([ctypes.POINTER(I8MoeDesc), _I], ctypes.c_size_t),
     "cw_i8_moe_layer": ([ctypes.POINTER(I8MoeDesc), _P, _P, _P, _I, _I, _P, _P, _P, _P, ctypes.c_size_t, _P], _I),
+    "cw_f8_row_bytes": ([_L], _L),
+    "cw_quantize_f8": ([_I, _P, _L, _L, _L, _P, _P, _P], _I),
+    "cw_swiglu_f8": ([_I, _P, _P, _L, _L, _L, _I, ctypes.c_float, ctypes.c_float, _P, _P, _P], _I),
+    "cw_quantize_f8_matrix": ([_I, _P, _L, _L, _L, _P, _P, _P], _I),
+    "cw_dequantize_f8": ([_P, _P, _L, _L, _I, _P, _P], _I),
+    "cw_f8_matmul": ([_P, _P, _L, _L, _P, _P, _L, _P, _I, _P, _L, _P], _I),
+    "cw_pile_tiles_bytes": ([_L, _I], _L),
+    "cw_sort_picks_workspace_size": ([_L, _I], ctypes.c_size_t),
+    "cw_sort_picks": ([_P, _L, _I, _P, _P, _P, _P, _P, ctypes.c_size_t, _P], _I),
+    "cw_to_piles": ([_I, _P, _L, _L, _I, _I, _L, _P, _P, _P, _P], _I),
+    "cw_from_piles": ([_I, _P, _L, _P, _L, _I, _I, _L, _P, _P, _P, _P], _I),
+    "cw_from_piles_grad": ([_I, _P, _L, _P, _L, _P, _L, _I, _I, _L, _P, _P, _P, _P, _P], _I),
+    "cw_f8_matmul_experts": ([_P, _L, _P, _I, _L, _L, _P, _P, _L, _P, _I, _L, _P, _P, _I, _P, _L, _P], _I),
+    "cw_f8_moe_workspace_size": ([ctypes.POINTER(F8MoeDesc), _I], ctypes.c_size_t),
+    "cw_f8_moe_layer": ([ctypes.POINTER(F8MoeDesc), _P, _P, _P, _I, _I, _P, _P, _P, _P, ctypes.c_size_t, _P], _I),
     "cw_gguf_open": ([ctypes.c_char_p], _P),
     "cw_gguf_close": ([_P], None),
     "cw_gguf_version": ([_P], _I),

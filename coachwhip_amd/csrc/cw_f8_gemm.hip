@@ -1,0 +1,369 @@
+// Products of rows of e4m3 codes with e4m3 matrices, scales of 128 columns of k (gfx950): one matrix, or of sorted rows each with its
+// expert's.
+#include <atomic>
+
+#include "cw_f8_rules.h"
+#include "cw_f8_tile.h"
+#include "cw_mfma.h"
+#include "cw_piles.h"
+
+namespace cw {
+
+struct F8MatArgs {
+    const uint8_t *w, *x;
+    const float *ws, *xs, *bias;
+    int64_t n, m;    // m: rows of x, whose scales are m apart
+    int rb, blocks;  // bytes of a row, scales of a row
+    void *y;
+    int64_t ldy;
+    // sorted rows
+    int64_t w_stride, ws_stride;  // from an expert's to the next
+    const void *tiles;
+    const int *order;  // NULL: x holds the sorted rows; else x's row of a position is order / K
+    int K, E;
+};
+
+// Few rows of x: a block takes 16 rows of W and up to 16 MB of x over all of k, its waves the steps of 128 codes in turn, both
+// operands straight from memory into registers (no byte of either is used by two waves of a block). The waves' sums meet in LDS, added
+// in the waves' order.
+template <class T, int MB>
+__global__ __launch_bounds__(64 * F8_FEW_WAVES) void k_f8_few(F8MatArgs a) {
+    __shared__ f32x4 part[F8_FEW_WAVES][MB][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = 16 * (lane >> 4);
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const uint8_t *w0 = a.w + n0 * a.rb;
+    const float *ws = a.ws + n0 / F8_BLOCK * a.blocks;
+    const uint32_t wrow = (uint32_t)(min(lane & 15, (int)(a.n - 1 - n0)) * a.rb + at);
+    uint32_t xrow[MB], srow[MB];
+#pragma unroll
+    for (int i = 0; i < MB; i++) {
+        srow[i] = min(16 * i + (lane & 15), (int)a.m - 1);
+        xrow[i] = srow[i] * a.rb + at;
+    }
+    f32x4 acc[MB];
+#pragma unroll
+    for (int i = 0; i < MB; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int step = wave; step < a.blocks; step += F8_FEW_WAVES) {
+        const uint8_t *w = w0 + (int64_t)step * F8_BLOCK + wrow, *x = a.x + (int64_t)step * F8_BLOCK;
+        F8Frag<true> wf, xf;
+        wf.load(w, w + 64);
+        const float sw = ws[step];
+#pragma unroll
+        for (int i = 0; i < MB; i++) {
+            const F8Scale s(a.xs[step * a.m + srow[i]], sw);
+            xf.load(x + xrow[i], x + xrow[i] + 64);
+            const f32x4 p = F8Frag<true>::product(wf, xf);
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[i][c] = s.add(p[c], acc[i][c]);
+        }
+    }
+    const int64_t m = 16 * (wave % MB) + (lane & 15), n = n0 + 4 * (lane >> 4);
+    float b[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) b[i] = a.bias ? a.bias[min(n + i, a.n - 1)] : 0.f;
+#pragma unroll
+    for (int i = 0; i < MB; i++) part[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave >= MB || m >= a.m || n >= a.n) return;
+    f32x4 v = part[0][wave][lane];
+#pragma unroll
+    for (int o = 1; o < F8_FEW_WAVES; o++) v += part[o][wave][lane];
+    f8_store4((T *)a.y + m * a.ldy + n, (int)min(a.n - n, (int64_t)4), v, b);
+}
+
+// Blocks go to the eight dies in turn: each die gets a contiguous range of tiles, in panels of four tiles of W, so that
+// those which it runs at once share both operands through its cache.
+__device__ __forceinline__ void f8_tile_of_block(int tiles_m, int tiles_n, int tm, int tn, int64_t &m0, int64_t &n0) {
+    const int total = tiles_m * tiles_n, die = blockIdx.x & 7, per = total >> 3, rest = total & 7;
+    const int id = die * per + min(die, rest) + (int)(blockIdx.x >> 3);
+    const int panel = id / (4 * tiles_m), width = min(4, tiles_n - 4 * panel), in = id - panel * 4 * tiles_m;
+    m0 = (int64_t)__builtin_amdgcn_readfirstlane(in / width) * tm;
+    n0 = (int64_t)__builtin_amdgcn_readfirstlane(4 * panel + in % width) * tn;
+}
+
+// A tile of 16 WM MF rows of x by 16 WN NF rows of W, a wave of 16 MF x 16 NF each; codes and scales of a step through a ring of LDS
+// stages by direct global-to-LDS loads, chunk c (16 bytes) of row r at chunk c ^ (r % 8) of its 128 bytes: the reads of one
+// chunk touch all banks once.
+template <int WN, int WM, int NF, int MF, int STAGES>
+struct F8Ring {
+    static constexpr int N_WAVES = WN, TN = 16 * WN * NF, TM = 16 * WM * MF, WAVES = WN * WM, NT = 64 * WAVES;
+    static constexpr int SCALES = TM < 64 ? 64 : TM;  // (a load of scales: 64 of them)
+    static constexpr int CODES = (TN + TM) * F8_BLOCK, STAGE = CODES + 4 * SCALES;
+    static constexpr int LOADS = (TN + TM) / 8, PER = (LOADS + WAVES - 1) / WAVES, D = STAGES - 1, LDS = STAGES * STAGE;
+    static_assert(LDS <= 159 * 1024 && SCALES / 64 <= WAVES, "the ring fits the CU, a load of scales a wave");
+};
+// xrow(r): x's row of row r < TM of the tile (any valid row past its end); n0: the tile's first row of W; w, ws: the matrix. ANY: for
+// scales of any size; else for usual ones, and true if the wave saw another (the WN waves of a row of the tile look at a WN'th of its
+// rows' scales each).
+template <class R, int NF, int MF, bool EXACT, bool ANY, class XRow>
+__device__ __forceinline__ bool f8_pass(uint8_t *lds, const F8MatArgs &a, const uint8_t *w, const float *ws, int64_t n0, XRow xrow, int wn, int wm,
+                                        f32x4 (&acc)[MF][NF]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), steps = a.blocks;
+    // a stage: TN rows of W, then TM of x, then x's scales; load i of this wave: 8 rows from 8 (wave + WAVES i) (past the last:
+    // the first ones again, the same bytes to the same place)
+    const uint8_t *from[R::PER];
+#pragma unroll
+    for (int i = 0; i < R::PER; i++) {
+        const int r = 8 * ((wave + R::WAVES * i) % R::LOADS) + (lane >> 3);
+        const uint8_t *row = r < R::TN ? w + min(n0 + r, a.n - 1) * a.rb : a.x + xrow(r - R::TN) * (int64_t)a.rb;
+        from[i] = row + 16 * ((lane & 7) ^ (r & 7));
+    }
+    constexpr int SEGMENTS = R::SCALES / 64;
+    const float *scale = a.xs + xrow(min(64 * (wave % SEGMENTS) + lane, R::TM - 1));
+    const uint32_t to = lds_addr(lds);
+    auto fetch = [&](int step, int buf) __attribute__((always_inline)) {
+        const uint32_t at = to + buf * R::STAGE;
+#pragma unroll
+        for (int i = 0; i < R::PER; i++)
+            dma16(from[i] + (int64_t)step * F8_BLOCK, __builtin_amdgcn_readfirstlane(at + 1024 * ((wave + R::WAVES * i) % R::LOADS)));
+        dma4(scale + step * a.m, __builtin_amdgcn_readfirstlane(at + R::CODES + 256 * (wave % SEGMENTS)));
+    };
+    const int c0 = 16 * ((lane >> 4) ^ (lane & 7)), c1 = 16 * ((4 + (lane >> 4)) ^ (lane & 7));
+    const uint8_t *wl = lds + (16 * NF * wn + (lane & 15)) * F8_BLOCK, *xl = lds + (R::TN + 16 * MF * wm + (lane & 15)) * F8_BLOCK;
+    const uint8_t *sl = lds + R::CODES + 4 * (16 * MF * wm + (lane & 15));
+    const float *sw_of = ws + (n0 + 16 * NF * wn < a.n ? (n0 + 16 * NF * wn) / F8_BLOCK : 0) * a.blocks;
+#pragma unroll
+    for (int i = 0; i < MF; i++)
+#pragma unroll
+        for (int j = 0; j < NF; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < R::D && s < steps; s++) fetch(s, s);
+    int buf = 0, next = R::D;
+    bool odd = false;
+    for (int step = 0; step < steps; step++) {
+        // this wave's part of the stage is in (the stages after it may still be on their way), then every wave's; and
+        // every wave has multiplied the stage before, whose place the stage D ahead takes
+        if (step + R::D <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((R::D - 1) * (R::PER + 1)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (step + R::D < steps) fetch(step + R::D, next);
+        next = next + 1 == R::D + 1 ? 0 : next + 1;
+        const float sw = sw_of[step];
+        const int o = buf * R::STAGE;
+        if constexpr (!ANY) odd |= !f8_usual(sw);
+        F8Frag<EXACT> wf[NF], xf;
+#pragma unroll
+        for (int j = 0; j < NF; j++) wf[j].load(wl + o + c0 + 2048 * j, wl + o + c1 + 2048 * j);
+#pragma unroll
+        for (int i = 0; i < MF; i++) {
+            xf.load(xl + o + c0 + 2048 * i, xl + o + c1 + 2048 * i);
+            const float sx = *(const float *)(sl + o + 64 * i);
+            if constexpr (!ANY)
+                if (i % R::N_WAVES == wn) odd |= !f8_usual(sx);
+            const float s = sx * sw;
+            const F8Scale any(sx, sw);
+#pragma unroll
+            for (int j = 0; j < NF; j++) {
+                const f32x4 p = F8Frag<EXACT>::product(wf[j], xf);
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[i][j][c] = ANY ? any.add(p[c], acc[i][j][c]) : fmaf(p[c], s, acc[i][j][c]);
+            }
+        }
+        buf = buf + 1 == R::D + 1 ? 0 : buf + 1;
+    }
+    return odd;
+}
+template <class R, int NF, int MF, bool EXACT, class XRow>
+__device__ __forceinline__ void f8_loop(uint8_t *lds, const F8MatArgs &a, const uint8_t *w, const float *ws, int64_t n0, XRow xrow, int wn, int wm,
+                                        f32x4 (&acc)[MF][NF]) {
+    const bool odd = f8_pass<R, NF, MF, EXACT, false>(lds, a, w, ws, n0, xrow, wn, wm, acc);
+    if (__syncthreads_or(odd)) f8_pass<R, NF, MF, EXACT, true>(lds, a, w, ws, n0, xrow, wn, wm, acc);
+}
+// A wave's sums stored: rows m0.. of m_end of y, columns n0.. . All biases are loaded before the bounds checks, from clamped places.
+template <class T, int MF, int NF>
+__device__ __forceinline__ void f8_finish(const F8MatArgs &a, const float *bias, int64_t m0, int64_t m_end, int64_t n0, const f32x4 (&acc)[MF][NF]) {
+    const int lane = threadIdx.x & 63;
+    const int64_t m = m0 + (lane & 15), n = n0 + 4 * (lane >> 4);
+    float b[NF][4];
+#pragma unroll
+    for (int j = 0; j < NF; j++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) b[j][c] = bias ? bias[min(n + 16 * j + c, a.n - 1)] : 0.f;
+#pragma unroll
+    for (int i = 0; i < MF; i++) {
+        if (m + 16 * i >= m_end) continue;
+#pragma unroll
+        for (int j = 0; j < NF; j++)
+            if (n + 16 * j < a.n) f8_store4((T *)a.y + (m + 16 * i) * a.ldy + n + 16 * j, (int)min(a.n - n - 16 * j, (int64_t)4), acc[i][j], b[j]);
+    }
+}
+
+// Results in f32 have exact products, f16's and bf16's rounding covers what the 8-bit instruction leaves out.
+template <class T>
+constexpr bool f8_exact_for = std::is_same_v<T, float>;
+
+template <class T, int WN, int WM, int NF, int MF, int STAGES>
+__global__ __launch_bounds__(64 * WN *WM, WN *WM / 4) void k_f8_tile(F8MatArgs a, int tiles_m, int tiles_n) {
+    using R = F8Ring<WN, WM, NF, MF, STAGES>;
+    extern __shared__ __align__(1024) uint8_t lds[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wm = wave / WN;
+    int64_t m0, n0;
+    f8_tile_of_block(tiles_m, tiles_n, R::TM, R::TN, m0, n0);
+    f32x4 acc[MF][NF];
+    f8_loop<R, NF, MF, f8_exact_for<T>>(lds, a, a.w, a.ws, n0, [&](int r) { return min(m0 + r, a.m - 1); }, wn, wm, acc);
+    f8_finish<T, MF, NF>(a, a.bias, m0 + 16 * MF * wm, a.m, n0 + 16 * NF * wn, acc);
+}
+
+// The item of a block: blocks go to the eight dies in turn; each die takes a contiguous range of the items, an expert's
+// blocks of W one after the other and its tiles side by side for each, so that an expert's rows and weights are read by
+// one die and not by all, the weights once for all its tiles.
+__device__ __forceinline__ bool f8_item_of_block(const void *list, int n_blocks, PileTile &tl, int &nb) {
+    const PileTile *tiles = pile_tiles(list);
+    const int64_t total = (int64_t)*(const int *)list * n_blocks, per = total >> 3;
+    const int die = blockIdx.x & 7, at = blockIdx.x >> 3, rest = (int)(total & 7);
+    if (at >= per + (die < rest)) return false;
+    const int64_t item = die * per + min(die, rest) + at;
+    const PileTile any = tiles[__builtin_amdgcn_readfirstlane((int)(item / n_blocks))];  // a tile of the item's expert
+    const int in = (int)(item - (int64_t)any.first * n_blocks);
+    nb = __builtin_amdgcn_readfirstlane(in / any.of);
+    if (any.of == 1) tl = any;
+    else tl = tiles[__builtin_amdgcn_readfirstlane(any.first + in - nb * any.of)];
+    return true;
+}
+
+template <class T, int MF, int STAGES>
+__device__ __forceinline__ void f8_expert_tile(const F8MatArgs &a, const PileTile &tl, int64_t n0, uint8_t *lds) {
+    using R = F8Ring<8, 1, 1, MF, STAGES>;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    f32x4 acc[MF][1];
+    f8_loop<R, 1, MF, f8_exact_for<T>>(lds, a, a.w + tl.expert * a.w_stride, a.ws + tl.expert * a.ws_stride, n0,
+                      [&](int r) {
+                          const int pos = tl.pos0 + min(r, tl.m - 1);
+                          return (int64_t)(a.order ? a.order[pos] / a.K : pos);
+                      },
+                      wave, 0, acc);
+    f8_finish<T, MF, 1>(a, a.bias ? a.bias + tl.expert * a.n : nullptr, tl.pos0, tl.pos0 + tl.m, n0 + 16 * wave, acc);
+}
+template <class T>
+__global__ __launch_bounds__(512, 2) void k_f8_experts(F8MatArgs a, int n_blocks) {
+    extern __shared__ __align__(1024) uint8_t lds[];
+    PileTile tl;
+    int nb;
+    if (!f8_item_of_block(a.tiles, n_blocks, tl, nb)) return;
+    const int64_t n0 = (int64_t)128 * nb;
+    if (tl.expert == a.E) {  // positions of no expert: zeros
+        const int cols = (int)min(a.n - n0, (int64_t)128);
+        for (int i = threadIdx.x; i < tl.m * cols; i += 512) ((T *)a.y)[(int64_t)(tl.pos0 + i / cols) * a.ldy + n0 + i % cols] = from_f32<T>(0.f);
+        return;
+    }
+    if (tl.m <= 16) f8_expert_tile<T, 1, 8>(a, tl, n0, lds);
+    else if (tl.m <= 32) f8_expert_tile<T, 2, 7>(a, tl, n0, lds);
+    else if (tl.m <= 64) f8_expert_tile<T, 4, 6>(a, tl, n0, lds);
+    else f8_expert_tile<T, 8, 4>(a, tl, n0, lds);
+}
+
+// dynamic LDS above 64 KB, opted into once per kernel and device
+template <class T, int I>
+static int f8_allow_lds(const void *kernel, int lds) {
+    static std::atomic<bool> set[MAX_DEVICES];
+    const int dev = current_device();
+    if (set[dev].load(std::memory_order_relaxed)) return CW_OK;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return set_error(CW_EHIP, "f8: %d bytes of LDS", lds);
+    set[dev].store(true, std::memory_order_relaxed);
+    return CW_OK;
+}
+template <class T, int WN, int WM, int NF, int MF, int STAGES>
+static int f8_tiles(const F8MatArgs &a, hipStream_t s) {
+    using R = F8Ring<WN, WM, NF, MF, STAGES>;
+    auto kernel = k_f8_tile<T, WN, WM, NF, MF, STAGES>;
+    const int64_t tm = (a.m + R::TM - 1) / R::TM, tn = (a.n + R::TN - 1) / R::TN;
+    if (int rc = f8_allow_lds<T, R::TM>((const void *)kernel, R::LDS)) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(R::NT), R::LDS, s, a, (int)tm, (int)tn);
+    return check_launch("k_f8_tile");
+}
+template <class T>
+static int f8_matmul(const F8MatArgs &a, int few_groups, int tile_of, hipStream_t s) {
+    auto few = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.n + 15) / 16)), dim3(64 * F8_FEW_WAVES), 0, s, a);
+        return check_launch("k_f8_few");
+    };
+    if (few_groups) return few_groups == 1 ? few(k_f8_few<T, 1>) : few_groups == 2 ? few(k_f8_few<T, 2>) : few(k_f8_few<T, 4>);
+    switch (tile_of) {
+    case 0: return f8_tiles<T, 4, 2, 1, 2, 8>(a, s);
+    case 1: return f8_tiles<T, 4, 2, 2, 4, 4>(a, s);
+    default: return f8_tiles<T, 4, 2, 4, 8, 2>(a, s);
+    }
+}
+
+template <class T>
+static int f8_experts(const F8MatArgs &a, int64_t tiles, hipStream_t s) {
+    constexpr int LDS = std::max({F8Ring<8, 1, 1, 1, 8>::LDS, F8Ring<8, 1, 1, 2, 7>::LDS, F8Ring<8, 1, 1, 4, 6>::LDS, F8Ring<8, 1, 1, 8, 4>::LDS});
+    const int blocks = (int)((a.n + 127) / 128);
+    if (int rc = f8_allow_lds<T, 0>((const void *)k_f8_experts<T>, LDS)) return rc;
+    hipLaunchKernelGGL(k_f8_experts<T>, dim3((unsigned)((tiles * blocks + 7) / 8 * 8)), dim3(512), LDS, s, a, blocks);
+    return check_launch("k_f8_experts");
+}
+
+static int check_product(const char *what, int ydtype, int64_t n, int64_t k, int64_t m, int64_t ldy) {
+    if (!f8_float_type(ydtype)) return set_error(CW_ENOTSUP, "%s: type %d of y (f32, f16 or bf16)", what, ydtype);
+    CW_REQUIRE(n > 0 && k > 0 && m >= 0 && n < (1ll << 31) && m < (1ll << 31), "%s: %lld x %lld, %lld rows of x", what, (long long)n, (long long)k,
+               (long long)m);
+    if (k > CW_F8_MAX_K) return set_error(CW_ENOTSUP, "%s: rows of %lld above %d", what, (long long)k, CW_F8_MAX_K);
+    if (n > 1 << 26) return set_error(CW_ENOTSUP, "%s: %lld rows of w above %d", what, (long long)n, 1 << 26);
+    CW_REQUIRE(ldy >= n, "%s: rows of y of %lld %lld apart", what, (long long)n, (long long)ldy);
+    return CW_OK;
+}
+static F8MatArgs product_args(const uint8_t *w, const float *w_scale, int64_t n, int64_t k, const uint8_t *x, const float *x_scale, int64_t m,
+                              const float *bias, void *y, int64_t ldy) {
+    F8MatArgs a = {};
+    a.w = w;
+    a.x = x;
+    a.ws = w_scale;
+    a.xs = x_scale;
+    a.bias = bias;
+    a.n = n;
+    a.m = m;
+    a.rb = (int)f8_row_bytes(k);
+    a.blocks = (int)f8_blocks(k);
+    a.y = y;
+    a.ldy = ldy;
+    return a;
+}
+
+}  // namespace cw
+
+using namespace cw;
+
+extern "C" {
+
+int cw_f8_matmul(const uint8_t *w, const float *w_scale, int64_t n, int64_t k, const uint8_t *x, const float *x_scale, int64_t m,
+                 const float *bias, int ydtype, void *y, int64_t ldy, cw_stream_t stream) {
+    if (int rc = check_product("f8_matmul", ydtype, n, k, m, ldy)) return rc;
+    if (m == 0) return CW_OK;
+    const int rb = (int)f8_row_bytes(k), few_groups = f8_few_groups(m, n, rb), tile = few_groups ? 0 : f8_pick_tile(m, n, rb, (int)resident_blocks(1));
+    if (tile < 0) return set_error(CW_ENOTSUP, "f8_matmul: %lld x %lld outputs", (long long)m, (long long)n);
+    CW_REQUIRE(w && w_scale && x && x_scale && y, "f8_matmul: null pointer");
+    CW_REQUIRE(f8_aligned(w, 16) && f8_aligned(x, 16), "f8_matmul: codes must be 16-byte aligned");
+    const F8MatArgs a = product_args(w, w_scale, n, k, x, x_scale, m, bias, y, ldy);
+    hipStream_t s = (hipStream_t)stream;
+    if (ydtype == CW_F16) return f8_matmul<_Float16>(a, few_groups, tile, s);
+    if (ydtype == CW_BF16) return f8_matmul<bf16_t>(a, few_groups, tile, s);
+    return f8_matmul<float>(a, few_groups, tile, s);
+}
+
+int cw_f8_matmul_experts(const uint8_t *w, int64_t w_stride, const float *w_scale, int n_experts, int64_t n, int64_t k, const uint8_t *x,
+                         const float *x_scale, int64_t m, const int32_t *order, int K, int64_t picks, const void *tiles, const float *bias,
+                         int ydtype, void *y, int64_t ldy, cw_stream_t stream) {
+    if (int rc = check_product("f8_matmul_experts", ydtype, n, k, m, ldy)) return rc;
+    CW_REQUIRE(n_experts > 0 && n_experts <= PILE_MAX_EXPERTS, "f8_matmul_experts: %d experts (1..%d supported)", n_experts, PILE_MAX_EXPERTS);
+    CW_REQUIRE(K > 0 && picks >= 0 && picks < 1 << 28, "f8_matmul_experts: %lld picks, %d a token", (long long)picks, K);
+    CW_REQUIRE(order ? m * K == picks : m == picks, "f8_matmul_experts: %lld rows of x for %lld picks, %d a token", (long long)m, (long long)picks, K);
+    CW_REQUIRE(w_stride >= n * f8_row_bytes(k) && w_stride % 16 == 0, "f8_matmul_experts: %lld bytes from an expert's matrix to the next",
+               (long long)w_stride);
+    const int64_t most = pile_max_tiles(picks, n_experts);
+    if (most * ((n + 127) / 128) >= 1 << 23) return set_error(CW_ENOTSUP, "f8_matmul_experts: %lld picks of %lld outputs", (long long)picks, (long long)n);
+    if (picks == 0) return CW_OK;
+    CW_REQUIRE(w && w_scale && x && x_scale && tiles && y, "f8_matmul_experts: null pointer");
+    CW_REQUIRE(f8_aligned(w, 16) && f8_aligned(x, 16) && f8_aligned(tiles, 16), "f8_matmul_experts: codes and tiles must be 16-byte aligned");
+    F8MatArgs a = product_args(w, w_scale, n, k, x, x_scale, m, bias, y, ldy);
+    a.w_stride = w_stride;
+    a.ws_stride = f8_blocks(n) * f8_blocks(k);
+    a.tiles = tiles;
+    a.order = order;
+    a.K = K;
+    a.E = n_experts;
+    hipStream_t s = (hipStream_t)stream;
+    if (ydtype == CW_F16) return f8_experts<_Float16>(a, most, s);
+    if (ydtype == CW_BF16) return f8_experts<bf16_t>(a, most, s);
+    return f8_experts<float>(a, most, s);
+}
+
+}  // extern "C"

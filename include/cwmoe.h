@@ -50,7 +50,7 @@ enum cw_status { CW_OK = 0, CW_ENOTSUP = 1, CW_EINVAL = 2, CW_EHIP = 3, CW_EFULL
 enum cw_dtype {
     CW_F32 = 0,
     CW_F16 = 1,
-    CW_BF16 = 30,    /* activations of the 8-bit integer path */
+    CW_BF16 = 30,    /* activations of the 8-bit paths */
     CW_Q8_0 = 8,     /* {f16 d; i8 qs[32]}: 34 B per 32 weights */
     CW_Q2_K = 10,    /* {u8 scales[16]; u8 qs[64]; f16 d, dmin}: 84 B per 256 (the shrink's output) */
     CW_Q3_K = 11,    /* {u8 hmask[32]; u8 qs[64]; u8 scales[12]; f16 d}: 110 B per 256 (shrink input) */
@@ -363,6 +363,100 @@ typedef struct cw_i8_moe_desc {
  * would exceed the grid. */
 size_t cw_i8_moe_workspace_size(const cw_i8_moe_desc *desc, int T);
 int cw_i8_moe_layer(const cw_i8_moe_desc *desc, const int8_t *x, const float *x_scale, const float *logits, int T, int ydtype,
+                    void *out, uint32_t *ids_out, float *w_out, void *ws, size_t ws_bytes, cw_stream_t stream);
+
+/* ---- experts in 8-bit floats, and the tokens' way to them ------------------------------------ */
+
+/* Rows and matrices of e4m3 codes (OCP: largest value 448, no infinity) with an f32 scale for each block of 128, the
+ * format that checkpoints of large MoE models are published in. No counterpart in the reference. Rows: row r of k codes starts
+ * at byte r * cw_f8_row_bytes(k), k rounded up to whole 128 bytes, 16-byte aligned; the bytes past k are zero (the calls that
+ * write codes write them). Scales of `rows` rows: scale[b * rows + r] is that of columns 128 b .. 128 b + 127 of row r. A matrix
+ * of n rows is such rows with a scale for each 128 x 128: scale[(r / 128) * ceil(k / 128) + b]. Value = code * scale.
+ * Activations and results are f32, f16 or bf16. Rows of at most CW_F8_MAX_K codes: CW_ENOTSUP above. None of the calls
+ * needs memory that was cleared, and none keeps anything for the next one. */
+#define CW_F8_MAX_K 32768
+int64_t cw_f8_row_bytes(int64_t k);
+
+/* Rows of k values (ldx elements apart, of type dtype, at any address of that type) to codes, each 128 columns by themselves: a the
+ * largest magnitude, scale = a / 448 rounded to f32, code = 448 x / a rounded to f32 and then to the nearest e4m3 (ties to even).
+ * A group of zeros gets the scale 0, one with an infinity or a NaN the scale NaN and zero codes, so that what is made of it is NaN.
+ * (Below a of 2^-117 the scale is subnormal and loses digits.) CW_ENOTSUP for 2^27 groups or more. */
+int cw_quantize_f8(int dtype, const void *x, int64_t ldx, int64_t rows, int64_t k, uint8_t *q, float *scale, cw_stream_t stream);
+
+/* The same of h = silu(g) * u, or of the clamped SwiGLU, as cw_swiglu_i8 has it. */
+int cw_swiglu_f8(int dtype, const void *g, const void *u, int64_t ld, int64_t rows, int64_t width, int act, float alpha, float limit,
+                 uint8_t *q, float *scale, cw_stream_t stream);
+
+/* The same of a matrix, a block of 128 x 128 by itself: for weights, once when they are loaded. */
+int cw_quantize_f8_matrix(int dtype, const void *w, int64_t ldw, int64_t n, int64_t k, uint8_t *q, float *scale, cw_stream_t stream);
+
+/* out (rows of k, of type dtype) = code * scale, of rows (not of a matrix). */
+int cw_dequantize_f8(const uint8_t *q, const float *scale, int64_t rows, int64_t k, int dtype, void *out, cw_stream_t stream);
+
+/* y[r][c] = sum over blocks b of 128 columns of x_scale[b][r] * w_scale[c / 128][b] * sum_{k in b} x[r][k] w[c][k] (+ bias[c], f32,
+ * may be NULL): a block's sum by the matrix instruction in f32, scaled and added in f32 (in an order that the number of rows
+ * may change), whatever the scales' exponents, and rounded once to ydtype. W is n rows of k codes, x m rows; rows of y are ldy elements
+ * apart. CW_ENOTSUP for n above 2^26 and for results of 2^22 tiles of 256 x 256 or more. */
+int cw_f8_matmul(const uint8_t *w, const float *w_scale, int64_t n, int64_t k, const uint8_t *x, const float *x_scale, int64_t m,
+                 const float *bias, int ydtype, void *y, int64_t ldy, cw_stream_t stream);
+
+/* Picks sorted by expert: pick p (token p / K's choice p % K) goes to expert ids[p]; ids outside 0 .. n_experts - 1 (experts
+ * that another device holds) go to none, behind all others. A stable sort: order[pos] = the pick at a position, place[p] = the
+ * position of a pick (each a permutation of 0 .. picks - 1), offsets[e] = picks of experts below e, for e = 0 .. n_experts: positions
+ * from offsets[n_experts] on are those of no expert. tiles (cw_pile_tiles_bytes bytes, 16-byte aligned) receives the plan
+ * that cw_f8_matmul_experts reads. ws: of cw_sort_picks_workspace_size bytes (0 for up to 65,536 picks), any contents; calls that
+ * overlap in time need distinct ones. n_experts <= 1024; CW_ENOTSUP from 2^28 picks on. */
+int64_t cw_pile_tiles_bytes(int64_t picks, int n_experts);
+size_t cw_sort_picks_workspace_size(int64_t picks, int n_experts);
+int cw_sort_picks(const uint32_t *ids, int64_t picks, int n_experts, int32_t *order, int32_t *place, int32_t *offsets, void *tiles,
+                  void *ws, size_t ws_bytes, cw_stream_t stream);
+
+/* Tokens to their experts' piles, and back: place and offsets as cw_sort_picks wrote them for T x K picks; rows of h values of type
+ * dtype, of the piles' rows T x K. rows[place[t][j]] = x[t], and zeros at the positions of no expert; its gradient is
+ * cw_from_piles without weights of the rows' gradient. x's rows are ldx elements apart, the piles' rows h. */
+int cw_to_piles(int dtype, const void *x, int64_t ldx, int64_t T, int K, int n_experts, int64_t h, const int32_t *place,
+                const int32_t *offsets, void *rows, cw_stream_t stream);
+/* out[t] = sum_j w[t][j] rows[place[t][j]] (w NULL: 1), in f32 in the picks' order, rounded once; picks of no expert add nothing,
+ * whatever their rows hold. The piles' rows are ldr elements apart, out's h. */
+int cw_from_piles(int dtype, const void *rows, int64_t ldr, const float *w, int64_t T, int K, int n_experts, int64_t h,
+                  const int32_t *place, const int32_t *offsets, void *out, cw_stream_t stream);
+/* Its gradient: drows[place[t][j]] = w[t][j] dout[t] (rows h apart), dw[t][j] = <dout[t], rows[place[t][j]]> (f32); zeros for picks of no
+ * expert. */
+int cw_from_piles_grad(int dtype, const void *dout, int64_t ldd, const void *rows, int64_t ldr, const float *w, int64_t T, int K,
+                       int n_experts, int64_t h, const int32_t *place, const int32_t *offsets, void *drows, float *dw,
+                       cw_stream_t stream);
+
+/* The experts' products of sorted rows: y[pos] = cw_f8_matmul of one row with the matrix of the position's expert (w_stride bytes
+ * from one to the next, their scales side by side; bias[expert][c], may be NULL), zeros at the positions of no expert. order NULL: x
+ * holds `picks` rows in the piles' order; else x holds the tokens' rows, m = picks / K of them, and a position's is order[pos] / K. m is
+ * x's rows (their scales are m apart); tiles as cw_sort_picks wrote them for these picks. CW_ENOTSUP where the launch would
+ * exceed the grid (2^23 tiles of 128 x 128). */
+int cw_f8_matmul_experts(const uint8_t *w, int64_t w_stride, const float *w_scale, int n_experts, int64_t n, int64_t k, const uint8_t *x,
+                         const float *x_scale, int64_t m, const int32_t *order, int K, int64_t picks, const void *tiles,
+                         const float *bias, int ydtype, void *y, int64_t ldy, cw_stream_t stream);
+
+/* One MoE layer's experts in 8-bit floats, every expert resident: gate and up are [experts][inter] rows of hidden codes, down
+ * [experts][hidden] rows of inter codes, each a matrix with its scales. */
+typedef struct cw_f8_moe_desc {
+    int n_experts;           /* E <= 1024 */
+    int top_k;               /* K <= 32 */
+    int hidden, inter;
+    int norm;                /* renormalise the K weights */
+    int act;                 /* enum cw_act */
+    float alpha, limit;      /* clamped SwiGLU constants */
+    const uint8_t *w[3];     /* gate, up, down */
+    int64_t slot_stride[3];  /* bytes per expert, a multiple of 16 */
+    const float *scale[3];   /* per expert the matrix's, side by side */
+    const float *bias[3];    /* E x inter, E x inter, E x hidden, or NULL (with either activation) */
+} cw_f8_moe_desc;
+
+/* out[T][hidden] = cw_moe_layer's contract on rows of 8-bit floats: route the logits (cw_route_topk), gate and up of the picked
+ * experts, the activation in f32, each pick's hidden row to codes as cw_quantize_f8 does, down, the weighted sum in f32, rounded
+ * once to ydtype. ids_out / w_out (T x K, may be NULL) receive the routing. ws: 256-byte aligned, of
+ * cw_f8_moe_workspace_size bytes, any contents; calls that overlap in time need distinct ones. CW_ENOTSUP where T x top_k reaches
+ * 2^28 and where a launch would exceed the grid. */
+size_t cw_f8_moe_workspace_size(const cw_f8_moe_desc *desc, int T);
+int cw_f8_moe_layer(const cw_f8_moe_desc *desc, const uint8_t *x, const float *x_scale, const float *logits, int T, int ydtype,
                     void *out, uint32_t *ids_out, float *w_out, void *ws, size_t ws_bytes, cw_stream_t stream);
 
 /* ---- GGUF files (host) -------------------------------------------------------------------- */
