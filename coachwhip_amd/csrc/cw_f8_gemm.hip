@@ -202,6 +202,103 @@ __global__ __launch_bounds__(64 * WN *WM, WN *WM / 4) void k_f8_tile(F8MatArgs a
     f8_finish<T, MF, NF>(a, a.bias, m0 + 16 * MF * wm, a.m, n0 + 16 * NF * wn, acc);
 }
 
+// Many rows of x: tiles of 256 x 256, eight waves of 64 columns x 128 rows, two to a SIMD: one multiplies while the other scales and
+// adds. Two LDS stages of 2 x 256 rows x 128 codes and 256 scales, swizzled as in f8_pass. A wave's four fragments of W stay in
+// registers for the step, x's eight pass by, each read while the one before is multiplied; the next step's first ones while the
+// last is, before which all waves meet: the stage of the next step is then in, and this step's, all of which has been read, free for the one after.
+template <class T>
+__global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int tiles_n) {
+    using R = F8Ring<4, 2, 4, 8, 2>;
+    using Frag = F8Frag<false>;
+    extern __shared__ __align__(1024) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave & 3, wm = wave >> 2, last = a.blocks - 1;
+    int64_t m0, n0;
+    f8_tile_of_block(tiles_m, tiles_n, R::TM, R::TN, m0, n0);
+    const uint8_t *w0 = a.w + n0 * a.rb, *x0 = a.x + m0 * a.rb;
+    // load i < 4 of this wave: 8 rows of W from 64 i + 8 wave, then x's likewise
+    uint32_t off[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int r = 64 * (i & 3) + 8 * wave + (lane >> 3);
+        off[i] = (uint32_t)min((int64_t)r, (i < 4 ? a.n - n0 : a.m - m0) - 1) * a.rb + 16 * ((lane & 7) ^ (r & 7));
+    }
+    const float *xs0 = a.xs + m0;
+    const uint32_t soff = 4 * (uint32_t)min((int64_t)(64 * wn + lane), a.m - m0 - 1);
+    const uint32_t to = lds_addr(lds);
+    // load i of a step (8: its scales); past the end the last step's bytes, unused
+    auto fetch = [&](int want, int i) __attribute__((always_inline)) {
+        const int step = min(want, last);
+        const uint32_t stage = to + (want & 1) * R::STAGE;
+        if (i < 8) dma16_s((i < 4 ? w0 : x0) + (int64_t)step * F8_BLOCK, off[i], __builtin_amdgcn_readfirstlane(stage + 8192 * i + 1024 * wave));
+        else dma4_s((const uint8_t *)(xs0 + step * a.m), soff, __builtin_amdgcn_readfirstlane(stage + R::CODES + 256 * wn));
+    };
+    const int c0 = 16 * ((lane >> 4) ^ (lane & 7)), c1 = 16 * ((4 + (lane >> 4)) ^ (lane & 7));
+    const uint8_t *wl = lds + (64 * wn + (lane & 15)) * F8_BLOCK, *xl = lds + (R::TN + 128 * wm + (lane & 15)) * F8_BLOCK;
+    const uint8_t *sl = lds + R::CODES + 4 * (128 * wm + (lane & 15)), *ol = lds + R::CODES + 4 * (128 * wm + 32 * wn + (lane & 31));
+    const float *sw_of = a.ws + (n0 + 64 * wn < a.n ? (n0 + 64 * wn) / F8_BLOCK : 0) * a.blocks;
+    f32x4 acc[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Frag wf[4], xf[2];
+    f32x4 p[2][4];  // the sums of these 16 rows, and of those before, which are scaled and added meanwhile
+    float sx[2], s = 0.f;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 9; i++) fetch(0, i);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    fetch(1, 0);
+    fetch(1, 1);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        wf[j].load(wl + c0 + 2048 * j, wl + c1 + 2048 * j);
+        p[1][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    xf[0].load(xl + c0, xl + c1);
+    sx[0] = *(const float *)sl;
+    auto add = [&](int i, int j) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) acc[i][j][c] = fmaf(p[i & 1][j][c], s, acc[i][j][c]);
+    };
+    for (int step = 0; step <= last; step++) {
+        const float sw = sw_of[step];
+        const int o = (step & 1) * R::STAGE, next = R::STAGE - o;
+        odd |= !f8_usual(*(const float *)(ol + o)) | !f8_usual(sw);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (i == 7) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            const int at = i < 7 ? o + 2048 * (i + 1) : next;
+            xf[(i + 1) & 1].load(xl + at + c0, xl + at + c1);
+            sx[(i + 1) & 1] = *(const float *)(sl + (i < 7 ? o + 64 * (i + 1) : next));
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                p[i & 1][j] = Frag::product(wf[j], xf[i & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+                if (i == 7) wf[j].load(wl + next + c0 + 2048 * j, wl + next + c1 + 2048 * j);
+                add((i + 7) & 7, j);
+                // the next step's loads, two at a time: nine at once after the barrier keep the waves from issuing
+                if (j & 1) {
+                    const int f = 2 * ((i + 1) & 7) + j / 2;
+                    if (f < 9) fetch(i == 7 ? step + 2 : step + 1, f);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            s = sx[i & 1] * sw;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) add(7, j);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (no load may land in LDS that is another block's, or another pass's)
+    if (__syncthreads_or(odd)) {
+        f8_pass<R, 4, 8, false, true>(lds, a, a.w, a.ws, n0, [&](int r) { return min(m0 + r, a.m - 1); }, wn, wm, acc);
+        f8_finish<T, 8, 4>(a, a.bias, m0 + 128 * wm, a.m, n0 + 64 * wn, acc);
+        return;
+    }
+    f8_finish<T, 8, 4>(a, a.bias, m0 + 128 * wm, a.m, n0 + 64 * wn, acc);
+}
+
 // The item of a block: blocks go to the eight dies in turn; each die takes a contiguous range of the items, an expert's
 // blocks of W one after the other and its tiles side by side for each, so that an expert's rows and weights are read by
 // one die and not by all, the weights once for all its tiles.
@@ -260,10 +357,8 @@ static int f8_allow_lds(const void *kernel, int lds) {
     set[dev].store(true, std::memory_order_relaxed);
     return CW_OK;
 }
-template <class T, int WN, int WM, int NF, int MF, int STAGES>
-static int f8_tiles(const F8MatArgs &a, hipStream_t s) {
-    using R = F8Ring<WN, WM, NF, MF, STAGES>;
-    auto kernel = k_f8_tile<T, WN, WM, NF, MF, STAGES>;
+template <class T, class R, class Kernel>
+static int f8_tiles(const F8MatArgs &a, Kernel kernel, hipStream_t s) {
     const int64_t tm = (a.m + R::TM - 1) / R::TM, tn = (a.n + R::TN - 1) / R::TN;
     if (int rc = f8_allow_lds<T, R::TM>((const void *)kernel, R::LDS)) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(R::NT), R::LDS, s, a, (int)tm, (int)tn);
@@ -277,9 +372,11 @@ static int f8_matmul(const F8MatArgs &a, int few_groups, int tile_of, hipStream_
     };
     if (few_groups) return few_groups == 1 ? few(k_f8_few<T, 1>) : few_groups == 2 ? few(k_f8_few<T, 2>) : few(k_f8_few<T, 4>);
     switch (tile_of) {
-    case 0: return f8_tiles<T, 4, 2, 1, 2, 8>(a, s);
-    case 1: return f8_tiles<T, 4, 2, 2, 4, 4>(a, s);
-    default: return f8_tiles<T, 4, 2, 4, 8, 2>(a, s);
+    case 0: return f8_tiles<T, F8Ring<4, 2, 1, 2, 8>>(a, k_f8_tile<T, 4, 2, 1, 2, 8>, s);
+    case 1: return f8_tiles<T, F8Ring<4, 2, 2, 4, 4>>(a, k_f8_tile<T, 4, 2, 2, 4, 4>, s);
+    default:
+        if constexpr (f8_exact_for<T>) return f8_tiles<T, F8Ring<4, 2, 4, 8, 2>>(a, k_f8_tile<T, 4, 2, 4, 8, 2>, s);
+        else return f8_tiles<T, F8Ring<4, 2, 4, 8, 2>>(a, k_f8_big<T>, s);
     }
 }
 
