@@ -77,7 +77,7 @@ def to_piles(x: torch.Tensor, piles: Piles) -> torch.Tensor:
             return to_piles(x, piles)
     h = x.shape[1]
     rows = x.new_empty((p.tokens * p.top_k, h))
-    check(lib().cw_to_piles(_DTYPES[x.dtype], x.data_ptr(), ld, p.tokens, p.top_k, p.n_experts, h, p.place.data_ptr(), p.offsets.data_ptr(),
+    check(lib().cw_to_piles(_DTYPES[x.dtype], x.data_ptr(), ld, p.tokens, p.top_k, p.n_experts, h, p.order.data_ptr(), p.offsets.data_ptr(),
                             rows.data_ptr(), _stream(x)))
     return rows
 

@@ -404,24 +404,24 @@ int cw_f8_matmul(const uint8_t *w, const float *w_scale, int64_t n, int64_t k, c
  * that another device holds) go to none, behind all others. A stable sort: order[pos] = the pick at a position, place[p] = the
  * position of a pick (each a permutation of 0 .. picks - 1), offsets[e] = picks of experts below e, for e = 0 .. n_experts: positions
  * from offsets[n_experts] on are those of no expert. tiles (cw_pile_tiles_bytes bytes, 16-byte aligned) receives the plan
- * that cw_f8_matmul_experts reads. ws: of cw_sort_picks_workspace_size bytes (0 for up to 65,536 picks), any contents; calls that
+ * that cw_f8_matmul_experts reads. ws: of cw_sort_picks_workspace_size bytes (0 for up to 2,048 picks), any contents; calls that
  * overlap in time need distinct ones. n_experts <= 1024; CW_ENOTSUP from 2^28 picks on. */
 int64_t cw_pile_tiles_bytes(int64_t picks, int n_experts);
 size_t cw_sort_picks_workspace_size(int64_t picks, int n_experts);
 int cw_sort_picks(const uint32_t *ids, int64_t picks, int n_experts, int32_t *order, int32_t *place, int32_t *offsets, void *tiles,
                   void *ws, size_t ws_bytes, cw_stream_t stream);
 
-/* Tokens to their experts' piles, and back: place and offsets as cw_sort_picks wrote them for T x K picks; rows of h values of type
- * dtype, of the piles' rows T x K. rows[place[t][j]] = x[t], and zeros at the positions of no expert; its gradient is
+/* Tokens to their experts' piles, and back: order, place and offsets as cw_sort_picks wrote them for T x K picks; rows of h values of
+ * type dtype, of the piles' rows T x K. rows[pos] = x[order[pos] / K], and zeros at the positions of no expert; its gradient is
  * cw_from_piles without weights of the rows' gradient. x's rows are ldx elements apart, the piles' rows h. */
-int cw_to_piles(int dtype, const void *x, int64_t ldx, int64_t T, int K, int n_experts, int64_t h, const int32_t *place,
+int cw_to_piles(int dtype, const void *x, int64_t ldx, int64_t T, int K, int n_experts, int64_t h, const int32_t *order,
                 const int32_t *offsets, void *rows, cw_stream_t stream);
 /* out[t] = sum_j w[t][j] rows[place[t][j]] (w NULL: 1), in f32 in the picks' order, rounded once; picks of no expert add nothing,
  * whatever their rows hold. The piles' rows are ldr elements apart, out's h. */
 int cw_from_piles(int dtype, const void *rows, int64_t ldr, const float *w, int64_t T, int K, int n_experts, int64_t h,
                   const int32_t *place, const int32_t *offsets, void *out, cw_stream_t stream);
-/* Its gradient: drows[place[t][j]] = w[t][j] dout[t] (rows h apart), dw[t][j] = <dout[t], rows[place[t][j]]> (f32); zeros for picks of no
- * expert. */
+/* Its gradient: drows[place[t][j]] = w[t][j] dout[t] (rows h apart), dw[t][j] = <dout[t], rows[place[t][j]]> (f32); zeros for picks of
+ * no expert. */
 int cw_from_piles_grad(int dtype, const void *dout, int64_t ldd, const void *rows, int64_t ldr, const float *w, int64_t T, int K,
                        int n_experts, int64_t h, const int32_t *place, const int32_t *offsets, void *drows, float *dw,
                        cw_stream_t stream);
