@@ -43,6 +43,7 @@ __global__ __launch_bounds__(64 * F8_FEW_WAVES) void k_f8_few(F8MatArgs a) {
     f32x4 acc[MB];
 #pragma unroll
     for (int i = 0; i < MB; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    bool strange = false;
     for (int step = wave; step < a.blocks; step += F8_FEW_WAVES) {
         const uint8_t *w = w0 + (int64_t)step * F8_BLOCK + wrow, *x = a.x + (int64_t)step * F8_BLOCK;
         F8Frag<true> wf, xf;
@@ -50,11 +51,12 @@ __global__ __launch_bounds__(64 * F8_FEW_WAVES) void k_f8_few(F8MatArgs a) {
         const float sw = ws[step];
 #pragma unroll
         for (int i = 0; i < MB; i++) {
-            const F8Scale s(a.xs[step * a.m + srow[i]], sw);
+            const float sx = a.xs[step * a.m + srow[i]], s = sx * sw;
+            strange |= f8_strange(sx) | f8_strange(sw);
             xf.load(x + xrow[i], x + xrow[i] + 64);
             const f32x4 p = F8Frag<true>::product(wf, xf);
 #pragma unroll
-            for (int c = 0; c < 4; c++) acc[i][c] = s.add(p[c], acc[i][c]);
+            for (int c = 0; c < 4; c++) acc[i][c] = fmaf(p[c], s, acc[i][c]);
         }
     }
     const int64_t m = 16 * (wave % MB) + (lane & 15), n = n0 + 4 * (lane >> 4);
@@ -63,11 +65,12 @@ __global__ __launch_bounds__(64 * F8_FEW_WAVES) void k_f8_few(F8MatArgs a) {
     for (int i = 0; i < 4; i++) b[i] = a.bias ? a.bias[min(n + i, a.n - 1)] : 0.f;
 #pragma unroll
     for (int i = 0; i < MB; i++) part[wave][i][lane] = acc[i];
-    __syncthreads();
+    strange = __syncthreads_or(strange);
     if (wave >= MB || m >= a.m || n >= a.n) return;
     f32x4 v = part[0][wave][lane];
 #pragma unroll
     for (int o = 1; o < F8_FEW_WAVES; o++) v += part[o][wave][lane];
+    if (strange) v = f8_strange_sums(a.x + m * a.rb, a.xs + m, a.m, a.w + n * a.rb, ws, a.rb, (int)min(a.n - n, (int64_t)4), v);
     f8_store4((T *)a.y + m * a.ldy + n, (int)min(a.n - n, (int64_t)4), v, b);
 }
 
@@ -92,11 +95,10 @@ struct F8Ring {
     static constexpr int LOADS = (TN + TM) / 8, PER = (LOADS + WAVES - 1) / WAVES, D = STAGES - 1, LDS = STAGES * STAGE;
     static_assert(LDS <= 159 * 1024 && SCALES / 64 <= WAVES, "the ring fits the CU, a load of scales a wave");
 };
-// xrow(r): x's row of row r < TM of the tile (any valid row past its end); n0: the tile's first row of W; w, ws: the matrix. ANY: for
-// scales of any size; else for usual ones, and true if the wave saw another (the WN waves of a row of the tile look at a WN'th of its
-// rows' scales each).
-template <class R, int NF, int MF, bool EXACT, bool ANY, class XRow>
-__device__ __forceinline__ bool f8_pass(uint8_t *lds, const F8MatArgs &a, const uint8_t *w, const float *ws, int64_t n0, XRow xrow, int wn, int wm,
+// xrow(r): x's row of row r < TM of the tile (any valid row past its end); n0: the tile's first row of W; w, ws: the matrix.
+// True if the wave saw a strange scale (the WN waves of a row of the tile look at a WN'th of its rows' scales each).
+template <class R, int NF, int MF, bool EXACT, class XRow>
+__device__ __forceinline__ bool f8_loop(uint8_t *lds, const F8MatArgs &a, const uint8_t *w, const float *ws, int64_t n0, XRow xrow, int wn, int wm,
                                         f32x4 (&acc)[MF][NF]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), steps = a.blocks;
     // a stage: TN rows of W, then TM of x, then x's scales; load i of this wave: 8 rows from 8 (wave + WAVES i) (past the last:
@@ -138,7 +140,7 @@ __device__ __forceinline__ bool f8_pass(uint8_t *lds, const F8MatArgs &a, const 
         next = next + 1 == R::D + 1 ? 0 : next + 1;
         const float sw = sw_of[step];
         const int o = buf * R::STAGE;
-        if constexpr (!ANY) odd |= !f8_usual(sw);
+        odd |= f8_strange(sw);
         F8Frag<EXACT> wf[NF], xf;
 #pragma unroll
         for (int j = 0; j < NF; j++) wf[j].load(wl + o + c0 + 2048 * j, wl + o + c1 + 2048 * j);
@@ -146,26 +148,34 @@ __device__ __forceinline__ bool f8_pass(uint8_t *lds, const F8MatArgs &a, const 
         for (int i = 0; i < MF; i++) {
             xf.load(xl + o + c0 + 2048 * i, xl + o + c1 + 2048 * i);
             const float sx = *(const float *)(sl + o + 64 * i);
-            if constexpr (!ANY)
-                if (i % R::N_WAVES == wn) odd |= !f8_usual(sx);
+            if (i % R::N_WAVES == wn) odd |= f8_strange(sx);
             const float s = sx * sw;
-            const F8Scale any(sx, sw);
 #pragma unroll
             for (int j = 0; j < NF; j++) {
                 const f32x4 p = F8Frag<EXACT>::product(wf[j], xf);
 #pragma unroll
-                for (int c = 0; c < 4; c++) acc[i][j][c] = ANY ? any.add(p[c], acc[i][j][c]) : fmaf(p[c], s, acc[i][j][c]);
+                for (int c = 0; c < 4; c++) acc[i][j][c] = fmaf(p[c], s, acc[i][j][c]);
             }
         }
         buf = buf + 1 == R::D + 1 ? 0 : buf + 1;
     }
     return odd;
 }
-template <class R, int NF, int MF, bool EXACT, class XRow>
-__device__ __forceinline__ void f8_loop(uint8_t *lds, const F8MatArgs &a, const uint8_t *w, const float *ws, int64_t n0, XRow xrow, int wn, int wm,
-                                        f32x4 (&acc)[MF][NF]) {
-    const bool odd = f8_pass<R, NF, MF, EXACT, false>(lds, a, w, ws, n0, xrow, wn, wm, acc);
-    if (__syncthreads_or(odd)) f8_pass<R, NF, MF, EXACT, true>(lds, a, w, ws, n0, xrow, wn, wm, acc);
+// A wave's sums of rows whose scales, or whose weights' scales, are strange: rows m0.. of m_end (x's: xrow), columns n0.. of the matrix w, ws
+template <int MF, int NF, class XRow>
+__device__ __forceinline__ void f8_strange_tile(const F8MatArgs &a, const uint8_t *w, const float *ws, XRow xrow, int64_t m0, int64_t m_end, int64_t n0,
+                                                f32x4 (&acc)[MF][NF]) {
+    const int lane = threadIdx.x & 63;
+    const int64_t m = m0 + (lane & 15), n = n0 + 4 * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < MF; i++)
+#pragma unroll
+        for (int j = 0; j < NF; j++) {
+            if (m + 16 * i >= m_end || n + 16 * j >= a.n) continue;
+            const int64_t row = xrow(m + 16 * i), col = n + 16 * j;
+            acc[i][j] = f8_strange_sums(a.x + row * a.rb, a.xs + row, a.m, w + col * a.rb, ws + col / F8_BLOCK * a.blocks, a.rb,
+                                        (int)min(a.n - col, (int64_t)4), acc[i][j]);
+        }
 }
 // A wave's sums stored: rows m0.. of m_end of y, columns n0.. . All biases are loaded before the bounds checks, from clamped places.
 template <class T, int MF, int NF>
@@ -186,10 +196,6 @@ __device__ __forceinline__ void f8_finish(const F8MatArgs &a, const float *bias,
     }
 }
 
-// Results in f32 have exact products, f16's and bf16's rounding covers what the 8-bit instruction leaves out.
-template <class T>
-constexpr bool f8_exact_for = std::is_same_v<T, float>;
-
 template <class T, int WN, int WM, int NF, int MF, int STAGES>
 __global__ __launch_bounds__(64 * WN *WM, WN *WM / 4) void k_f8_tile(F8MatArgs a, int tiles_m, int tiles_n) {
     using R = F8Ring<WN, WM, NF, MF, STAGES>;
@@ -198,12 +204,13 @@ __global__ __launch_bounds__(64 * WN *WM, WN *WM / 4) void k_f8_tile(F8MatArgs a
     int64_t m0, n0;
     f8_tile_of_block(tiles_m, tiles_n, R::TM, R::TN, m0, n0);
     f32x4 acc[MF][NF];
-    f8_loop<R, NF, MF, f8_exact_for<T>>(lds, a, a.w, a.ws, n0, [&](int r) { return min(m0 + r, a.m - 1); }, wn, wm, acc);
+    const bool odd = f8_loop<R, NF, MF, f8_exact_for<T>>(lds, a, a.w, a.ws, n0, [&](int r) { return min(m0 + r, a.m - 1); }, wn, wm, acc);
+    if (__syncthreads_or(odd)) f8_strange_tile(a, a.w, a.ws, [](int64_t r) { return r; }, m0 + 16 * MF * wm, a.m, n0 + 16 * NF * wn, acc);
     f8_finish<T, MF, NF>(a, a.bias, m0 + 16 * MF * wm, a.m, n0 + 16 * NF * wn, acc);
 }
 
 // Many rows of x: tiles of 256 x 256, eight waves of 64 columns x 128 rows, two to a SIMD: one multiplies while the other scales and
-// adds. Two LDS stages of 2 x 256 rows x 128 codes and 256 scales, swizzled as in f8_pass. A wave's four fragments of W stay in
+// adds. Two LDS stages of 2 x 256 rows x 128 codes and 256 scales, swizzled as in f8_loop. A wave's four fragments of W stay in
 // registers for the step, x's eight pass by, each read while the one before is multiplied; the next step's first ones while the
 // last is, before which all waves meet: the stage of the next step is then in, and this step's, all of which has been read, free for the one after.
 template <class T>
@@ -264,7 +271,7 @@ __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int
     for (int step = 0; step <= last; step++) {
         const float sw = sw_of[step];
         const int o = (step & 1) * R::STAGE, next = R::STAGE - o;
-        odd |= !f8_usual(*(const float *)(ol + o)) | !f8_usual(sw);
+        odd |= f8_strange(*(const float *)(ol + o)) | f8_strange(sw);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             if (i == 7) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -290,61 +297,47 @@ __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) add(7, j);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (no load may land in LDS that is another block's, or another pass's)
-    if (__syncthreads_or(odd)) {
-        f8_pass<R, 4, 8, false, true>(lds, a, a.w, a.ws, n0, [&](int r) { return min(m0 + r, a.m - 1); }, wn, wm, acc);
-        f8_finish<T, 8, 4>(a, a.bias, m0 + 128 * wm, a.m, n0 + 64 * wn, acc);
-        return;
-    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (no load may land in LDS that is another block's)
+    if (__syncthreads_or(odd)) f8_strange_tile(a, a.w, a.ws, [](int64_t r) { return r; }, m0 + 128 * wm, a.m, n0 + 64 * wn, acc);
     f8_finish<T, 8, 4>(a, a.bias, m0 + 128 * wm, a.m, n0 + 64 * wn, acc);
 }
 
-// The item of a block: blocks go to the eight dies in turn; each die takes a contiguous range of the items, an expert's
-// blocks of W one after the other and its tiles side by side for each, so that an expert's rows and weights are read by
-// one die and not by all, the weights once for all its tiles.
-__device__ __forceinline__ bool f8_item_of_block(const void *list, int n_blocks, PileTile &tl, int &nb) {
-    const PileTile *tiles = pile_tiles(list);
-    const int64_t total = (int64_t)*(const int *)list * n_blocks, per = total >> 3;
-    const int die = blockIdx.x & 7, at = blockIdx.x >> 3, rest = (int)(total & 7);
-    if (at >= per + (die < rest)) return false;
-    const int64_t item = die * per + min(die, rest) + at;
-    const PileTile any = tiles[__builtin_amdgcn_readfirstlane((int)(item / n_blocks))];  // a tile of the item's expert
-    const int in = (int)(item - (int64_t)any.first * n_blocks);
-    nb = __builtin_amdgcn_readfirstlane(in / any.of);
-    if (any.of == 1) tl = any;
-    else tl = tiles[__builtin_amdgcn_readfirstlane(any.first + in - nb * any.of)];
-    return true;
-}
-
-template <class T, int MF, int STAGES>
-__device__ __forceinline__ void f8_expert_tile(const F8MatArgs &a, const PileTile &tl, int64_t n0, uint8_t *lds) {
-    using R = F8Ring<8, 1, 1, MF, STAGES>;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    f32x4 acc[MF][1];
-    f8_loop<R, 1, MF, f8_exact_for<T>>(lds, a, a.w + tl.expert * a.w_stride, a.ws + tl.expert * a.ws_stride, n0,
-                      [&](int r) {
-                          const int pos = tl.pos0 + min(r, tl.m - 1);
-                          return (int64_t)(a.order ? a.order[pos] / a.K : pos);
-                      },
-                      wave, 0, acc);
-    f8_finish<T, MF, 1>(a, a.bias ? a.bias + tl.expert * a.n : nullptr, tl.pos0, tl.pos0 + tl.m, n0 + 16 * wave, acc);
-}
-template <class T>
-__global__ __launch_bounds__(512, 2) void k_f8_experts(F8MatArgs a, int n_blocks) {
+// Sorted rows times their experts' matrices: a tile of up to 128 positions, 64 NW columns.
+template <class T, int NW, bool EXACT>
+__global__ __launch_bounds__(256, 2) void k_f8_experts(F8MatArgs a, int n_blocks) {
     extern __shared__ __align__(1024) uint8_t lds[];
     PileTile tl;
     int nb;
     if (!f8_item_of_block(a.tiles, n_blocks, tl, nb)) return;
-    const int64_t n0 = (int64_t)128 * nb;
+    constexpr int COLS = 64 * NW;
+    const int lane = threadIdx.x & 63;
     if (tl.expert == a.E) {  // positions of no expert: zeros
-        const int cols = (int)min(a.n - n0, (int64_t)128);
-        for (int i = threadIdx.x; i < tl.m * cols; i += 512) ((T *)a.y)[(int64_t)(tl.pos0 + i / cols) * a.ldy + n0 + i % cols] = from_f32<T>(0.f);
+        const int64_t n0 = (int64_t)COLS * nb;
+        const int cols = (int)min(a.n - n0, (int64_t)COLS);
+        for (int i = threadIdx.x; i < tl.m * cols; i += 256) ((T *)a.y)[(int64_t)(tl.pos0 + i / cols) * a.ldy + n0 + i % cols] = from_f32<T>(0.f);
         return;
     }
-    if (tl.m <= 16) f8_expert_tile<T, 1, 8>(a, tl, n0, lds);
-    else if (tl.m <= 32) f8_expert_tile<T, 2, 7>(a, tl, n0, lds);
-    else if (tl.m <= 64) f8_expert_tile<T, 4, 6>(a, tl, n0, lds);
-    else f8_expert_tile<T, 8, 4>(a, tl, n0, lds);
+    const int64_t n0 = (int64_t)COLS * nb + 16 * NW * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_in = min(n0, a.n - 1);
+    F8Operands<1> o;
+    o.x = a.x;
+    o.xs = a.xs;
+    o.m = a.m;
+    o.rb = a.rb;
+    o.blocks = a.blocks;
+    o.w0[0] = a.w + tl.expert * a.w_stride + n_in * a.rb;
+    o.ws0[0] = a.ws + tl.expert * a.ws_stride + n_in / F8_BLOCK * a.blocks;
+    uint32_t wrow[NW];
+#pragma unroll
+    for (int j = 0; j < NW; j++) wrow[j] = (uint32_t)min((int64_t)(16 * j + (lane & 15)), a.n - 1 - n_in) * (uint32_t)a.rb + 16 * (lane >> 4);
+    f8_by_height(tl.m, [&](auto mb) __attribute__((always_inline)) {
+        constexpr int MB = decltype(mb)::value;
+        f32x4 acc[MB][NW];
+        auto row_at = [&](int64_t pos) __attribute__((always_inline)) { return a.order ? (int64_t)(a.order[pos] / a.K) : pos; };
+        const bool odd = f8_stream<MB, NW, 1, EXACT>(lds, o, [&](int r) { return row_at(tl.pos0 + min(r, tl.m - 1)); }, wrow, acc);
+        if (__syncthreads_or(odd))
+            f8_strange_tile(a, a.w + tl.expert * a.w_stride, a.ws + tl.expert * a.ws_stride, row_at, tl.pos0, tl.pos0 + tl.m, n0, acc);
+        f8_finish<T, MB, NW>(a, a.bias ? a.bias + tl.expert * a.n : nullptr, tl.pos0, tl.pos0 + tl.m, n0, acc);
+    });
 }
 
 // dynamic LDS above 64 KB, opted into once per kernel and device
@@ -380,13 +373,14 @@ static int f8_matmul(const F8MatArgs &a, int few_groups, int tile_of, hipStream_
     }
 }
 
-template <class T>
-static int f8_experts(const F8MatArgs &a, int64_t tiles, hipStream_t s) {
-    constexpr int LDS = std::max({F8Ring<8, 1, 1, 1, 8>::LDS, F8Ring<8, 1, 1, 2, 7>::LDS, F8Ring<8, 1, 1, 4, 6>::LDS, F8Ring<8, 1, 1, 8, 4>::LDS});
-    const int blocks = (int)((a.n + 127) / 128);
-    if (int rc = f8_allow_lds<T, 0>((const void *)k_f8_experts<T>, LDS)) return rc;
-    hipLaunchKernelGGL(k_f8_experts<T>, dim3((unsigned)((tiles * blocks + 7) / 8 * 8)), dim3(512), LDS, s, a, blocks);
-    return check_launch("k_f8_experts");
+template <class T, bool EXACT>
+static int f8_experts(const F8MatArgs &a, int64_t tiles, bool four, hipStream_t s) {
+    auto go = [&](auto kernel, int nw, int lds) {
+        const int blocks = (int)((a.n + 64 * nw - 1) / (64 * nw));
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles * blocks + 7) / 8 * 8)), dim3(256), lds, s, a, blocks);
+        return check_launch("k_f8_experts");
+    };
+    return four ? go(k_f8_experts<T, 4, EXACT>, 4, F8Stream<8, 4>::LDS) : go(k_f8_experts<T, 2, EXACT>, 2, F8Stream<8, 2>::LDS);
 }
 
 static int check_product(const char *what, int ydtype, int64_t n, int64_t k, int64_t m, int64_t ldy) {
@@ -415,6 +409,33 @@ static F8MatArgs product_args(const uint8_t *w, const float *w_scale, int64_t n,
     return a;
 }
 
+int f8_matmul_experts(const uint8_t *w, int64_t w_stride, const float *w_scale, int n_experts, int64_t n, int64_t k, const uint8_t *x,
+                         const float *x_scale, int64_t m, const int32_t *order, int K, int64_t picks, const void *tiles, const float *bias,
+                         int ydtype, void *y, int64_t ldy, bool exact, hipStream_t s) {
+    if (int rc = check_product("f8_matmul_experts", ydtype, n, k, m, ldy)) return rc;
+    CW_REQUIRE(n_experts > 0 && n_experts <= PILE_MAX_EXPERTS, "f8_matmul_experts: %d experts (1..%d supported)", n_experts, PILE_MAX_EXPERTS);
+    CW_REQUIRE(K > 0 && picks >= 0 && picks < 1 << 28, "f8_matmul_experts: %lld picks, %d a token", (long long)picks, K);
+    CW_REQUIRE(order ? m * K == picks : m == picks, "f8_matmul_experts: %lld rows of x for %lld picks, %d a token", (long long)m, (long long)picks, K);
+    CW_REQUIRE(w_stride >= n * f8_row_bytes(k) && w_stride % 16 == 0, "f8_matmul_experts: %lld bytes from an expert's matrix to the next",
+               (long long)w_stride);
+    const int64_t most = pile_max_tiles(picks, n_experts);
+    if (most * ((n + 127) / 128) >= 1 << 23) return set_error(CW_ENOTSUP, "f8_matmul_experts: %lld picks of %lld outputs", (long long)picks, (long long)n);
+    if (picks == 0) return CW_OK;
+    CW_REQUIRE(w && w_scale && x && x_scale && tiles && y, "f8_matmul_experts: null pointer");
+    CW_REQUIRE(f8_aligned(w, 16) && f8_aligned(x, 16) && f8_aligned(tiles, 16), "f8_matmul_experts: codes and tiles must be 16-byte aligned");
+    F8MatArgs a = product_args(w, w_scale, n, k, x, x_scale, m, bias, y, ldy);
+    a.w_stride = w_stride;
+    a.ws_stride = f8_blocks(n) * f8_blocks(k);
+    a.tiles = tiles;
+    a.order = order;
+    a.K = K;
+    a.E = n_experts;
+    const bool four = f8_four_groups(n_experts, picks, n, (int)resident_blocks(1));
+    if (ydtype == CW_F16) return f8_experts<_Float16, false>(a, most, four, s);
+    if (ydtype == CW_BF16) return f8_experts<bf16_t, false>(a, most, four, s);
+    return exact ? f8_experts<float, true>(a, most, four, s) : f8_experts<float, false>(a, most, four, s);
+}
+
 }  // namespace cw
 
 using namespace cw;
@@ -439,28 +460,8 @@ int cw_f8_matmul(const uint8_t *w, const float *w_scale, int64_t n, int64_t k, c
 int cw_f8_matmul_experts(const uint8_t *w, int64_t w_stride, const float *w_scale, int n_experts, int64_t n, int64_t k, const uint8_t *x,
                          const float *x_scale, int64_t m, const int32_t *order, int K, int64_t picks, const void *tiles, const float *bias,
                          int ydtype, void *y, int64_t ldy, cw_stream_t stream) {
-    if (int rc = check_product("f8_matmul_experts", ydtype, n, k, m, ldy)) return rc;
-    CW_REQUIRE(n_experts > 0 && n_experts <= PILE_MAX_EXPERTS, "f8_matmul_experts: %d experts (1..%d supported)", n_experts, PILE_MAX_EXPERTS);
-    CW_REQUIRE(K > 0 && picks >= 0 && picks < 1 << 28, "f8_matmul_experts: %lld picks, %d a token", (long long)picks, K);
-    CW_REQUIRE(order ? m * K == picks : m == picks, "f8_matmul_experts: %lld rows of x for %lld picks, %d a token", (long long)m, (long long)picks, K);
-    CW_REQUIRE(w_stride >= n * f8_row_bytes(k) && w_stride % 16 == 0, "f8_matmul_experts: %lld bytes from an expert's matrix to the next",
-               (long long)w_stride);
-    const int64_t most = pile_max_tiles(picks, n_experts);
-    if (most * ((n + 127) / 128) >= 1 << 23) return set_error(CW_ENOTSUP, "f8_matmul_experts: %lld picks of %lld outputs", (long long)picks, (long long)n);
-    if (picks == 0) return CW_OK;
-    CW_REQUIRE(w && w_scale && x && x_scale && tiles && y, "f8_matmul_experts: null pointer");
-    CW_REQUIRE(f8_aligned(w, 16) && f8_aligned(x, 16) && f8_aligned(tiles, 16), "f8_matmul_experts: codes and tiles must be 16-byte aligned");
-    F8MatArgs a = product_args(w, w_scale, n, k, x, x_scale, m, bias, y, ldy);
-    a.w_stride = w_stride;
-    a.ws_stride = f8_blocks(n) * f8_blocks(k);
-    a.tiles = tiles;
-    a.order = order;
-    a.K = K;
-    a.E = n_experts;
-    hipStream_t s = (hipStream_t)stream;
-    if (ydtype == CW_F16) return f8_experts<_Float16>(a, most, s);
-    if (ydtype == CW_BF16) return f8_experts<bf16_t>(a, most, s);
-    return f8_experts<float>(a, most, s);
+    return f8_matmul_experts(w, w_stride, w_scale, n_experts, n, k, x, x_scale, m, order, K, picks, tiles, bias, ydtype, y, ldy, ydtype == CW_F32,
+                             (hipStream_t)stream);
 }
 
 }  // extern "C"

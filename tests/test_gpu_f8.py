@@ -319,6 +319,8 @@ def test_all_on_one_expert(t, pick):
 
 
 def check_layer(t, e, kp, h, i, dtype, act, norm=True, seed=0):
+    # the 8-bit instruction's products (check_product) make gate and up of bf16 results, and down of bf16 and f16 ones
+    less = [2.0 ** -15 if dtype == torch.bfloat16 else 0.0, 0.0 if dtype == torch.float32 else 2.0 ** -15]
     g = gen(seed + t + h)
     banks = [rand_bank(g, e, *s) for s in ((i, h), (i, h), (h, i))]
     for b in banks:
@@ -339,7 +341,7 @@ def check_layer(t, e, kp, h, i, dtype, act, norm=True, seed=0):
         gate, up, down = (matrix_values(b.q[x_], b.scale[x_], b.k) for b in banks)
         gb, ub, db = (0.0 if b is None else b[x_].double() for b in biases)
         gv, uv = xv[tok] @ gate.t() + gb, xv[tok] @ up.t() + ub
-        ge, ue = (sums_off(h) * (xv[tok].abs() @ m.abs().t()) + 2 * U * v.abs() for m, v in ((gate, gv), (up, uv)))
+        ge, ue = ((sums_off(h) + less[0]) * (xv[tok].abs() @ m.abs().t()) + 2 * U * v.abs() for m, v in ((gate, gv), (up, uv)))
         hv = glu64(gv, uv, act)
         # the activation's slope in g is at most 1.1 |u| (2 |u + 1| of the clamped form), in u |silu(g)| <= |g|; its own roundings
         he = ge * 2 * (uv.abs() + 1) + ue * gv.abs() + 12 * U * (gv.abs() * (uv.abs() + 1))
@@ -355,7 +357,7 @@ def check_layer(t, e, kp, h, i, dtype, act, norm=True, seed=0):
         hq, s = (code * a / 448).view(hv.shape[0], -1)[:, :i], a / 448
         ho = (far * s + code.abs() * s * (U + ae / a)).view(hv.shape[0], -1)[:, :i]
         y = hq @ down.t() + db
-        yo = ho @ down.abs().t() + sums_off(i) * (hq.abs() @ down.abs().t()) + U * y.abs()
+        yo = ho @ down.abs().t() + (sums_off(i) + less[1]) * (hq.abs() @ down.abs().t()) + U * y.abs()
         wt = w[tok, j].double()[:, None]
         want.index_add_(0, tok, wt * y)
         off.index_add_(0, tok, wt * (yo + 2 * U * kp * y.abs()))
