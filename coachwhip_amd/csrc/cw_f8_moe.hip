@@ -2,8 +2,250 @@
 #include <algorithm>
 
 #include "cw_f8_tile.h"
+#include "cw_i8_rules.h"
+#include "cw_mfma.h"
 
 namespace cw {
+
+// ------------------------------------------------------------------------------ a few tokens
+
+struct F8FewArgs {
+    const uint8_t *w[3], *x;
+    const float *ws[3], *bias[3], *xs, *logits;
+    int64_t stride[3];
+    int E, K, H, I, T, norm;
+    Glu glu;
+    int rbh, rbi, ldh;  // bytes of a row of H and of I codes, floats of a hidden row
+    uint32_t *ids;
+    float *wt, *h;
+    void *out;
+};
+
+// 16 codes as f16, and the sum of 16 products with them
+struct F8Half16 {
+    f16x2 v[8];
+    __device__ __forceinline__ F8Half16() {}
+    __device__ __forceinline__ F8Half16(i32x4 q) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((uint32_t)q[i], 1.0f, false);
+            v[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((uint32_t)q[i], 1.0f, true);
+        }
+    }
+    __device__ __forceinline__ float dot(i32x4 q) const {
+        const F8Half16 o(q);
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) s = __builtin_amdgcn_fdot2(v[i], o.v[i], s, false);
+        return s;
+    }
+};
+
+// Gate and up of one pick of a token, eight waves of R rows of both matrices each: lane l takes the 16 bytes l, l + 64, ... of each row and of
+// x, which lie in one block of 128 each. Sums of 16 products in f32, scaled and added in 64 bits (one operation for 16 products). One wave routes the
+// token for its block, no further than this pick; the last pick's first block, which goes all the way, stores the routing.
+template <int PER, int NC, int R>
+__global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_f8_few_gateup(F8FewArgs a) {
+    __shared__ uint32_t expert;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.z, j = blockIdx.y;
+    const int r0 = (blockIdx.x * I8_FEW_WAVES + wave) * R, blocks = a.rbh / F8_BLOCK;
+    if (wave == 0) {
+        uint32_t id;
+        float wt;
+        wave_route<PER>(a.logits + (int64_t)t * a.E, a.E, j + 1, a.norm, &id, &wt);
+        if (blockIdx.x == 0 && j == a.K - 1 && lane < a.K) {
+            a.ids[(int64_t)t * a.K + lane] = id;
+            a.wt[(int64_t)t * a.K + lane] = wt;
+        }
+        if (lane == j) expert = id;
+    }
+    F8Half16 x[NC];
+    int off[NC];
+    float sx[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int o = 16 * (lane + 64 * c);
+        off[c] = o < a.rbh ? o : 0;  // past the row: any valid bytes, times zeros
+        i32x4 q = *(const i32x4 *)(a.x + (int64_t)t * a.rbh + off[c]);
+        sx[c] = a.xs[(int64_t)(off[c] / F8_BLOCK) * a.T + t];
+        if (o >= a.rbh) {
+            q = i32x4{0, 0, 0, 0};
+            sx[c] = 0.f;
+        }
+        x[c] = F8Half16(q);
+    }
+    __syncthreads();
+    if (r0 >= a.I) return;
+    const int64_t e = __builtin_amdgcn_readfirstlane((int)expert);
+    const int64_t mine = e * a.I + min(r0 + (lane & (R - 1)), a.I - 1);  // lane r < R ends row r0 + r
+    float b[2], sw[2][NC];
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+        b[m] = a.bias[m] ? a.bias[m][mine] : 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; c++) sw[m][c] = a.ws[m][(e * ((a.I + 127) / 128) + r0 / F8_BLOCK) * blocks + off[c] / F8_BLOCK];
+    }
+    i32x4 g[R][NC], u[R][NC];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int row = min(r0 + r, a.I - 1);
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            g[r][c] = *(const i32x4 *)(a.w[0] + e * a.stride[0] + (int64_t)row * a.rbh + off[c]);
+            u[r][c] = *(const i32x4 *)(a.w[1] + e * a.stride[1] + (int64_t)row * a.rbh + off[c]);
+        }
+    }
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        double sg = 0.0, su = 0.0;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            sg = fma((double)x[c].dot(g[r][c]), (double)sx[c] * sw[0][c], sg);
+            su = fma((double)x[c].dot(u[r][c]), (double)sx[c] * sw[1][c], su);
+        }
+        const float fg = (float)wave_sum_d(sg), fu = (float)wave_sum_d(su);
+        sum[0] = lane == r ? fg : sum[0];
+        sum[1] = lane == r ? fu : sum[1];
+    }
+    const float h = glu(sum[0] + b[0], sum[1] + b[1], a.glu);
+    if (lane < R && r0 + lane < a.I) a.h[((int64_t)t * a.K + j) * a.ldh + r0 + lane] = h;
+}
+
+// Down and the weighted sum of a token: the block makes the token's K hidden rows codes in LDS (every block of the token does, one, two, four or
+// eight waves a row; 32 lanes hold a group of 128 columns), then each wave sums R outputs: lane l holds the 16 bytes l, l + 64, ... of the
+// K rows' codes laid end to end. The hidden rows are asked for before the weights: loads return in order, and the codes are made while the
+// weights come in.
+template <class T, int NC, int R>
+__global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 || R == 4 ? 4 : NC == 4 ? 6 : 8) void k_f8_few_down(F8FewArgs a) {
+    constexpr int NH = NC < 12 ? (NC + 1) / 2 : 6;  // pieces of a hidden row held in registers (the others are read later)
+    extern __shared__ __align__(16) uint8_t hq[];  // K rows of rbi codes, then their scales
+    __shared__ float wk[32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.y, cpr = a.rbi / 16, blocks = a.rbi / F8_BLOCK;
+    float *hs = (float *)(hq + a.K * a.rbi);
+    const int row0 = (blockIdx.x * I8_FEW_WAVES + wave) * R, nb = min(row0, a.H - 1) / F8_BLOCK;
+    const int wpp = a.K > 4 ? 1 : a.K > 2 ? 2 : a.K > 1 ? 4 : 8, at0 = 4 * ((wave & (wpp - 1)) * 64 + lane), stride = 256 * wpp;
+    const float *h = a.h + (int64_t)t * a.K * a.ldh;
+    float hv[NH][4];
+    auto fetch_h = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NH; i++) load_row<4>(h + (int64_t)j * a.ldh + at0 + i * stride, a.I - at0 - i * stride, hv[i]);
+    };
+    fetch_h(min(wave / wpp, a.K - 1));
+    const uint32_t *ids = a.ids + (int64_t)t * a.K;
+    const float *wt = a.wt + (int64_t)t * a.K;
+    i32x4 w[R][NC];
+    float sd[NC];  // of each chunk: its weights' scale
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int i = min(lane + 64 * c, a.K * cpr - 1), pick = i / cpr, o = i - pick * cpr;
+        const int64_t e = ids[pick];
+        const uint8_t *p = a.w[2] + e * a.stride[2] + 16 * o;
+#pragma unroll
+        for (int r = 0; r < R; r++) w[r][c] = *(const i32x4 *)(p + (int64_t)min(row0 + r, a.H - 1) * a.rbi);
+        sd[c] = a.ws[2][(e * ((a.H + 127) / 128) + nb) * blocks + o / 8];
+    }
+    // lane j < K: the pick's weight and bias
+    const int mine = min(lane, a.K - 1);
+    const float wj = wt[mine];
+    if (wave == 0 && lane < a.K) wk[lane] = wj;
+    float b[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) b[r] = a.bias[2] && lane < a.K ? a.bias[2][(int64_t)ids[mine] * a.H + min(row0 + r, a.H - 1)] : 0.f;
+    for (int j0 = 0; j0 < a.K; j0 += I8_FEW_WAVES / wpp) {
+        const int j = j0 + wave / wpp;
+        const float *row = h + (int64_t)min(j, a.K - 1) * a.ldh;
+        if (j0) fetch_h(min(j, a.K - 1));
+        if (j >= a.K) continue;
+        auto store = [&](int at, const float (&v)[4]) __attribute__((always_inline)) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) bits = max_bits(bits, v[i]);
+            bits = max16_u(bits);
+            bits = max(bits, (uint32_t)__shfl_xor((int)bits, 16));  // (the 32 lanes of a group are all in the row's codes, or none)
+            if (at >= a.rbi) return;
+            const F8Group g(bits);
+            *(uint32_t *)(hq + j * a.rbi + at) = f8_codes4(g.quotient(v[0]), g.quotient(v[1]), g.quotient(v[2]), g.quotient(v[3]));
+            if ((lane & 31) == 0) hs[j * blocks + at / F8_BLOCK] = g.scale;
+        };
+#pragma unroll
+        for (int i = 0; i < NH; i++) store(at0 + i * stride, hv[i]);
+        for (int at = at0 + NH * stride; at - 4 * lane < a.rbi; at += stride) {
+            float v[4];
+            load_row<4>(row + at, a.I - at, v);
+            store(at, v);
+        }
+    }
+    __syncthreads();
+    if (row0 >= a.H) return;
+    double acc[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) acc[r] = (double)wj * b[r];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int i = lane + 64 * c;
+        if (i < a.K * cpr) {
+            const F8Half16 x(*(const i32x4 *)(hq + 16 * i));
+            const double s = (double)wk[i / cpr] * sd[c] * hs[i / 8];
+#pragma unroll
+            for (int r = 0; r < R; r++) acc[r] = fma((double)x.dot(w[r][c]), s, acc[r]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const float v = (float)wave_sum_d(acc[r]);
+        if (lane == 0 && row0 + r < a.H) ((T *)a.out)[(int64_t)t * a.H + row0 + r] = from_f32<T>(v);
+    }
+}
+
+template <class T, int NC>
+static int few_down(const F8FewArgs &a, hipStream_t s) {
+    const int r = i8_down_rows(NC, a.H, a.T, (int)resident_blocks(1));
+    auto go = [&](auto kernel) {
+        const int per = I8_FEW_WAVES * r;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.H + per - 1) / per), a.T), dim3(64 * I8_FEW_WAVES), a.K * (a.rbi + a.rbi / 32), s, a);
+        return check_launch("k_f8_few_down");
+    };
+    if constexpr (NC <= 4)
+        if (r == 4) return go(k_f8_few_down<T, NC, 4>);
+    if constexpr (NC <= 8)
+        if (r == 2) return go(k_f8_few_down<T, NC, 2>);
+    return go(k_f8_few_down<T, NC, 1>);
+}
+template <class T>
+static int few_down(const F8FewArgs &a, hipStream_t s) {
+    switch (i8_down_pieces(a.K, a.rbi)) {
+    case 1: return few_down<T, 1>(a, s);
+    case 2: return few_down<T, 2>(a, s);
+    case 4: return few_down<T, 4>(a, s);
+    case 8: return few_down<T, 8>(a, s);
+    case 12: return few_down<T, 12>(a, s);
+    default: return few_down<T, 16>(a, s);
+    }
+}
+template <int PER, int NC>
+static int few_gateup(const F8FewArgs &a, hipStream_t s) {
+    const int r = i8_gateup_rows(NC, a.I, a.T * a.K, (int)resident_blocks(1));
+    auto go = [&](auto kernel) {
+        const int per = I8_FEW_WAVES * r;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.I + per - 1) / per), a.K, a.T), dim3(64 * I8_FEW_WAVES), 0, s, a);
+        return check_launch("k_f8_few_gateup");
+    };
+    if constexpr (NC <= 2)
+        if (r == 4) return go(k_f8_few_gateup<PER, NC, 4>);
+    return r == 2 ? go(k_f8_few_gateup<PER, NC, 2>) : go(k_f8_few_gateup<PER, NC, 1>);
+}
+template <int PER>
+static int few_gateup(const F8FewArgs &a, hipStream_t s) {
+    switch (i8_gateup_pieces(a.rbh)) {
+    case 1: return few_gateup<PER, 1>(a, s);
+    case 2: return few_gateup<PER, 2>(a, s);
+    case 3: return few_gateup<PER, 3>(a, s);
+    default: return few_gateup<PER, 4>(a, s);
+    }
+}
+
+// ------------------------------------------------------------------------------ many tokens
 
 struct F8GateUpArgs {
     const uint8_t *w[2], *x;
@@ -101,7 +343,8 @@ __global__ __launch_bounds__(256, 2) void k_f8_gateup(F8GateUpArgs a, int n_bloc
 }
 
 struct F8MoeLayout {
-    size_t ids, w, order, place, offsets, tiles, sort, hq, hs, dn, total;
+    size_t ids, w, h, order, place, offsets, tiles, sort, hq, hs, dn, total;
+    bool few;
 };
 
 static F8MoeLayout layout(const cw_f8_moe_desc *d, int T) {
@@ -111,6 +354,12 @@ static F8MoeLayout layout(const cw_f8_moe_desc *d, int T) {
     const size_t TK = (size_t)T * d->top_k;
     take(L.ids, TK * 4);
     take(L.w, TK * 4);
+    L.few = i8_few_tokens(d->n_experts, d->top_k, d->hidden, d->inter, T);
+    if (L.few) {
+        take(L.h, TK * ((d->inter + 3) & ~3) * 4);
+        L.total = off;
+        return L;
+    }
     take(L.order, TK * 4);
     take(L.place, TK * 4);
     take(L.offsets, (size_t)(d->n_experts + 1) * 4);
@@ -176,9 +425,38 @@ int cw_f8_moe_layer(const cw_f8_moe_desc *d, const uint8_t *x, const float *x_sc
     int32_t *order = (int32_t *)(base + L.order), *place = (int32_t *)(base + L.place), *offsets = (int32_t *)(base + L.offsets);
     void *tiles = base + L.tiles;
     uint8_t *hq = base + L.hq;
+    hipStream_t s = (hipStream_t)stream;
+    if (L.few) {
+        F8FewArgs a = {};
+        for (int m = 0; m < 3; m++) {
+            a.w[m] = d->w[m];
+            a.stride[m] = d->slot_stride[m];
+            a.ws[m] = d->scale[m];
+            a.bias[m] = d->bias[m];
+        }
+        a.x = x;
+        a.xs = x_scale;
+        a.logits = logits;
+        a.E = E;
+        a.K = K;
+        a.H = H;
+        a.I = I;
+        a.T = T;
+        a.norm = d->norm;
+        a.glu = glu_of(d->act, d->alpha, d->limit);
+        a.rbh = (int)f8_row_bytes(H);
+        a.rbi = (int)f8_row_bytes(I);
+        a.ldh = (I + 3) & ~3;
+        a.ids = ids;
+        a.wt = w;
+        a.h = (float *)(base + L.h);
+        a.out = out;
+        const int per = i8_route_width(E);
+        if (int rc = per == 4 ? few_gateup<4>(a, s) : per == 8 ? few_gateup<8>(a, s) : few_gateup<16>(a, s)) return rc;
+        return ydtype == CW_F16 ? few_down<_Float16>(a, s) : ydtype == CW_BF16 ? few_down<bf16_t>(a, s) : few_down<float>(a, s);
+    }
     if (int rc = cw_route_topk(logits, T, E, K, d->norm, ids, w, stream)) return rc;
     if (int rc = cw_sort_picks(ids, TK, E, order, place, offsets, tiles, base + L.sort, cw_sort_picks_workspace_size(TK, E), stream)) return rc;
-    hipStream_t s = (hipStream_t)stream;
     F8GateUpArgs a = {};
     for (int m = 0; m < 2; m++) {
         a.w[m] = d->w[m];

@@ -251,19 +251,24 @@ __global__ __launch_bounds__(256) void k_from_piles(PileArgs a) {
         const int t = (int)((uint64_t)i / (uint32_t)a.per), e = 8 * (int)(i - (int64_t)t * a.per), valid = a.h - e;
         const int64_t p0 = (int64_t)t * a.K;
         float acc[8] = {};
-        for (int j = 0; j < a.K; j++) {
-            const int pos = a.place[p0 + j];
-            if (pos >= here) continue;
-            float v[8];
-            load_row<8>((const T *)a.y + (int64_t)pos * a.ldy + e, valid, v);
-            if constexpr (WEIGHTS) {
-                const float w = a.w[p0 + j];
+        // four picks at a time, their loads together (a pick of no expert: any row, not used)
+        for (int j0 = 0; j0 < a.K; j0 += 4) {
+            float v[4][8], w[4];
+            int pos[4];
 #pragma unroll
-                for (int c = 0; c < 8; c++) acc[c] = fmaf(w, v[c], acc[c]);
-            } else {
-#pragma unroll
-                for (int c = 0; c < 8; c++) acc[c] += v[c];
+            for (int u = 0; u < 4; u++) {
+                const int j = min(j0 + u, a.K - 1);
+                pos[u] = a.place[p0 + j];
+                w[u] = WEIGHTS ? a.w[p0 + j] : 1.f;
+                if (j0 + u >= a.K) pos[u] = here;
             }
+#pragma unroll
+            for (int u = 0; u < 4; u++) load_row<8>((const T *)a.y + (int64_t)min(pos[u], max(here - 1, 0)) * a.ldy + e, valid, v[u]);
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (pos[u] < here)
+#pragma unroll
+                    for (int c = 0; c < 8; c++) acc[c] = fmaf(w[u], v[u][c], acc[c]);
         }
         store_row<8>((O *)a.out + (int64_t)t * a.h + e, valid, acc);
     }
