@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "cw_f8_tile.h"
+#include "cw_f8_rules.h"
 #include "cw_i8_rules.h"
 #include "cw_mfma.h"
 
@@ -21,34 +22,16 @@ struct F8FewArgs {
     void *out;
 };
 
-// 16 codes as f16, and the sum of 16 products with them
-struct F8Half16 {
-    f16x2 v[8];
-    __device__ __forceinline__ F8Half16() {}
-    __device__ __forceinline__ F8Half16(i32x4 q) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((uint32_t)q[i], 1.0f, false);
-            v[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((uint32_t)q[i], 1.0f, true);
-        }
-    }
-    __device__ __forceinline__ float dot(i32x4 q) const {
-        const F8Half16 o(q);
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) s = __builtin_amdgcn_fdot2(v[i], o.v[i], s, false);
-        return s;
-    }
-};
-
-// Gate and up of one pick of a token, eight waves of R rows of both matrices each: lane l takes the 16 bytes l, l + 64, ... of each row and of
-// x, which lie in one block of 128 each. Sums of 16 products in f32, scaled and added in 64 bits (one operation for 16 products). One wave routes the
-// token for its block, no further than this pick; the last pick's first block, which goes all the way, stores the routing.
-template <int PER, int NC, int R>
-__global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_f8_few_gateup(F8FewArgs a) {
+// Gate and up of one pick of a token, 16 columns a block: 16 rows of either matrix against the token's row (in all 16 columns of the
+// instruction: its sums cost nothing here, unpacking the codes for the vector unit 1.3 times the bytes' time), the steps of 128
+// codes dealt to eight waves, even ones gate, odd ones up, their sums joined in LDS in the waves' order. One wave routes the token for its block, no
+// further than this pick; the last pick's first block, which goes all the way, stores the routing.
+template <int PER, int NS, bool EXACT>
+__global__ __launch_bounds__(64 * F8_FEW_WAVES, NS > 4 ? 2 : 4) void k_f8_few_gateup(F8FewArgs a) {
     __shared__ uint32_t expert;
+    __shared__ float part[F8_FEW_WAVES][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.z, j = blockIdx.y;
-    const int r0 = (blockIdx.x * I8_FEW_WAVES + wave) * R, blocks = a.rbh / F8_BLOCK;
+    const int n0 = blockIdx.x * 16, blocks = a.rbh / F8_BLOCK, m = wave & 1, at = 16 * (lane >> 4);
     if (wave == 0) {
         uint32_t id;
         float wt;
@@ -59,71 +42,66 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES) void k_f8_few_gateup(F8FewArgs a
         }
         if (lane == j) expert = id;
     }
-    F8Half16 x[NC];
-    int off[NC];
-    float sx[NC];
+    F8Frag<EXACT> x[NS], w[NS];
+    float s[NS];
+    auto step_of = [&](int i) __attribute__((always_inline)) { return (wave >> 1) + F8_FEW_WAVES / 2 * i; };
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const int o = 16 * (lane + 64 * c);
-        off[c] = o < a.rbh ? o : 0;  // past the row: any valid bytes, times zeros
-        i32x4 q = *(const i32x4 *)(a.x + (int64_t)t * a.rbh + off[c]);
-        sx[c] = a.xs[(int64_t)(off[c] / F8_BLOCK) * a.T + t];
-        if (o >= a.rbh) {
-            q = i32x4{0, 0, 0, 0};
-            sx[c] = 0.f;
-        }
-        x[c] = F8Half16(q);
+    for (int i = 0; i < NS; i++) {
+        const int step = min(step_of(i), blocks - 1);
+        const uint8_t *p = a.x + (int64_t)t * a.rbh + step * F8_BLOCK + at;
+        x[i].load(p, p + 64);
+        s[i] = a.xs[(int64_t)step * a.T + t];
     }
     __syncthreads();
-    if (r0 >= a.I) return;
     const int64_t e = __builtin_amdgcn_readfirstlane((int)expert);
-    const int64_t mine = e * a.I + min(r0 + (lane & (R - 1)), a.I - 1);  // lane r < R ends row r0 + r
-    float b[2], sw[2][NC];
+    const uint8_t *row = a.w[m] + e * a.stride[m] + (int64_t)min(n0 + (lane & 15), a.I - 1) * a.rbh + at;
+    const float *ws = a.ws[m] + (e * ((a.I + 127) / 128) + n0 / F8_BLOCK) * blocks;
+    bool strange = false;
 #pragma unroll
-    for (int m = 0; m < 2; m++) {
-        b[m] = a.bias[m] ? a.bias[m][mine] : 0.f;
-#pragma unroll
-        for (int c = 0; c < NC; c++) sw[m][c] = a.ws[m][(e * ((a.I + 127) / 128) + r0 / F8_BLOCK) * blocks + off[c] / F8_BLOCK];
+    for (int i = 0; i < NS; i++) {
+        const int step = min(step_of(i), blocks - 1);
+        const uint8_t *p = row + step * F8_BLOCK;
+        w[i].load(p, p + 64);
+        const float sw = ws[step];
+        strange |= f8_strange(s[i]) | f8_strange(sw);
+        s[i] = step_of(i) < blocks ? s[i] * sw : 0.f;  // (past the end the last step again, times nothing)
     }
-    i32x4 g[R][NC], u[R][NC];
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        const int row = min(r0 + r, a.I - 1);
+    for (int i = 0; i < NS; i++) {
+        const f32x4 p = F8Frag<EXACT>::product(w[i], x[i]);
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            g[r][c] = *(const i32x4 *)(a.w[0] + e * a.stride[0] + (int64_t)row * a.rbh + off[c]);
-            u[r][c] = *(const i32x4 *)(a.w[1] + e * a.stride[1] + (int64_t)row * a.rbh + off[c]);
-        }
+        for (int c = 0; c < 4; c++) acc[c] = fmaf(p[c], s[i], acc[c]);
     }
-    float sum[2] = {0.f, 0.f};
+    if ((lane & 15) == 0) *(f32x4 *)&part[wave][4 * (lane >> 4)] = acc;
+    strange = __syncthreads_or(strange);
+    if (threadIdx.x >= 16 || n0 + threadIdx.x >= a.I) return;
+    const int n = n0 + threadIdx.x;
+    float v[2];
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        double sg = 0.0, su = 0.0;
+    for (int i = 0; i < 2; i++) {
+        v[i] = part[i][threadIdx.x];
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            sg = fma((double)x[c].dot(g[r][c]), (double)sx[c] * sw[0][c], sg);
-            su = fma((double)x[c].dot(u[r][c]), (double)sx[c] * sw[1][c], su);
-        }
-        const float fg = (float)wave_sum_d(sg), fu = (float)wave_sum_d(su);
-        sum[0] = lane == r ? fg : sum[0];
-        sum[1] = lane == r ? fu : sum[1];
+        for (int q = 2; q < F8_FEW_WAVES; q += 2) v[i] += part[q + i][threadIdx.x];
+        if (strange)
+            v[i] = f8_strange_sums(a.x + (int64_t)t * a.rbh, a.xs + t, a.T, a.w[i] + e * a.stride[i] + (int64_t)n * a.rbh,
+                                   a.ws[i] + (e * ((a.I + 127) / 128) + n0 / F8_BLOCK) * blocks, a.rbh, 1, f32x4{v[i], 0.f, 0.f, 0.f})[0];
+        if (a.bias[i]) v[i] += a.bias[i][e * a.I + n];
     }
-    const float h = glu(sum[0] + b[0], sum[1] + b[1], a.glu);
-    if (lane < R && r0 + lane < a.I) a.h[((int64_t)t * a.K + j) * a.ldh + r0 + lane] = h;
+    a.h[((int64_t)t * a.K + j) * a.ldh + n] = glu(v[0], v[1], a.glu);
 }
 
-// Down and the weighted sum of a token: the block makes the token's K hidden rows codes in LDS (every block of the token does, one, two, four or
-// eight waves a row; 32 lanes hold a group of 128 columns), then each wave sums R outputs: lane l holds the 16 bytes l, l + 64, ... of the
-// K rows' codes laid end to end. The hidden rows are asked for before the weights: loads return in order, and the codes are made while the
-// weights come in.
-template <class T, int NC, int R>
-__global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 || R == 4 ? 4 : NC == 4 ? 6 : 8) void k_f8_few_down(F8FewArgs a) {
-    constexpr int NH = NC < 12 ? (NC + 1) / 2 : 6;  // pieces of a hidden row held in registers (the others are read later)
+// Down and the weighted sum of a token, 16 outputs a block: the block makes the token's K hidden rows codes in LDS (every block of the token does,
+// one, two, four or eight waves a row; 32 lanes hold a group of 128 columns), then its waves take the steps of the K rows end to end in turn. The hidden
+// rows are asked for before the weights: loads return in order, and the codes are made while the weights come in.
+template <class T, int NS, bool EXACT>
+__global__ __launch_bounds__(64 * F8_FEW_WAVES, NS > 4 ? 2 : 4) void k_f8_few_down(F8FewArgs a) {
+    constexpr int NH = NS < 12 ? (NS + 1) / 2 : 6;  // pieces of a hidden row held in registers (the others are read later)
     extern __shared__ __align__(16) uint8_t hq[];  // K rows of rbi codes, then their scales
-    __shared__ float wk[32];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.y, cpr = a.rbi / 16, blocks = a.rbi / F8_BLOCK;
+    __shared__ float wk[32], part[F8_FEW_WAVES][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.y, blocks = a.rbi / F8_BLOCK, steps = a.K * blocks;
     float *hs = (float *)(hq + a.K * a.rbi);
-    const int row0 = (blockIdx.x * I8_FEW_WAVES + wave) * R, nb = min(row0, a.H - 1) / F8_BLOCK;
+    const int n0 = blockIdx.x * 16, at = 16 * (lane >> 4);
     const int wpp = a.K > 4 ? 1 : a.K > 2 ? 2 : a.K > 1 ? 4 : 8, at0 = 4 * ((wave & (wpp - 1)) * 64 + lane), stride = 256 * wpp;
     const float *h = a.h + (int64_t)t * a.K * a.ldh;
     float hv[NH][4];
@@ -134,25 +112,21 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 || R == 4 ? 4 : NC == 4 
     fetch_h(min(wave / wpp, a.K - 1));
     const uint32_t *ids = a.ids + (int64_t)t * a.K;
     const float *wt = a.wt + (int64_t)t * a.K;
-    i32x4 w[R][NC];
-    float sd[NC];  // of each chunk: its weights' scale
+    auto step_of = [&](int i) __attribute__((always_inline)) { return min(wave + F8_FEW_WAVES * i, steps - 1); };
+    auto matrix_of = [&](int pick) __attribute__((always_inline)) { return a.w[2] + (int64_t)ids[pick] * a.stride[2]; };
+    auto scales_of = [&](int pick) __attribute__((always_inline)) { return a.ws[2] + ((int64_t)ids[pick] * ((a.H + 127) / 128) + n0 / F8_BLOCK) * blocks; };
+    i32x4 w[NS][2];
+    float sd[NS];
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const int i = min(lane + 64 * c, a.K * cpr - 1), pick = i / cpr, o = i - pick * cpr;
-        const int64_t e = ids[pick];
-        const uint8_t *p = a.w[2] + e * a.stride[2] + 16 * o;
-#pragma unroll
-        for (int r = 0; r < R; r++) w[r][c] = *(const i32x4 *)(p + (int64_t)min(row0 + r, a.H - 1) * a.rbi);
-        sd[c] = a.ws[2][(e * ((a.H + 127) / 128) + nb) * blocks + o / 8];
+    for (int i = 0; i < NS; i++) {
+        const int step = step_of(i), pick = step / blocks, b = step - pick * blocks;
+        const uint8_t *p = matrix_of(pick) + (int64_t)min(n0 + (lane & 15), a.H - 1) * a.rbi + b * F8_BLOCK + at;
+        w[i][0] = *(const i32x4 *)p;
+        w[i][1] = *(const i32x4 *)(p + 64);
+        sd[i] = scales_of(pick)[b];
     }
-    // lane j < K: the pick's weight and bias
-    const int mine = min(lane, a.K - 1);
-    const float wj = wt[mine];
-    if (wave == 0 && lane < a.K) wk[lane] = wj;
-    float b[R];
-#pragma unroll
-    for (int r = 0; r < R; r++) b[r] = a.bias[2] && lane < a.K ? a.bias[2][(int64_t)ids[mine] * a.H + min(row0 + r, a.H - 1)] : 0.f;
-    for (int j0 = 0; j0 < a.K; j0 += I8_FEW_WAVES / wpp) {
+    if (threadIdx.x < a.K) wk[threadIdx.x] = wt[threadIdx.x];
+    for (int j0 = 0; j0 < a.K; j0 += F8_FEW_WAVES / wpp) {
         const int j = j0 + wave / wpp;
         const float *row = h + (int64_t)min(j, a.K - 1) * a.ldh;
         if (j0) fetch_h(min(j, a.K - 1));
@@ -170,79 +144,70 @@ __global__ __launch_bounds__(64 * I8_FEW_WAVES, NC >= 8 || R == 4 ? 4 : NC == 4 
         };
 #pragma unroll
         for (int i = 0; i < NH; i++) store(at0 + i * stride, hv[i]);
-        for (int at = at0 + NH * stride; at - 4 * lane < a.rbi; at += stride) {
+        for (int o = at0 + NH * stride; o - 4 * lane < a.rbi; o += stride) {
             float v[4];
-            load_row<4>(row + at, a.I - at, v);
-            store(at, v);
+            load_row<4>(row + o, a.I - o, v);
+            store(o, v);
         }
     }
     __syncthreads();
-    if (row0 >= a.H) return;
-    double acc[R];
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    bool strange = false;
 #pragma unroll
-    for (int r = 0; r < R; r++) acc[r] = (double)wj * b[r];
+    for (int i = 0; i < NS; i++) {
+        if (wave + F8_FEW_WAVES * i >= steps) break;
+        const int step = step_of(i), pick = step / blocks;
+        const uint8_t *p = hq + step * F8_BLOCK + at;
+        F8Frag<EXACT> x, wf;
+        x.load(p, p + 64);
+        wf.load((const uint8_t *)&w[i][0], (const uint8_t *)&w[i][1]);
+        const float sx = hs[step], s = sx * sd[i], wj = wk[pick];
+        strange |= f8_strange(sx) | f8_strange(sd[i]);
+        const f32x4 v = F8Frag<EXACT>::product(wf, x);
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const int i = lane + 64 * c;
-        if (i < a.K * cpr) {
-            const F8Half16 x(*(const i32x4 *)(hq + 16 * i));
-            const double s = (double)wk[i / cpr] * sd[c] * hs[i / 8];
-#pragma unroll
-            for (int r = 0; r < R; r++) acc[r] = fma((double)x.dot(w[r][c]), s, acc[r]);
-        }
+        for (int c = 0; c < 4; c++) acc[c] = fmaf(v[c] * s, wj, acc[c]);
     }
+    if ((lane & 15) == 0) *(f32x4 *)&part[wave][4 * (lane >> 4)] = acc;
+    strange = __syncthreads_or(strange);
+    if (threadIdx.x >= 16 || n0 + threadIdx.x >= a.H) return;
+    const int n = n0 + threadIdx.x;
+    float v = part[0][threadIdx.x];
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        const float v = (float)wave_sum_d(acc[r]);
-        if (lane == 0 && row0 + r < a.H) ((T *)a.out)[(int64_t)t * a.H + row0 + r] = from_f32<T>(v);
+    for (int q = 1; q < F8_FEW_WAVES; q++) v += part[q][threadIdx.x];
+    if (strange) {
+        v = 0.f;
+        for (int j = 0; j < a.K; j++)
+            v = fmaf(f8_strange_sums(hq + j * a.rbi, hs + j * blocks, 1, matrix_of(j) + (int64_t)n * a.rbi, scales_of(j), a.rbi, 1, f32x4{}, true)[0], wk[j], v);
     }
+    if (a.bias[2])
+        for (int j = 0; j < a.K; j++) v = fmaf(wk[j], a.bias[2][(int64_t)ids[j] * a.H + n], v);
+    ((T *)a.out)[(int64_t)t * a.H + n] = from_f32<T>(v);
 }
 
-template <class T, int NC>
+template <class T, bool EXACT>
 static int few_down(const F8FewArgs &a, hipStream_t s) {
-    const int r = i8_down_rows(NC, a.H, a.T, (int)resident_blocks(1));
     auto go = [&](auto kernel) {
-        const int per = I8_FEW_WAVES * r;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.H + per - 1) / per), a.T), dim3(64 * I8_FEW_WAVES), a.K * (a.rbi + a.rbi / 32), s, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.H + 15) / 16), a.T), dim3(64 * F8_FEW_WAVES), a.K * (a.rbi + a.rbi / 32), s, a);
         return check_launch("k_f8_few_down");
     };
-    if constexpr (NC <= 4)
-        if (r == 4) return go(k_f8_few_down<T, NC, 4>);
-    if constexpr (NC <= 8)
-        if (r == 2) return go(k_f8_few_down<T, NC, 2>);
-    return go(k_f8_few_down<T, NC, 1>);
+    const int steps = (a.K * (a.rbi / F8_BLOCK) + F8_FEW_WAVES - 1) / F8_FEW_WAVES;  // of a wave
+    return steps <= 1 ? go(k_f8_few_down<T, 1, EXACT>) : steps <= 2 ? go(k_f8_few_down<T, 2, EXACT>) : steps <= 4 ? go(k_f8_few_down<T, 4, EXACT>)
+         : steps <= 8 ? go(k_f8_few_down<T, 8, EXACT>) : steps <= 12 ? go(k_f8_few_down<T, 12, EXACT>) : go(k_f8_few_down<T, 16, EXACT>);
 }
-template <class T>
-static int few_down(const F8FewArgs &a, hipStream_t s) {
-    switch (i8_down_pieces(a.K, a.rbi)) {
-    case 1: return few_down<T, 1>(a, s);
-    case 2: return few_down<T, 2>(a, s);
-    case 4: return few_down<T, 4>(a, s);
-    case 8: return few_down<T, 8>(a, s);
-    case 12: return few_down<T, 12>(a, s);
-    default: return few_down<T, 16>(a, s);
-    }
-}
-template <int PER, int NC>
+template <int PER, bool EXACT>
 static int few_gateup(const F8FewArgs &a, hipStream_t s) {
-    const int r = i8_gateup_rows(NC, a.I, a.T * a.K, (int)resident_blocks(1));
     auto go = [&](auto kernel) {
-        const int per = I8_FEW_WAVES * r;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.I + per - 1) / per), a.K, a.T), dim3(64 * I8_FEW_WAVES), 0, s, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.I + 15) / 16), a.K, a.T), dim3(64 * F8_FEW_WAVES), 0, s, a);
         return check_launch("k_f8_few_gateup");
     };
-    if constexpr (NC <= 2)
-        if (r == 4) return go(k_f8_few_gateup<PER, NC, 4>);
-    return r == 2 ? go(k_f8_few_gateup<PER, NC, 2>) : go(k_f8_few_gateup<PER, NC, 1>);
+    const int steps = (a.rbh / F8_BLOCK + F8_FEW_WAVES / 2 - 1) / (F8_FEW_WAVES / 2);
+    return steps <= 2 ? go(k_f8_few_gateup<PER, 2, EXACT>) : steps <= 4 ? go(k_f8_few_gateup<PER, 4, EXACT>) : steps <= 6 ? go(k_f8_few_gateup<PER, 6, EXACT>)
+                      : go(k_f8_few_gateup<PER, 8, EXACT>);
 }
-template <int PER>
+template <bool EXACT>
 static int few_gateup(const F8FewArgs &a, hipStream_t s) {
-    switch (i8_gateup_pieces(a.rbh)) {
-    case 1: return few_gateup<PER, 1>(a, s);
-    case 2: return few_gateup<PER, 2>(a, s);
-    case 3: return few_gateup<PER, 3>(a, s);
-    default: return few_gateup<PER, 4>(a, s);
-    }
+    const int per = i8_route_width(a.E);
+    return per == 4 ? few_gateup<4, EXACT>(a, s) : per == 8 ? few_gateup<8, EXACT>(a, s) : few_gateup<16, EXACT>(a, s);
 }
 
 // ------------------------------------------------------------------------------ many tokens
@@ -451,9 +416,9 @@ int cw_f8_moe_layer(const cw_f8_moe_desc *d, const uint8_t *x, const float *x_sc
         a.wt = w;
         a.h = (float *)(base + L.h);
         a.out = out;
-        const int per = i8_route_width(E);
-        if (int rc = per == 4 ? few_gateup<4>(a, s) : per == 8 ? few_gateup<8>(a, s) : few_gateup<16>(a, s)) return rc;
-        return ydtype == CW_F16 ? few_down<_Float16>(a, s) : ydtype == CW_BF16 ? few_down<bf16_t>(a, s) : few_down<float>(a, s);
+        // (as below: hidden codes of results in f16 and f32 from exact products)
+        if (int rc = ydtype == CW_BF16 ? few_gateup<false>(a, s) : few_gateup<true>(a, s)) return rc;
+        return ydtype == CW_F16 ? few_down<_Float16, false>(a, s) : ydtype == CW_BF16 ? few_down<bf16_t, false>(a, s) : few_down<float, true>(a, s);
     }
     if (int rc = cw_route_topk(logits, T, E, K, d->norm, ids, w, stream)) return rc;
     if (int rc = cw_sort_picks(ids, TK, E, order, place, offsets, tiles, base + L.sort, cw_sort_picks_workspace_size(TK, E), stream)) return rc;

@@ -60,9 +60,9 @@ __device__ __forceinline__ bool f8_strange(float s) {
 // Four neighbouring outputs, weight rows w .. w + 3 rb (of `valid`; the last again past them) times one row of x, if one of its scales or of
 // theirs is strange, else acc: whether is a matter of this row and these weights alone, whatever lies beside them. Slow: a lane reads
 // its rows by itself.
-__device__ __forceinline__ f32x4 f8_strange_sums(const uint8_t *x, const float *xs, int64_t m, const uint8_t *w, const float *ws, int rb, int valid, f32x4 acc) {
+__device__ __forceinline__ f32x4 f8_strange_sums(const uint8_t *x, const float *xs, int64_t m, const uint8_t *w, const float *ws, int rb, int valid, f32x4 acc,
+                                                 bool strange = false) {
     double sum[4] = {};
-    bool strange = false;
 #pragma unroll 1
     for (int b = 0; b < rb / F8_BLOCK; b++) {
         const float sx = xs[b * m], sw = ws[b];
