@@ -24,15 +24,16 @@ struct F8MatArgs {
 };
 
 // Few rows of x: a block takes 16 rows of W and up to 16 MB of x over all of k, its waves the steps of 128 codes in turn, both
-// operands straight from memory into registers (no byte of either is used by two waves of a block). The waves' sums meet in LDS, added
-// in the waves' order.
-template <class T, int MB>
+// operands straight from memory into registers (no byte of either is used by two waves of a block). The waves' sums meet in LDS: the
+// upper four's onto the lower four's, then those in their order.
+template <class T, int MB, bool EXACT>
 __global__ __launch_bounds__(64 * F8_FEW_WAVES) void k_f8_few(F8MatArgs a) {
-    __shared__ f32x4 part[F8_FEW_WAVES][MB][64];
+    constexpr int HALF = F8_FEW_WAVES / 2;
+    __shared__ f32x4 part[HALF][MB][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = 16 * (lane >> 4);
     const int64_t n0 = (int64_t)blockIdx.x * 16;
     const uint8_t *w0 = a.w + n0 * a.rb;
-    const float *ws = a.ws + n0 / F8_BLOCK * a.blocks;
+    const float *ws = f8_uniform(a.ws + n0 / F8_BLOCK * a.blocks);
     const uint32_t wrow = (uint32_t)(min(lane & 15, (int)(a.n - 1 - n0)) * a.rb + at);
     uint32_t xrow[MB], srow[MB];
 #pragma unroll
@@ -46,30 +47,40 @@ __global__ __launch_bounds__(64 * F8_FEW_WAVES) void k_f8_few(F8MatArgs a) {
     bool strange = false;
     for (int step = wave; step < a.blocks; step += F8_FEW_WAVES) {
         const uint8_t *w = w0 + (int64_t)step * F8_BLOCK + wrow, *x = a.x + (int64_t)step * F8_BLOCK;
-        F8Frag<true> wf, xf;
+        F8Frag<EXACT> wf, xf;
         wf.load(w, w + 64);
-        const float sw = ws[step];
+        const float sw = f8_scale_at(ws + step);
+        strange |= f8_strange(sw);
+        float sx[MB];
 #pragma unroll
         for (int i = 0; i < MB; i++) {
-            const float sx = a.xs[step * a.m + srow[i]], s = sx * sw;
-            strange |= f8_strange(sx) | f8_strange(sw);
-            xf.load(x + xrow[i], x + xrow[i] + 64);
-            const f32x4 p = F8Frag<true>::product(wf, xf);
+            sx[i] = a.xs[step * a.m + srow[i]];
+            if (i % 4 == lane >> 4) strange |= f8_strange(sx[i]);
+        }
 #pragma unroll
-            for (int c = 0; c < 4; c++) acc[i][c] = fmaf(p[c], s, acc[i][c]);
+        for (int i = 0; i < MB; i++) {
+            xf.load(x + xrow[i], x + xrow[i] + 64);
+            const f32x4 p = F8Frag<EXACT>::product(wf, xf);
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[i][c] = fmaf(p[c], sx[i] * sw, acc[i][c]);
         }
     }
-    const int64_t m = 16 * (wave % MB) + (lane & 15), n = n0 + 4 * (lane >> 4);
+    if (wave >= HALF)
+#pragma unroll
+        for (int i = 0; i < MB; i++) part[wave - HALF][i][lane] = acc[i];
+    strange = __syncthreads_or(strange);
+    if (wave < HALF)
+#pragma unroll
+        for (int i = 0; i < MB; i++) part[wave][i][lane] += acc[i];
+    __syncthreads();
+    const int64_t m = 16 * wave + (lane & 15), n = n0 + 4 * (lane >> 4);
+    if (wave >= MB || m >= a.m || n >= a.n) return;
     float b[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) b[i] = a.bias ? a.bias[min(n + i, a.n - 1)] : 0.f;
-#pragma unroll
-    for (int i = 0; i < MB; i++) part[wave][i][lane] = acc[i];
-    strange = __syncthreads_or(strange);
-    if (wave >= MB || m >= a.m || n >= a.n) return;
     f32x4 v = part[0][wave][lane];
 #pragma unroll
-    for (int o = 1; o < F8_FEW_WAVES; o++) v += part[o][wave][lane];
+    for (int o = 1; o < HALF; o++) v += part[o][wave][lane];
     if (strange) v = f8_strange_sums(a.x + m * a.rb, a.xs + m, a.m, a.w + n * a.rb, ws, a.rb, (int)min(a.n - n, (int64_t)4), v);
     f8_store4((T *)a.y + m * a.ldy + n, (int)min(a.n - n, (int64_t)4), v, b);
 }
@@ -84,83 +95,17 @@ __device__ __forceinline__ void f8_tile_of_block(int tiles_m, int tiles_n, int t
     n0 = (int64_t)__builtin_amdgcn_readfirstlane(4 * panel + in % width) * tn;
 }
 
-// A tile of 16 WM MF rows of x by 16 WN NF rows of W, a wave of 16 MF x 16 NF each; codes and scales of a step through a ring of LDS
-// stages by direct global-to-LDS loads, chunk c (16 bytes) of row r at chunk c ^ (r % 8) of its 128 bytes: the reads of one
+// A tile of 16 WM MF rows of x by 16 WN NF rows of W, a wave of 16 MF x 16 NF each; codes and scales of Q steps a stage through a ring
+// of LDS stages by direct global-to-LDS loads, chunk c (16 bytes) of row r at chunk c ^ (r % 8) of its 128 bytes: the reads of one
 // chunk touch all banks once.
-template <int WN, int WM, int NF, int MF, int STAGES>
+template <int WN, int WM, int NF, int MF, int Q, int STAGES>
 struct F8Ring {
-    static constexpr int N_WAVES = WN, TN = 16 * WN * NF, TM = 16 * WM * MF, WAVES = WN * WM, NT = 64 * WAVES;
-    static constexpr int SCALES = TM < 64 ? 64 : TM;  // (a load of scales: 64 of them)
-    static constexpr int CODES = (TN + TM) * F8_BLOCK, STAGE = CODES + 4 * SCALES;
-    static constexpr int LOADS = (TN + TM) / 8, PER = (LOADS + WAVES - 1) / WAVES, D = STAGES - 1, LDS = STAGES * STAGE;
-    static_assert(LDS <= 159 * 1024 && SCALES / 64 <= WAVES, "the ring fits the CU, a load of scales a wave");
+    static constexpr int TN = 16 * WN * NF, TM = 16 * WM * MF, WAVES = WN * WM, NT = 64 * WAVES;
+    static constexpr int CODES = (TN + TM) * F8_BLOCK, STEP = CODES + 4 * TM, STAGE = Q * STEP;
+    static constexpr int PER = (TN + TM) / 8 / WAVES, D = STAGES - 1, LDS = STAGES * STAGE;  // loads of codes of a wave and step; stages ahead
+    static_assert((TN + TM) % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && TM % 64 == 0 && TM / 64 <= WAVES && D * Q * (PER + 1) < 64, "whole loads for every wave");
+    static_assert(LDS <= 159 * 1024, "the ring fits the CU");
 };
-// xrow(r): x's row of row r < TM of the tile (any valid row past its end); n0: the tile's first row of W; w, ws: the matrix.
-// True if the wave saw a strange scale (the WN waves of a row of the tile look at a WN'th of its rows' scales each).
-template <class R, int NF, int MF, bool EXACT, class XRow>
-__device__ __forceinline__ bool f8_loop(uint8_t *lds, const F8MatArgs &a, const uint8_t *w, const float *ws, int64_t n0, XRow xrow, int wn, int wm,
-                                        f32x4 (&acc)[MF][NF]) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), steps = a.blocks;
-    // a stage: TN rows of W, then TM of x, then x's scales; load i of this wave: 8 rows from 8 (wave + WAVES i) (past the last:
-    // the first ones again, the same bytes to the same place)
-    const uint8_t *from[R::PER];
-#pragma unroll
-    for (int i = 0; i < R::PER; i++) {
-        const int r = 8 * ((wave + R::WAVES * i) % R::LOADS) + (lane >> 3);
-        const uint8_t *row = r < R::TN ? w + min(n0 + r, a.n - 1) * a.rb : a.x + xrow(r - R::TN) * (int64_t)a.rb;
-        from[i] = row + 16 * ((lane & 7) ^ (r & 7));
-    }
-    constexpr int SEGMENTS = R::SCALES / 64;
-    const float *scale = a.xs + xrow(min(64 * (wave % SEGMENTS) + lane, R::TM - 1));
-    const uint32_t to = lds_addr(lds);
-    auto fetch = [&](int step, int buf) __attribute__((always_inline)) {
-        const uint32_t at = to + buf * R::STAGE;
-#pragma unroll
-        for (int i = 0; i < R::PER; i++)
-            dma16(from[i] + (int64_t)step * F8_BLOCK, __builtin_amdgcn_readfirstlane(at + 1024 * ((wave + R::WAVES * i) % R::LOADS)));
-        dma4(scale + step * a.m, __builtin_amdgcn_readfirstlane(at + R::CODES + 256 * (wave % SEGMENTS)));
-    };
-    const int c0 = 16 * ((lane >> 4) ^ (lane & 7)), c1 = 16 * ((4 + (lane >> 4)) ^ (lane & 7));
-    const uint8_t *wl = lds + (16 * NF * wn + (lane & 15)) * F8_BLOCK, *xl = lds + (R::TN + 16 * MF * wm + (lane & 15)) * F8_BLOCK;
-    const uint8_t *sl = lds + R::CODES + 4 * (16 * MF * wm + (lane & 15));
-    const float *sw_of = ws + (n0 + 16 * NF * wn < a.n ? (n0 + 16 * NF * wn) / F8_BLOCK : 0) * a.blocks;
-#pragma unroll
-    for (int i = 0; i < MF; i++)
-#pragma unroll
-        for (int j = 0; j < NF; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < R::D && s < steps; s++) fetch(s, s);
-    int buf = 0, next = R::D;
-    bool odd = false;
-    for (int step = 0; step < steps; step++) {
-        // this wave's part of the stage is in (the stages after it may still be on their way), then every wave's; and
-        // every wave has multiplied the stage before, whose place the stage D ahead takes
-        if (step + R::D <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((R::D - 1) * (R::PER + 1)) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (step + R::D < steps) fetch(step + R::D, next);
-        next = next + 1 == R::D + 1 ? 0 : next + 1;
-        const float sw = sw_of[step];
-        const int o = buf * R::STAGE;
-        odd |= f8_strange(sw);
-        F8Frag<EXACT> wf[NF], xf;
-#pragma unroll
-        for (int j = 0; j < NF; j++) wf[j].load(wl + o + c0 + 2048 * j, wl + o + c1 + 2048 * j);
-#pragma unroll
-        for (int i = 0; i < MF; i++) {
-            xf.load(xl + o + c0 + 2048 * i, xl + o + c1 + 2048 * i);
-            const float sx = *(const float *)(sl + o + 64 * i);
-            if (i % R::N_WAVES == wn) odd |= f8_strange(sx);
-            const float s = sx * sw;
-#pragma unroll
-            for (int j = 0; j < NF; j++) {
-                const f32x4 p = F8Frag<EXACT>::product(wf[j], xf);
-#pragma unroll
-                for (int c = 0; c < 4; c++) acc[i][j][c] = fmaf(p[c], s, acc[i][j][c]);
-            }
-        }
-        buf = buf + 1 == R::D + 1 ? 0 : buf + 1;
-    }
-    return odd;
-}
 // A wave's sums of rows whose scales, or whose weights' scales, are strange: rows m0.. of m_end (x's: xrow), columns n0.. of the matrix w, ws
 template <int MF, int NF, class XRow>
 __device__ __forceinline__ void f8_strange_tile(const F8MatArgs &a, const uint8_t *w, const float *ws, XRow xrow, int64_t m0, int64_t m_end, int64_t n0,
@@ -196,26 +141,103 @@ __device__ __forceinline__ void f8_finish(const F8MatArgs &a, const float *bias,
     }
 }
 
-template <class T, int WN, int WM, int NF, int MF, int STAGES>
+template <class T, int WN, int WM, int NF, int MF, int Q, int STAGES>
 __global__ __launch_bounds__(64 * WN *WM, WN *WM / 4) void k_f8_tile(F8MatArgs a, int tiles_m, int tiles_n) {
-    using R = F8Ring<WN, WM, NF, MF, STAGES>;
+    using R = F8Ring<WN, WM, NF, MF, Q, STAGES>;
+    constexpr bool EXACT = f8_exact_for<T>;
     extern __shared__ __align__(1024) uint8_t lds[];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wm = wave / WN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wm = wave / WN;
+    const int last = a.blocks - 1, stages = (a.blocks + Q - 1) / Q;
     int64_t m0, n0;
     f8_tile_of_block(tiles_m, tiles_n, R::TM, R::TN, m0, n0);
+    const uint8_t *w0 = a.w + n0 * a.rb, *x0 = a.x + m0 * a.rb;
+    // load i of this wave: 8 rows, of TN of W, then TM of x, from 8 (wave + WAVES i)
+    uint32_t off[R::PER];
+#pragma unroll
+    for (int i = 0; i < R::PER; i++) {
+        const int r = 8 * (wave + R::WAVES * i) + (lane >> 3);
+        const int64_t row = 8 * R::WAVES * i < R::TN ? min((int64_t)r, a.n - 1 - n0) : min((int64_t)r - R::TN, a.m - 1 - m0);
+        off[i] = (uint32_t)row * a.rb + 16 * ((lane & 7) ^ (r & 7));
+    }
+    const bool scales = wave < R::TM / 64;  // the waves that load them, 64 each
+    const uint32_t soff = 4 * (uint32_t)min((int64_t)(64 * wave + lane), a.m - m0 - 1);
+    const float *xs0 = a.xs + m0;
+    const uint32_t to = lds_addr(lds);
+    auto fetch = [&](int stage, int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            const int step = min(stage * Q + q, last);  // (past the end: the last step's bytes, unused)
+            const uint32_t at = to + buf * R::STAGE + q * R::STEP;
+#pragma unroll
+            for (int i = 0; i < R::PER; i++)
+                dma16_s((8 * R::WAVES * i < R::TN ? w0 : x0) + (int64_t)step * F8_BLOCK, off[i], __builtin_amdgcn_readfirstlane(at + 1024 * (wave + R::WAVES * i)));
+            if (scales) dma4_s((const uint8_t *)(xs0 + step * a.m), soff, __builtin_amdgcn_readfirstlane(at + R::CODES + 256 * wave));
+        }
+    };
+    const int c0 = 16 * ((lane >> 4) ^ (lane & 7)), c1 = 16 * ((4 + (lane >> 4)) ^ (lane & 7));
+    const uint8_t *wl = lds + (16 * NF * wn + (lane & 15)) * F8_BLOCK, *xl = lds + (R::TN + 16 * MF * wm + (lane & 15)) * F8_BLOCK;
+    const uint8_t *sl = lds + R::CODES + 4 * (16 * MF * wm + (lane & 15));
+    const float *sw_of = f8_uniform(a.ws + (n0 + 16 * NF * wn < a.n ? (n0 + 16 * NF * wn) / F8_BLOCK : 0) * a.blocks);
     f32x4 acc[MF][NF];
-    const bool odd = f8_loop<R, NF, MF, f8_exact_for<T>>(lds, a, a.w, a.ws, n0, [&](int r) { return min(m0 + r, a.m - 1); }, wn, wm, acc);
+#pragma unroll
+    for (int i = 0; i < MF; i++)
+#pragma unroll
+        for (int j = 0; j < NF; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < R::D && s < stages; s++) fetch(s, s);
+    int buf = 0, next = R::D;
+    bool odd = false;
+    float sw[Q];  // (a step ahead: the scalar loads of a step would be waited for with its reads of LDS)
+#pragma unroll
+    for (int q = 0; q < Q; q++) sw[q] = f8_scale_at(sw_of + min(q, last));
+    for (int stage = 0; stage < stages; stage++) {
+        // this wave's part of the stage is in (the stages after it may still be on their way), then every wave's; and
+        // every wave has multiplied the stage before, whose place the stage D ahead takes
+        if (stage + R::D > stages) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else if (scales) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((R::D - 1) * Q * (R::PER + 1)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"((R::D - 1) * Q * R::PER) : "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (stage + R::D < stages) fetch(stage + R::D, next);
+        next = next + 1 == R::D + 1 ? 0 : next + 1;
+        float now[Q];
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            now[q] = sw[q];
+            odd |= f8_strange(now[q]);
+            sw[q] = f8_scale_at(sw_of + min((stage + 1) * Q + q, last));
+        }
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            if (Q > 1 && stage * Q + q > last) break;
+            const int o = buf * R::STAGE + q * R::STEP;
+            F8Frag<EXACT> wf[NF], xf;
+#pragma unroll
+            for (int j = 0; j < NF; j++) wf[j].load(wl + o + c0 + 2048 * j, wl + o + c1 + 2048 * j);
+#pragma unroll
+            for (int i = 0; i < MF; i++) {
+                xf.load(xl + o + c0 + 2048 * i, xl + o + c1 + 2048 * i);
+                const float sx = *(const float *)(sl + o + 64 * i), s = sx * now[q];
+                if (i % WN == wn) odd |= f8_strange(sx);  // (the WN waves of a row of the tile look at a WN'th of its rows' scales each)
+#pragma unroll
+                for (int j = 0; j < NF; j++) {
+                    const f32x4 p = F8Frag<EXACT>::product(wf[j], xf);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) acc[i][j][c] = fmaf(p[c], s, acc[i][j][c]);
+                }
+            }
+        }
+        buf = buf + 1 == R::D + 1 ? 0 : buf + 1;
+    }
     if (__syncthreads_or(odd)) f8_strange_tile(a, a.w, a.ws, [](int64_t r) { return r; }, m0 + 16 * MF * wm, a.m, n0 + 16 * NF * wn, acc);
     f8_finish<T, MF, NF>(a, a.bias, m0 + 16 * MF * wm, a.m, n0 + 16 * NF * wn, acc);
 }
 
 // Many rows of x: tiles of 256 x 256, eight waves of 64 columns x 128 rows, two to a SIMD: one multiplies while the other scales and
-// adds. Two LDS stages of 2 x 256 rows x 128 codes and 256 scales, swizzled as in f8_loop. A wave's four fragments of W stay in
+// adds. Two LDS stages of 2 x 256 rows x 128 codes and 256 scales, swizzled as in k_f8_tile. A wave's four fragments of W stay in
 // registers for the step, x's eight pass by, each read while the one before is multiplied; the next step's first ones while the
 // last is, before which all waves meet: the stage of the next step is then in, and this step's, all of which has been read, free for the one after.
 template <class T>
 __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int tiles_n) {
-    using R = F8Ring<4, 2, 4, 8, 2>;
+    using R = F8Ring<4, 2, 4, 8, 1, 2>;
     using Frag = F8Frag<false>;
     extern __shared__ __align__(1024) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave & 3, wm = wave >> 2, last = a.blocks - 1;
@@ -242,7 +264,7 @@ __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int
     const int c0 = 16 * ((lane >> 4) ^ (lane & 7)), c1 = 16 * ((4 + (lane >> 4)) ^ (lane & 7));
     const uint8_t *wl = lds + (64 * wn + (lane & 15)) * F8_BLOCK, *xl = lds + (R::TN + 128 * wm + (lane & 15)) * F8_BLOCK;
     const uint8_t *sl = lds + R::CODES + 4 * (128 * wm + (lane & 15)), *ol = lds + R::CODES + 4 * (128 * wm + 32 * wn + (lane & 31));
-    const float *sw_of = a.ws + (n0 + 64 * wn < a.n ? (n0 + 64 * wn) / F8_BLOCK : 0) * a.blocks;
+    const float *sw_of = f8_uniform(a.ws + (n0 + 64 * wn < a.n ? (n0 + 64 * wn) / F8_BLOCK : 0) * a.blocks);
     f32x4 acc[8][4];
 #pragma unroll
     for (int i = 0; i < 8; i++)
@@ -268,8 +290,10 @@ __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int
 #pragma unroll
         for (int c = 0; c < 4; c++) acc[i][j][c] = fmaf(p[i & 1][j][c], s, acc[i][j][c]);
     };
+    float sw_next = f8_scale_at(sw_of);
     for (int step = 0; step <= last; step++) {
-        const float sw = sw_of[step];
+        const float sw = sw_next;
+        sw_next = f8_scale_at(sw_of + min(step + 1, last));
         const int o = (step & 1) * R::STAGE, next = R::STAGE - o;
         odd |= f8_strange(*(const float *)(ol + o)) | f8_strange(sw);
 #pragma unroll
@@ -363,13 +387,23 @@ static int f8_matmul(const F8MatArgs &a, int few_groups, int tile_of, hipStream_
         hipLaunchKernelGGL(kernel, dim3((unsigned)((a.n + 15) / 16)), dim3(64 * F8_FEW_WAVES), 0, s, a);
         return check_launch("k_f8_few");
     };
-    if (few_groups) return few_groups == 1 ? few(k_f8_few<T, 1>) : few_groups == 2 ? few(k_f8_few<T, 2>) : few(k_f8_few<T, 4>);
+    constexpr bool exact = f8_exact_for<T>;
+    switch (few_groups) {
+    case 0: break;
+    case 1: return few(k_f8_few<T, 1, exact>);
+    case 2: return few(k_f8_few<T, 2, exact>);
+    case 3: return few(k_f8_few<T, 3, exact>);
+    case 4: return few(k_f8_few<T, 4, exact>);
+    case 5: return few(k_f8_few<T, 5, exact>);
+    case 6: return few(k_f8_few<T, 6, exact>);
+    default: return few(k_f8_few<T, 8, exact>);
+    }
     switch (tile_of) {
-    case 0: return f8_tiles<T, F8Ring<4, 2, 1, 2, 8>>(a, k_f8_tile<T, 4, 2, 1, 2, 8>, s);
-    case 1: return f8_tiles<T, F8Ring<4, 2, 2, 4, 4>>(a, k_f8_tile<T, 4, 2, 2, 4, 4>, s);
+    case 0: return f8_tiles<T, F8Ring<4, 2, 1, 2, 2, 4>>(a, k_f8_tile<T, 4, 2, 1, 2, 2, 4>, s);
+    case 1: return f8_tiles<T, F8Ring<4, 2, 2, 4, 1, 4>>(a, k_f8_tile<T, 4, 2, 2, 4, 1, 4>, s);
     default:
-        if constexpr (f8_exact_for<T>) return f8_tiles<T, F8Ring<4, 2, 4, 8, 2>>(a, k_f8_tile<T, 4, 2, 4, 8, 2>, s);
-        else return f8_tiles<T, F8Ring<4, 2, 4, 8, 2>>(a, k_f8_big<T>, s);
+        if constexpr (exact) return f8_tiles<T, F8Ring<4, 2, 4, 8, 1, 2>>(a, k_f8_tile<T, 4, 2, 4, 8, 1, 2>, s);
+        else return f8_tiles<T, F8Ring<4, 2, 4, 8, 1, 2>>(a, k_f8_big<T>, s);
     }
 }
 

@@ -1,6 +1,7 @@
 // Which kernels the products of the 8-bit float path take, by their sizes and the device's compute units: plain functions of the host.
 #pragma once
 #include <math.h>
+#include <stdlib.h>
 #include <stdint.h>
 #include <algorithm>
 
@@ -32,6 +33,7 @@ inline int f8_pick_tile(int64_t m, int64_t n, int rb, int cus) {
 }
 // Groups of 16 rows of x that k_f8_few takes (0: tiles).
 inline int f8_few_groups(int64_t m, int64_t n, int rb) {
+    if (getenv("FEW")) { int f = atoi(getenv("FEW")); if (!f || m > 128) return 0; int g = (int)((m + 15) / 16); return g == 7 ? 8 : g; }
     return m <= 16 ? 1 : m <= 32 && n * rb <= 1 << 24 ? 2 : m <= 64 && n * rb <= 1 << 21 ? 4 : 0;
 }
 

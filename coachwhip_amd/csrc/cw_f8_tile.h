@@ -88,6 +88,15 @@ __device__ __forceinline__ f32x4 f8_strange_sums(const uint8_t *x, const float *
     return acc;
 }
 
+// A weights' scale by a scalar load, at a wave-uniform place. (A vector load, which the compiler makes of it beside the inline waits, returns after
+// all loads asked for before it: with the weights of the steps ahead in flight it waits for them.)
+__device__ __forceinline__ const float *f8_uniform(const float *p) {
+    const uint64_t u = (uint64_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)u), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
+    return (const float *)(lo | (uint64_t)hi << 32);
+}
+__device__ __forceinline__ float f8_scale_at(const float *p) { return *(const __attribute__((address_space(4))) float *)(uint64_t)p; }
+
 // Results in f32 have exact products, f16's and bf16's rounding covers what the 8-bit instruction leaves out.
 template <class T>
 constexpr bool f8_exact_for = std::is_same_v<T, float>;
@@ -134,7 +143,16 @@ __device__ __forceinline__ bool f8_stream(uint8_t *lds, const F8Operands<MATS> &
     const int st = threadIdx.x % (16 * MB * Q), sb = st / (16 * MB);
     const float *sp = a.xs + xrow(st % (16 * MB));
     i32x4 xr[S::PER], w[2][NW][2 * Q];
-    float xsr = 0.f;
+    const float *ws[MATS];
+    float xsr = 0.f, sw[MATS][Q];
+#pragma unroll
+    for (int i = 0; i < MATS; i++) ws[i] = f8_uniform(a.ws0[i]);
+    auto fetch_sw = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < MATS; i++)
+#pragma unroll
+            for (int q = 0; q < Q; q++) sw[i][q] = f8_scale_at(ws[i] + min(step * Q + q, a.blocks - 1));
+    };
     bool odd = false;
     // the lane's chunk of k of a step, and whether the row has it (past its end: its last line, not used)
     auto fetch_x = [&](int step) __attribute__((always_inline)) {
@@ -179,14 +197,17 @@ __device__ __forceinline__ bool f8_stream(uint8_t *lds, const F8Operands<MATS> &
         __builtin_amdgcn_sched_barrier(0);
         const uint8_t *b = lds + (step & 1) * S::STAGE + (lane & 15) * WIDE;
         const float *sx = (const float *)(lds + (step & 1) * S::STAGE + S::CODES) + (lane & 15);
+        float sn[MATS][Q];  // (the next step's are asked for a step ahead)
+#pragma unroll
+        for (int i = 0; i < MATS; i++)
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+                sn[i][q] = sw[i][q];
+                odd |= f8_strange(sn[i][q]);
+            }
+        fetch_sw(step + 1);
 #pragma unroll
         for (int q = 0; q < Q; q++) {
-            float sw[MATS];
-#pragma unroll
-            for (int i = 0; i < MATS; i++) {
-                sw[i] = a.ws0[i][min(step * Q + q, a.blocks - 1)];
-                odd |= f8_strange(sw[i]);
-            }
             auto frag = [&](int mb) __attribute__((always_inline)) {
                 F8Frag<EXACT> f;
                 const uint8_t *p = b + mb * 16 * WIDE;
@@ -194,7 +215,7 @@ __device__ __forceinline__ bool f8_stream(uint8_t *lds, const F8Operands<MATS> &
                 return f;
             };
             auto add = [&](int mb, int j, f32x4 p) __attribute__((always_inline)) {
-                const float s = sx[q * 16 * MB + 16 * mb] * sw[j / (NW / MATS)];
+                const float s = sx[q * 16 * MB + 16 * mb] * sn[j / (NW / MATS)][q];
 #pragma unroll
                 for (int c = 0; c < 4; c++) acc[mb][j][c] = fmaf(p[c], s, acc[mb][j][c]);
                 asm volatile("" : "+v"(acc[mb][j]));  // (here and now: sunk to the next step, the products would need registers of their own)
@@ -233,6 +254,7 @@ __device__ __forceinline__ bool f8_stream(uint8_t *lds, const F8Operands<MATS> &
             }
         }
     };
+    fetch_sw(0);
     fetch_x(0);
     store_x(0);
     fetch_x(1);
