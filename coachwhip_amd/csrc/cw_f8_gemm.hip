@@ -141,6 +141,22 @@ __device__ __forceinline__ void f8_finish(const F8MatArgs &a, const float *bias,
     }
 }
 
+// Whether a tile has a strange scale: its rows' from m0, its weights' from row n0, looked at once, while the first codes are on their way (in the
+// steps, where every wave meets them, the checks were a sixth of the instructions).
+template <int TM, int TN, int WAVES>
+__device__ __forceinline__ bool f8_any_strange(const F8MatArgs &a, int64_t m0, int64_t n0) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    bool strange = false;
+    for (int b = wave; b < a.blocks; b += WAVES)
+#pragma unroll
+        for (int r = lane; r < TM; r += 64) strange |= f8_strange(a.xs[b * a.m + min(m0 + r, a.m - 1)]);
+    const int64_t last = (a.n - 1) / F8_BLOCK;
+#pragma unroll
+    for (int c = 0; c < (TN + F8_BLOCK - 1) / F8_BLOCK; c++)
+        for (int b = threadIdx.x; b < a.blocks; b += 64 * WAVES) strange |= f8_strange(a.ws[min(n0 / F8_BLOCK + c, last) * a.blocks + b]);
+    return strange;
+}
+
 template <class T, int WN, int WM, int NF, int MF, int Q, int STAGES>
 __global__ __launch_bounds__(64 * WN *WM, WN *WM / 4) void k_f8_tile(F8MatArgs a, int tiles_m, int tiles_n) {
     using R = F8Ring<WN, WM, NF, MF, Q, STAGES>;
@@ -185,7 +201,7 @@ __global__ __launch_bounds__(64 * WN *WM, WN *WM / 4) void k_f8_tile(F8MatArgs a
         for (int j = 0; j < NF; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < R::D && s < stages; s++) fetch(s, s);
     int buf = 0, next = R::D;
-    bool odd = false;
+    const bool strange = f8_any_strange<R::TM, R::TN, R::WAVES>(a, m0, n0);
     float sw[Q];  // (a step ahead: the scalar loads of a step would be waited for with its reads of LDS)
 #pragma unroll
     for (int q = 0; q < Q; q++) sw[q] = f8_scale_at(sw_of + min(q, last));
@@ -198,36 +214,67 @@ __global__ __launch_bounds__(64 * WN *WM, WN *WM / 4) void k_f8_tile(F8MatArgs a
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (stage + R::D < stages) fetch(stage + R::D, next);
         next = next + 1 == R::D + 1 ? 0 : next + 1;
+        const int o = buf * R::STAGE;
+        F8Frag<EXACT> wf[Q][NF];
         float now[Q];
 #pragma unroll
         for (int q = 0; q < Q; q++) {
             now[q] = sw[q];
-            odd |= f8_strange(now[q]);
             sw[q] = f8_scale_at(sw_of + min((stage + 1) * Q + q, last));
         }
+        if constexpr (EXACT && NF * MF > 4) {  // (the fragments of a step as f16 would take too many registers)
 #pragma unroll
-        for (int q = 0; q < Q; q++) {
-            if (Q > 1 && stage * Q + q > last) break;
-            const int o = buf * R::STAGE + q * R::STEP;
-            F8Frag<EXACT> wf[NF], xf;
+            for (int q = 0; q < Q; q++) {
+                const int at = o + q * R::STEP;
 #pragma unroll
-            for (int j = 0; j < NF; j++) wf[j].load(wl + o + c0 + 2048 * j, wl + o + c1 + 2048 * j);
+                for (int j = 0; j < NF; j++) wf[0][j].load(wl + at + c0 + 2048 * j, wl + at + c1 + 2048 * j);
 #pragma unroll
-            for (int i = 0; i < MF; i++) {
-                xf.load(xl + o + c0 + 2048 * i, xl + o + c1 + 2048 * i);
-                const float sx = *(const float *)(sl + o + 64 * i), s = sx * now[q];
-                if (i % WN == wn) odd |= f8_strange(sx);  // (the WN waves of a row of the tile look at a WN'th of its rows' scales each)
+                for (int i = 0; i < MF; i++) {
+                    F8Frag<EXACT> xi;
+                    xi.load(xl + at + c0 + 2048 * i, xl + at + c1 + 2048 * i);
+                    const float s = Q == 1 || stage * Q + q <= last ? *(const float *)(sl + at + 64 * i) * now[q] : 0.f;
 #pragma unroll
-                for (int j = 0; j < NF; j++) {
-                    const f32x4 p = F8Frag<EXACT>::product(wf[j], xf);
+                    for (int j = 0; j < NF; j++) {
+                        const f32x4 p = F8Frag<EXACT>::product(wf[0][j], xi);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) acc[i][j][c] = fmaf(p[c], s, acc[i][j][c]);
+                        for (int c = 0; c < 4; c++) acc[i][j][c] = fmaf(p[c], s, acc[i][j][c]);
+                    }
                 }
             }
+        } else {
+            F8Frag<EXACT> xf[Q][MF];
+            f32x4 p[Q][MF][NF];
+            float s[Q][MF];
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+#pragma unroll
+                for (int j = 0; j < NF; j++) wf[q][j].load(wl + o + q * R::STEP + c0 + 2048 * j, wl + o + q * R::STEP + c1 + 2048 * j);
+#pragma unroll
+                for (int i = 0; i < MF; i++) {
+                    xf[q][i].load(xl + o + q * R::STEP + c0 + 2048 * i, xl + o + q * R::STEP + c1 + 2048 * i);
+                    s[q][i] = *(const float *)(sl + o + q * R::STEP + 64 * i);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+#pragma unroll
+                for (int i = 0; i < MF; i++) {
+#pragma unroll
+                    for (int j = 0; j < NF; j++) p[q][i][j] = F8Frag<EXACT>::product(wf[q][j], xf[q][i]);
+                    s[q][i] = Q == 1 || stage * Q + q <= last ? s[q][i] * now[q] : 0.f;  // (past the end the last step again, times nothing)
+                }
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+#pragma unroll
+                for (int i = 0; i < MF; i++)
+#pragma unroll
+                    for (int j = 0; j < NF; j++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) acc[i][j][c] = fmaf(p[q][i][j][c], s[q][i], acc[i][j][c]);
         }
         buf = buf + 1 == R::D + 1 ? 0 : buf + 1;
     }
-    if (__syncthreads_or(odd)) f8_strange_tile(a, a.w, a.ws, [](int64_t r) { return r; }, m0 + 16 * MF * wm, a.m, n0 + 16 * NF * wn, acc);
+    if (__syncthreads_or(strange)) f8_strange_tile(a, a.w, a.ws, [](int64_t r) { return r; }, m0 + 16 * MF * wm, a.m, n0 + 16 * NF * wn, acc);
     f8_finish<T, MF, NF>(a, a.bias, m0 + 16 * MF * wm, a.m, n0 + 16 * NF * wn, acc);
 }
 
@@ -263,7 +310,7 @@ __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int
     };
     const int c0 = 16 * ((lane >> 4) ^ (lane & 7)), c1 = 16 * ((4 + (lane >> 4)) ^ (lane & 7));
     const uint8_t *wl = lds + (64 * wn + (lane & 15)) * F8_BLOCK, *xl = lds + (R::TN + 128 * wm + (lane & 15)) * F8_BLOCK;
-    const uint8_t *sl = lds + R::CODES + 4 * (128 * wm + (lane & 15)), *ol = lds + R::CODES + 4 * (128 * wm + 32 * wn + (lane & 31));
+    const uint8_t *sl = lds + R::CODES + 4 * (128 * wm + (lane & 15));
     const float *sw_of = f8_uniform(a.ws + (n0 + 64 * wn < a.n ? (n0 + 64 * wn) / F8_BLOCK : 0) * a.blocks);
     f32x4 acc[8][4];
 #pragma unroll
@@ -273,9 +320,9 @@ __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int
     Frag wf[4], xf[2];
     f32x4 p[2][4];  // the sums of these 16 rows, and of those before, which are scaled and added meanwhile
     float sx[2], s = 0.f;
-    bool odd = false;
 #pragma unroll
     for (int i = 0; i < 9; i++) fetch(0, i);
+    const bool strange = f8_any_strange<R::TM, R::TN, R::WAVES>(a, m0, n0);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     fetch(1, 0);
     fetch(1, 1);
@@ -295,7 +342,6 @@ __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int
         const float sw = sw_next;
         sw_next = f8_scale_at(sw_of + min(step + 1, last));
         const int o = (step & 1) * R::STAGE, next = R::STAGE - o;
-        odd |= f8_strange(*(const float *)(ol + o)) | f8_strange(sw);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             if (i == 7) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -322,7 +368,7 @@ __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int
 #pragma unroll
     for (int j = 0; j < 4; j++) add(7, j);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (no load may land in LDS that is another block's)
-    if (__syncthreads_or(odd)) f8_strange_tile(a, a.w, a.ws, [](int64_t r) { return r; }, m0 + 128 * wm, a.m, n0 + 64 * wn, acc);
+    if (__syncthreads_or(strange)) f8_strange_tile(a, a.w, a.ws, [](int64_t r) { return r; }, m0 + 128 * wm, a.m, n0 + 64 * wn, acc);
     f8_finish<T, 8, 4>(a, a.bias, m0 + 128 * wm, a.m, n0 + 64 * wn, acc);
 }
 
@@ -394,13 +440,14 @@ static int f8_matmul(const F8MatArgs &a, int few_groups, int tile_of, hipStream_
     case 2: return few(k_f8_few<T, 2, exact>);
     case 3: return few(k_f8_few<T, 3, exact>);
     case 4: return few(k_f8_few<T, 4, exact>);
-    case 5: return few(k_f8_few<T, 5, exact>);
-    case 6: return few(k_f8_few<T, 6, exact>);
-    default: return few(k_f8_few<T, 8, exact>);
+    default:
+        if constexpr (exact) return few(k_f8_few<T, 5, exact>);
     }
     switch (tile_of) {
-    case 0: return f8_tiles<T, F8Ring<4, 2, 1, 2, 2, 4>>(a, k_f8_tile<T, 4, 2, 1, 2, 2, 4>, s);
-    case 1: return f8_tiles<T, F8Ring<4, 2, 2, 4, 1, 4>>(a, k_f8_tile<T, 4, 2, 2, 4, 1, 4>, s);
+    case 0:
+        if constexpr (exact) return f8_tiles<T, F8Ring<2, 2, 2, 2, 2, 4>>(a, k_f8_tile<T, 2, 2, 2, 2, 2, 4>, s);
+        else return f8_tiles<T, F8Ring<4, 2, 1, 2, 4, 2>>(a, k_f8_tile<T, 4, 2, 1, 2, 4, 2>, s);
+    case 1: return f8_tiles<T, F8Ring<4, 2, 2, 4, 2, 2>>(a, k_f8_tile<T, 4, 2, 2, 4, 2, 2>, s);
     default:
         if constexpr (exact) return f8_tiles<T, F8Ring<4, 2, 4, 8, 1, 2>>(a, k_f8_tile<T, 4, 2, 4, 8, 1, 2>, s);
         else return f8_tiles<T, F8Ring<4, 2, 4, 8, 1, 2>>(a, k_f8_big<T>, s);
@@ -480,7 +527,9 @@ int cw_f8_matmul(const uint8_t *w, const float *w_scale, int64_t n, int64_t k, c
                  const float *bias, int ydtype, void *y, int64_t ldy, cw_stream_t stream) {
     if (int rc = check_product("f8_matmul", ydtype, n, k, m, ldy)) return rc;
     if (m == 0) return CW_OK;
-    const int rb = (int)f8_row_bytes(k), few_groups = f8_few_groups(m, n, rb), tile = few_groups ? 0 : f8_pick_tile(m, n, rb, (int)resident_blocks(1));
+    const int rb = (int)f8_row_bytes(k), cus = (int)resident_blocks(1);
+    const bool exact = ydtype == CW_F32;
+    const int few_groups = f8_few_groups(exact, m, n, cus), tile = few_groups ? 0 : f8_pick_tile(exact, m, n, rb, cus);
     if (tile < 0) return set_error(CW_ENOTSUP, "f8_matmul: %lld x %lld outputs", (long long)m, (long long)n);
     CW_REQUIRE(w && w_scale && x && x_scale && y, "f8_matmul: null pointer");
     CW_REQUIRE(f8_aligned(w, 16) && f8_aligned(x, 16), "f8_matmul: codes must be 16-byte aligned");

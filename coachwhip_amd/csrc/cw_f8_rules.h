@@ -1,7 +1,6 @@
 // Which kernels the products of the 8-bit float path take, by their sizes and the device's compute units: plain functions of the host.
 #pragma once
 #include <math.h>
-#include <stdlib.h>
 #include <stdint.h>
 #include <algorithm>
 
@@ -9,18 +8,24 @@ namespace cw {
 
 constexpr int F8_FEW_WAVES = 8;  // waves of a block of the kernel for few rows
 
+// The tile whose estimated time is the least. A CU runs one block of any of them; a round of blocks on every CU takes b + s k / 1024 us, more than
+// one on some of them. Exact products (results in f32) take about twice the time. Measured in a graph (4096 x 4096 in bf16; launch 2.5 us
+// included), estimate / measured: 64 x 64 at 128 rows 13.4 / 13.4, 256 rows (every CU) 14.3 / 14.3, 512 rows 26.1 / 29; 128 x 128 at 512 rows 26.9 / 26.9,
+// 1,024 rows 29.4 / 29.4, 2,048 rows 56.3 / 55.8; 256 x 256 at 2,048 rows 58.5 / 59.4, 4,096 rows 71.5 / 71.1. In f32: 64 x 64 at 77 rows of 4001 x
+// 2880 13.1 / 13.2; 128 x 128 at 512 rows of 4096 x 4096 44 / 44.5; 256 x 256 118 / 118.7.
 struct F8TileTime {
     int tm, tn;
     double some_b, some_s, all_b, all_s;
 };
-constexpr F8TileTime F8_TILES[3] = {{64, 64, 2.4, 1.6, 3.0, 1.8}, {128, 128, 4.2, 3.6, 5.5, 4.6}, {256, 256, 12, 9, 15, 13}};
+constexpr F8TileTime F8_TILES[2][3] = {{{64, 64, 2.6, 2.07, 3.0, 2.2}, {128, 128, 2.8, 5.4, 3.3, 5.9}, {256, 256, 8, 12, 19, 12.5}},
+                                       {{64, 64, 2.0, 3.0, 2.4, 3.2}, {128, 128, 1.0, 10.1, 2.0, 11}, {256, 256, 2, 28.4, 4, 30}}};
 constexpr int64_t F8_MAX_TILES = 1 << 22;  // (a launch holds fewer than 2^32 threads, 512 of a tile at most)
 // (-1: every tile's count exceeds the launch)
-inline int f8_pick_tile(int64_t m, int64_t n, int rb, int cus) {
+inline int f8_pick_tile(bool exact, int64_t m, int64_t n, int rb, int cus) {
     int best = -1;
     double least = 0;
     for (int i = 0; i < 3; i++) {
-        const F8TileTime &t = F8_TILES[i];
+        const F8TileTime &t = F8_TILES[exact][i];
         const int64_t blocks = (m + t.tm - 1) / t.tm * ((n + t.tn - 1) / t.tn);
         if (blocks >= F8_MAX_TILES) continue;
         const double k = rb / 1024.0, us = (double)(blocks / cus) * (t.all_b + t.all_s * k) + (blocks % cus ? t.some_b + t.some_s * k : 0.0);
@@ -31,10 +36,13 @@ inline int f8_pick_tile(int64_t m, int64_t n, int rb, int cus) {
     }
     return best;
 }
-// Groups of 16 rows of x that k_f8_few takes (0: tiles).
-inline int f8_few_groups(int64_t m, int64_t n, int rb) {
-    if (getenv("FEW")) { int f = atoi(getenv("FEW")); if (!f || m > 128) return 0; int g = (int)((m + 15) / 16); return g == 7 ? 8 : g; }
-    return m <= 16 ? 1 : m <= 32 && n * rb <= 1 << 24 ? 2 : m <= 64 && n * rb <= 1 << 21 ? 4 : 0;
+// Groups of 16 rows of x that k_f8_few takes (0: tiles): each block, of 16 columns, reads all of x. Measured in a graph, few rows / 64 x 64 tiles, bf16: 32
+// rows of 4096 x 4096 9.1 / 13.4 us, of 8192 x 8192 25.5 / 31; 48 rows of 4096 x 4096 12.6 / 13.4, of 8192 x 8192 34.8 / 31; 64 rows of 2048 x 2048 8.5 /
+// 8.7, of 4096 x 4096 15.0 / 13.4. f32, 77 rows: of 4001 x 2880 12.2 / 13.2, of 4096 x 4096 17.7 / 18, of 8192 x 8192 48.5 / 44.
+inline int f8_few_groups(bool exact, int64_t m, int64_t n, int cus) {
+    const int64_t columns = 16ll * cus;  // a block to a CU
+    const int most = exact && n <= columns ? 5 : n <= columns / 2 ? 4 : n <= columns ? 3 : 2;
+    return m <= 16 * most ? (int)((m + 15) / 16) : 0;
 }
 
 // Four groups of weight rows a wave instead of two (whose steps are twice as wide and whose sums leave more registers): where the weights'
