@@ -280,30 +280,30 @@ __global__ __launch_bounds__(256) void k_from_piles(PileArgs a) {
 template <class T>
 __global__ __launch_bounds__(256) void k_from_piles_grad(PileArgs a) {
     const int here = a.offsets[a.E], lane = threadIdx.x & 63;
-    const int64_t p = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (p >= (int64_t)a.T * a.K) return;
-    const int64_t pos = a.place[p];
-    const bool in = pos < here;
-    const float w = a.w[p];
-    const T *x = (const T *)a.x + p / a.K * a.ldx, *y = (const T *)a.y + pos * a.ldy;
-    T *out = (T *)a.out + pos * a.h;
-    float dot = 0.f;
-    for (int e = 8 * lane; e < a.h; e += 512) {
-        float g[8] = {}, v[8];
-        const int valid = a.h - e;
-        if (in) {
-            load_row<8>(x + e, valid, g);
-            load_row<8>(y + e, valid, v);
+    for (int64_t p = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); p < (int64_t)a.T * a.K; p += 4 * (int64_t)gridDim.x) {
+        const int64_t pos = a.place[p];
+        const bool in = pos < here;
+        const float w = a.w[p];
+        const T *x = (const T *)a.x + p / a.K * a.ldx, *y = (const T *)a.y + pos * a.ldy;
+        T *out = (T *)a.out + pos * a.h;
+        float dot = 0.f;
+        for (int e = 8 * lane; e < a.h; e += 512) {
+            float g[8] = {}, v[8];
+            const int valid = a.h - e;
+            if (in) {
+                load_row<8>(x + e, valid, g);
+                load_row<8>(y + e, valid, v);
 #pragma unroll
-            for (int c = 0; c < 8; c++) {
-                dot = fmaf(g[c], v[c], dot);
-                g[c] *= w;
+                for (int c = 0; c < 8; c++) {
+                    dot = fmaf(g[c], v[c], dot);
+                    g[c] *= w;
+                }
             }
+            store_row<8>(out + e, valid, g);
         }
-        store_row<8>(out + e, valid, g);
+        dot = wave_sum(dot);
+        if (lane == 0) a.dw[p] = dot;
     }
-    dot = wave_sum(dot);
-    if (lane == 0) a.dw[p] = dot;
 }
 
 static int check_piles(const char *what, int dtype, int64_t T, int K, int E, int64_t h) {
@@ -325,6 +325,7 @@ static PileArgs pile_args(const int *order, const int *place, const int *offsets
     a.per = (int)((h + 7) / 8);
     return a;
 }
+// (a launch holds fewer than 2^32 threads)
 static dim3 piece_grid(const PileArgs &a, int64_t rows) { return dim3((unsigned)std::min<int64_t>((rows * a.per + 255) / 256, 1 << 22)); }
 
 template <class R>
@@ -349,7 +350,7 @@ int from_piles_f32(int dtype, const float *rows, const float *w, int64_t T, int 
 }
 template <class T>
 static int from_piles_grad(const PileArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL(k_from_piles_grad<T>, dim3((unsigned)(((int64_t)a.T * a.K + 3) / 4)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(k_from_piles_grad<T>, dim3((unsigned)std::min<int64_t>(((int64_t)a.T * a.K + 3) / 4, 1 << 22)), dim3(256), 0, s, a);
     return check_launch("k_from_piles_grad");
 }
 

@@ -9,13 +9,15 @@ No counterpart in the reference, whose piles exist inside its kernels only. Rows
 stream of their own device; all arithmetic runs in libcwmoe.so, in a fixed order: the same inputs give the same bits. Shape and
 type errors raise ``CwError``.
 """
+import functools
 from dataclasses import dataclass
 from typing import Optional
 
 import torch
 
+from . import ops
 from ._lib import CW_EINVAL, CwError, check, lib
-from .i8 import _DTYPES, _elsewhere, _fail, _floats, _ptr, _same_device, _stream, _vector
+from .i8 import _DTYPES, _elsewhere, _fail, _floats, _ptr, _same_device, _stream
 
 
 @dataclass
@@ -45,19 +47,23 @@ def sort_picks(ids: torch.Tensor, n_experts: int) -> Piles:
     if _elsewhere(ids):
         with torch.cuda.device(ids.device):
             return sort_picks(ids, n_experts)
-    n, size = t * k, lib().cw_pile_tiles_bytes(t * k, n_experts)
+    n = t * k
+    sizes, need = _sizes(n, n_experts)
+    buf = ids.new_empty(sum(sizes))
+    order, _, place, _, offsets, _, tiles, ws = buf.split_with_sizes(sizes)
+    check(lib().cw_sort_picks(ids.data_ptr(), n, n_experts, order.data_ptr(), place.data_ptr(), offsets.data_ptr(), tiles.data_ptr(),
+                              ws.data_ptr() if need else None, need, _stream(ids)))
+    return Piles(order, place, offsets, tiles, t, k, n_experts)
+
+
+@functools.lru_cache(maxsize=256)
+def _sizes(picks, n_experts):
+    """int32s of order, place, offsets, tiles (each in whole 16 bytes) and the workspace; the workspace's bytes."""
+    size = lib().cw_pile_tiles_bytes(picks, n_experts)
     if size == 0:
         raise CwError(CW_EINVAL, lib().cw_last_error().decode(errors="replace"))
-    need = lib().cw_sort_picks_workspace_size(n, n_experts)
-    # (one allocation, in whole 16 bytes)
-    at = [0, (n + 3) // 4 * 4]
-    at += [2 * at[1], 2 * at[1] + (n_experts + 4) // 4 * 4]
-    buf = ids.new_empty(at[3] + size // 4 + need // 4)
-    order, place, offsets, tiles = buf[:n], buf[at[1]:at[1] + n], buf[at[2]:at[2] + n_experts + 1], buf[at[3]:at[3] + size // 4]
-    base = buf.data_ptr()
-    check(lib().cw_sort_picks(ids.data_ptr(), n, n_experts, base, base + 4 * at[1], base + 4 * at[2], base + 4 * at[3],
-                              base + 4 * at[3] + size if need else None, need, _stream(ids)))
-    return Piles(order, place, offsets, tiles, t, k, n_experts)
+    need = lib().cw_sort_picks_workspace_size(picks, n_experts)
+    return [picks, -picks % 4, picks, -picks % 4, n_experts + 1, -(n_experts + 1) % 4, size // 4, need // 4], need
 
 
 def _rows(x, n, h, what):
@@ -83,7 +89,10 @@ def to_piles(x: torch.Tensor, piles: Piles) -> torch.Tensor:
 
 
 def _weights(w, p):
-    _vector(w, p.tokens * p.top_k, "weights")
+    if w is not None:
+        ops._need(w, torch.float32, "weights")
+        if w.shape != (p.tokens, p.top_k):
+            _fail("weights %s: expected (%d, %d)", tuple(w.shape), p.tokens, p.top_k)
 
 
 def from_piles(rows: torch.Tensor, w: Optional[torch.Tensor], piles: Piles) -> torch.Tensor:

@@ -196,7 +196,7 @@ def test_refusals():
     bad = [lambda: piles.sort_picks(ids.long(), 3), lambda: piles.sort_picks(ids.cpu(), 3), lambda: piles.sort_picks(ids.t(), 3),
            lambda: piles.sort_picks(ids, 0), lambda: piles.sort_picks(ids, 1025), lambda: piles.sort_picks(ids[:, :0], 3),
            lambda: piles.to_piles(x[:3], p), lambda: piles.to_piles(x.double(), p), lambda: piles.to_piles(x.t(), p), lambda: piles.to_piles(x.cpu(), p),
-           lambda: piles.from_piles(x, w, p), lambda: piles.from_piles(rows, w.double(), p), lambda: piles.from_piles(rows, w[:3], p),
+           lambda: piles.from_piles(x, w, p), lambda: piles.from_piles(rows, w.double(), p), lambda: piles.from_piles(rows, w[:3], p), lambda: piles.from_piles(rows, w.view(2, 4), p),
            lambda: piles.from_piles_grad(x, rows, None, p), lambda: piles.from_piles_grad(x, rows.half(), w, p),
            lambda: piles.from_piles_grad(x, rows[:, :7], w, p), lambda: piles.from_piles_grad(rows, rows, w, p)]
     for call in bad:
