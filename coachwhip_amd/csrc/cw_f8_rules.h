@@ -45,13 +45,12 @@ inline int f8_few_groups(bool exact, int64_t m, int64_t n, int cus) {
     return m <= 16 * most ? (int)((m + 15) / 16) : 0;
 }
 
-// Four groups of weight rows a wave instead of two (whose steps are twice as wide and whose sums leave more registers): where the weights'
-// bytes bound, at up to 128 picks an expert, and there is a block for every CU twice. Measured in a graph, two / four groups, bf16: 128 experts of
-// 2,880 x 2,880, 64 tokens of 4 picks 239 / 202 us, 2,048 tokens (64 an expert) 318 / 275; 256 of 512 x 2,048, 512 of 8 (16) 57 / 51; 64 of
-// 1,408 x 2,048, 2,048 of 6 (192) 118 / 125; 8 of 4,096 x 2,048, 2,048 of 2 (512) 115 / 130; 256 of 1,024 x 2,048, 8 of 8 (228 blocks) 28 / 32.
+// Four groups of weight rows a wave instead of two (whose steps are twice as wide and whose sums leave more registers): where both the weights' bytes
+// and the products count, and there is a block for every CU twice. Measured in a graph, two / four groups, bf16: 128 experts of 2,880 x 2,880, 4 picks of
+// 64 tokens (2 an expert) 183 / 196 us, of 2,048 (64) 290 / 276; 256 of 512 x 2,048, 8 of 512 (16) 47.0 / 46.3; 256 of 2,048 x 512, 8 of 2,048
+// (64) 94 / 92; 64 of 1,408 x 2,048, 6 of 2,048 (192) 100 / 132; 8 of 4,096 x 2,048, 2 of 2,048 (512) 90 / 123; 256 of 1,024 x 2,048, 8 of 8 23.9 / 24.3.
 inline bool f8_four_groups(int E, int64_t picks, int64_t n, int cus) {
-    const double used = E * (1 - pow(1 - 1.0 / E, (double)picks));
-    return picks <= 128ll * E && used * ((n + 255) / 256) >= 2 * cus;
+    return picks >= 32ll * E && picks <= 128ll * E && E * ((n + 255) / 256) >= 2 * cus;
 }
 
 }  // namespace cw

@@ -27,6 +27,7 @@ def test_results_too_large_for_a_launch():
 
 def test_groups_of_the_experts():
     r = rules()
-    assert r.four_groups(128, 8192, 2880, CUS) and r.four_groups(256, 4096, 1024, CUS)
+    assert r.four_groups(128, 8192, 2880, CUS) and r.four_groups(256, 8192, 512, CUS)
     assert not r.four_groups(8, 4096, 4096, CUS)  # 512 picks an expert
-    assert not r.four_groups(256, 8, 1024, CUS)  # 32 blocks
+    assert not r.four_groups(256, 4096, 1024, CUS)  # 16
+    assert not r.four_groups(64, 4096, 1024, CUS)  # 256 blocks
