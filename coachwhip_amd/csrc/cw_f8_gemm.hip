@@ -81,7 +81,7 @@ __global__ __launch_bounds__(64 * F8_FEW_WAVES) void k_f8_few(F8MatArgs a) {
     f32x4 v = part[0][wave][lane];
 #pragma unroll
     for (int o = 1; o < HALF; o++) v += part[o][wave][lane];
-    if (strange) v = f8_strange_sums(a.x + m * a.rb, a.xs + m, a.m, a.w + n * a.rb, ws, a.rb, (int)min(a.n - n, (int64_t)4), v);
+    if (strange) f8_strange_sums(a.x + m * a.rb, a.xs + m, a.m, a.w + n * a.rb, ws, a.rb, (int)min(a.n - n, (int64_t)4), v);
     f8_store4((T *)a.y + m * a.ldy + n, (int)min(a.n - n, (int64_t)4), v, b);
 }
 
@@ -106,25 +106,31 @@ struct F8Ring {
     static_assert((TN + TM) % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && TM % 64 == 0 && TM / 64 <= WAVES && D * Q * (PER + 1) < 64, "whole loads for every wave");
     static_assert(LDS <= 159 * 1024, "the ring fits the CU");
 };
-// A wave's sums of rows whose scales, or whose weights' scales, are strange: rows m0.. of m_end (x's: xrow), columns n0.. of the matrix w, ws
-template <int MF, int NF, class XRow>
-__device__ __forceinline__ void f8_strange_tile(const F8MatArgs &a, const uint8_t *w, const float *ws, XRow xrow, int64_t m0, int64_t m_end, int64_t n0,
-                                                f32x4 (&acc)[MF][NF]) {
-    const int lane = threadIdx.x & 63;
-    const int64_t m = m0 + (lane & 15), n = n0 + 4 * (lane >> 4);
+// After a tile's outputs are stored, those with strange scales again: rows m0 .. m_end - 1 of y (x's: xrow), columns n0 .. n0 + cols - 1 of the
+// matrix w, ws. (Behind the stores, where no sums are held: beside them this cost the tiles of 256 x 256 registers, and 45 MB of spills.)
+template <class T, class XRow>
+__device__ __forceinline__ void f8_strange_tile(const F8MatArgs &a, const uint8_t *w, const float *ws, const float *bias, XRow xrow, int64_t m0, int64_t m_end,
+                                                int64_t n0, int cols) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const int quads = cols / 4, n = (int)(m_end - m0) * quads;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const int64_t m = m0 + i / quads, c = n0 + 4 * (i % quads);
+        if (c >= a.n) continue;
+        const int64_t row = xrow(m);
+        const int valid = (int)min(a.n - c, (int64_t)4);
+        f32x4 v;
+        if (!f8_strange_sums(a.x + row * a.rb, a.xs + row, a.m, w + c * a.rb, ws + c / F8_BLOCK * a.blocks, a.rb, valid, v)) continue;
+        float b[4];
 #pragma unroll
-    for (int i = 0; i < MF; i++)
-#pragma unroll
-        for (int j = 0; j < NF; j++) {
-            if (m + 16 * i >= m_end || n + 16 * j >= a.n) continue;
-            const int64_t row = xrow(m + 16 * i), col = n + 16 * j;
-            acc[i][j] = f8_strange_sums(a.x + row * a.rb, a.xs + row, a.m, w + col * a.rb, ws + col / F8_BLOCK * a.blocks, a.rb,
-                                        (int)min(a.n - col, (int64_t)4), acc[i][j]);
-        }
+        for (int k = 0; k < 4; k++) b[k] = bias ? bias[min(c + k, a.n - 1)] : 0.f;
+        f8_store4((T *)a.y + m * a.ldy + c, valid, v, b);
+    }
 }
 // A wave's sums stored: rows m0.. of m_end of y, columns n0.. . All biases are loaded before the bounds checks, from clamped places. Where all its
 // columns are inside, 16 rows at a time go through LDS (`stage`: 16 rows of this wave alone, chunk c of 16 bytes of row r at c ^ (r % chunks)) and
-// leave as whole rows, 16 bytes a lane (8,192 sorted rows of 2,880 x 2,880 262 -> 249 us; 8,192 x 4,096 x 4,096 145 either way, of which its
+// leave as whole rows, 16 bytes a lane (8,192 sorted rows of 2,880 x 2,880 262 -> 249 us; 8,192 x 4,096 x 4,096 the same either way, of which its
 // 67 MB take 24: all blocks write at once).
 template <class T, int MF, int NF>
 __device__ __forceinline__ void f8_finish(const F8MatArgs &a, const float *bias, int64_t m0, int64_t m_end, int64_t n0, const f32x4 (&acc)[MF][NF], uint8_t *stage) {
@@ -302,8 +308,9 @@ __global__ __launch_bounds__(64 * WN *WM, WN *WM / 4) void k_f8_tile(F8MatArgs a
         }
         buf = buf + 1 == R::D + 1 ? 0 : buf + 1;
     }
-    if (__syncthreads_or(strange)) f8_strange_tile(a, a.w, a.ws, [](int64_t r) { return r; }, m0 + 16 * MF * wm, a.m, n0 + 16 * NF * wn, acc);
+    const bool again = __syncthreads_or(strange);
     f8_finish<T, MF, NF>(a, a.bias, m0 + 16 * MF * wm, a.m, n0 + 16 * NF * wn, acc, lds + wave * 256 * NF * sizeof(T));
+    if (again) f8_strange_tile<T>(a, a.w, a.ws, a.bias, [](int64_t r) { return r; }, m0, min(m0 + R::TM, a.m), n0, R::TN);
 }
 
 // Many rows of x: tiles of 256 x 256, eight waves of 64 columns x 128 rows, two to a SIMD: one multiplies while the other scales and
@@ -396,8 +403,9 @@ __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int
 #pragma unroll
     for (int j = 0; j < 4; j++) add(7, j);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (no load may land in LDS that is another block's)
-    if (__syncthreads_or(strange)) f8_strange_tile(a, a.w, a.ws, [](int64_t r) { return r; }, m0 + 128 * wm, a.m, n0 + 64 * wn, acc);
+    const bool again = __syncthreads_or(strange);
     f8_finish<T, 8, 4>(a, a.bias, m0 + 128 * wm, a.m, n0 + 64 * wn, acc, lds + wave * 1024 * sizeof(T));
+    if (again) f8_strange_tile<T>(a, a.w, a.ws, a.bias, [](int64_t r) { return r; }, m0, min(m0 + R::TM, a.m), n0, R::TN);
 }
 
 // Sorted rows times their experts' matrices: a tile of up to 128 positions, 64 NW columns.
@@ -432,10 +440,11 @@ __global__ __launch_bounds__(256, 2) void k_f8_experts(F8MatArgs a, int n_blocks
         f32x4 acc[MB][NW];
         auto row_at = [&](int64_t pos) __attribute__((always_inline)) { return a.order ? (int64_t)(a.order[pos] / a.K) : pos; };
         const bool odd = f8_stream<MB, NW, 1, EXACT>(lds, o, [&](int r) { return row_at(tl.pos0 + min(r, tl.m - 1)); }, wrow, acc);
-        if (__syncthreads_or(odd))
-            f8_strange_tile(a, a.w + tl.expert * a.w_stride, a.ws + tl.expert * a.ws_stride, row_at, tl.pos0, tl.pos0 + tl.m, n0, acc);
-        f8_finish<T, MB, NW>(a, a.bias ? a.bias + tl.expert * a.n : nullptr, tl.pos0, tl.pos0 + tl.m, n0, acc,
-                             lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 256 * NW * sizeof(T));
+        const bool again = __syncthreads_or(odd);
+        const float *bias = a.bias ? a.bias + tl.expert * a.n : nullptr;
+        f8_finish<T, MB, NW>(a, bias, tl.pos0, tl.pos0 + tl.m, n0, acc, lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 256 * NW * sizeof(T));
+        if (again)
+            f8_strange_tile<T>(a, a.w + tl.expert * a.w_stride, a.ws + tl.expert * a.ws_stride, bias, row_at, tl.pos0, tl.pos0 + tl.m, (int64_t)COLS * nb, COLS);
     });
 }
 

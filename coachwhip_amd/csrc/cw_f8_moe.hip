@@ -83,9 +83,12 @@ __global__ __launch_bounds__(64 * F8_FEW_WAVES, NS > 4 ? 2 : 4) void k_f8_few_ga
         v[i] = part[i][threadIdx.x];
 #pragma unroll
         for (int q = 2; q < F8_FEW_WAVES; q += 2) v[i] += part[q + i][threadIdx.x];
-        if (strange)
-            v[i] = f8_strange_sums(a.x + (int64_t)t * a.rbh, a.xs + t, a.T, a.w[i] + e * a.stride[i] + (int64_t)n * a.rbh,
-                                   a.ws[i] + (e * ((a.I + 127) / 128) + n0 / F8_BLOCK) * blocks, a.rbh, 1, f32x4{v[i], 0.f, 0.f, 0.f})[0];
+        if (strange) {
+            f32x4 sum = {v[i], 0.f, 0.f, 0.f};
+            f8_strange_sums(a.x + (int64_t)t * a.rbh, a.xs + t, a.T, a.w[i] + e * a.stride[i] + (int64_t)n * a.rbh,
+                            a.ws[i] + (e * ((a.I + 127) / 128) + n0 / F8_BLOCK) * blocks, a.rbh, 1, sum);
+            v[i] = sum[0];
+        }
         if (a.bias[i]) v[i] += a.bias[i][e * a.I + n];
     }
     a.h[((int64_t)t * a.K + j) * a.ldh + n] = glu(v[0], v[1], a.glu);
@@ -176,8 +179,11 @@ __global__ __launch_bounds__(64 * F8_FEW_WAVES, NS > 4 ? 2 : 4) void k_f8_few_do
     for (int q = 1; q < F8_FEW_WAVES; q++) v += part[q][threadIdx.x];
     if (strange) {
         v = 0.f;
-        for (int j = 0; j < a.K; j++)
-            v = fmaf(f8_strange_sums(hq + j * a.rbi, hs + j * blocks, 1, matrix_of(j) + (int64_t)n * a.rbi, scales_of(j), a.rbi, 1, f32x4{}, true)[0], wk[j], v);
+        for (int j = 0; j < a.K; j++) {
+            f32x4 sum;
+            f8_strange_sums(hq + j * a.rbi, hs + j * blocks, 1, matrix_of(j) + (int64_t)n * a.rbi, scales_of(j), a.rbi, 1, sum, true);
+            v = fmaf(sum[0], wk[j], v);
+        }
     }
     if (a.bias[2])
         for (int j = 0; j < a.K; j++) v = fmaf(wk[j], a.bias[2][(int64_t)ids[j] * a.H + n], v);
@@ -263,7 +269,7 @@ __global__ __launch_bounds__(256, 2) void k_f8_gateup(F8GateUpArgs a, int n_bloc
                     const int n = col + 16 * (j & 1);
                     if (n >= a.I) continue;
                     const int64_t row = row_at(16 * mb + (lane & 15));
-                    acc[mb][j] = f8_strange_sums(a.x + row * a.rb, a.xs + row, a.m, a.w[j >> 1] + tl.expert * a.stride[j >> 1] + (int64_t)n * a.rb,
+                    f8_strange_sums(a.x + row * a.rb, a.xs + row, a.m, a.w[j >> 1] + tl.expert * a.stride[j >> 1] + (int64_t)n * a.rb,
                                                  o.ws0[j >> 1], a.rb, min(a.I - n, 4), acc[mb][j]);
                 }
         }

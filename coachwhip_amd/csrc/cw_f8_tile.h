@@ -57,11 +57,11 @@ __device__ __forceinline__ bool f8_strange(float s) {
     const uint32_t u = __float_as_uint(s) & 0x7FFFFFFFu;
     return u - 1 < (64u << 23) - 1 || u - ((190u << 23) + 1) < (255u << 23) - ((190u << 23) + 1);
 }
-// Four neighbouring outputs, weight rows w .. w + 3 rb (of `valid`; the last again past them) times one row of x, if one of its scales or of
-// theirs is strange, else acc: whether is a matter of this row and these weights alone, whatever lies beside them. Slow: a lane reads
+// Four neighbouring outputs, weight rows w .. w + 3 rb (of `valid`; the last again past them) times one row of x, into acc if one of its scales or
+// of theirs is strange (or it is said so): whether is a matter of this row and these weights alone, whatever lies beside them. Slow: a lane reads
 // its rows by itself.
-__device__ __forceinline__ f32x4 f8_strange_sums(const uint8_t *x, const float *xs, int64_t m, const uint8_t *w, const float *ws, int rb, int valid, f32x4 acc,
-                                                 bool strange = false) {
+__device__ __forceinline__ bool f8_strange_sums(const uint8_t *x, const float *xs, int64_t m, const uint8_t *w, const float *ws, int rb, int valid, f32x4 &acc,
+                                                bool strange = false) {
     double sum[4] = {};
 #pragma unroll 1
     for (int b = 0; b < rb / F8_BLOCK; b++) {
@@ -85,7 +85,7 @@ __device__ __forceinline__ f32x4 f8_strange_sums(const uint8_t *x, const float *
     if (strange)
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[i] = (float)sum[i];
-    return acc;
+    return strange;
 }
 
 // A weights' scale by a scalar load, at a wave-uniform place. (A vector load, which the compiler makes of it beside the inline waits, returns after
