@@ -25,7 +25,8 @@ struct F8MatArgs {
 
 // Few rows of x: a block takes 16 rows of W and up to 16 MB of x over all of k, its waves the steps of 128 codes in turn, both
 // operands straight from memory into registers (no byte of either is used by two waves of a block). The waves' sums meet in LDS: the
-// upper four's onto the lower four's, then those in their order.
+// upper four's onto the lower four's, then those in their order. One row of 2048 x 2048: 4.0 us, a launch, one round trip and the join; 77 rows of 4001 x 2880 in
+// f32 12.2 in a graph: each block makes x's codes f16 for itself.
 template <class T, int MB, bool EXACT>
 __global__ __launch_bounds__(64 * F8_FEW_WAVES) void k_f8_few(F8MatArgs a) {
     constexpr int HALF = F8_FEW_WAVES / 2;
@@ -131,7 +132,7 @@ __device__ __forceinline__ void f8_strange_tile(const F8MatArgs &a, const uint8_
 // A wave's sums stored: rows m0.. of m_end of y, columns n0.. . All biases are loaded before the bounds checks, from clamped places. Where all its
 // columns are inside, 16 rows at a time go through LDS (`stage`: 16 rows of this wave alone, chunk c of 16 bytes of row r at c ^ (r % chunks)) and
 // leave as whole rows, 16 bytes a lane (8,192 sorted rows of 2,880 x 2,880 262 -> 249 us; 8,192 x 4,096 x 4,096 the same either way, of which its
-// 67 MB take 24: all blocks write at once).
+// 67 MB take 12 to 16: all blocks write at once).
 template <class T, int MF, int NF>
 __device__ __forceinline__ void f8_finish(const F8MatArgs &a, const float *bias, int64_t m0, int64_t m_end, int64_t n0, const f32x4 (&acc)[MF][NF], uint8_t *stage) {
     const int lane = threadIdx.x & 63;
@@ -317,6 +318,8 @@ __global__ __launch_bounds__(64 * WN *WM, WN *WM / 4) void k_f8_tile(F8MatArgs a
 // adds. Two LDS stages of 2 x 256 rows x 128 codes and 256 scales, swizzled as in k_f8_tile. A wave's four fragments of W stay in
 // registers for the step, x's eight pass by, each read while the one before is multiplied; the next step's first ones while the
 // last is, before which all waves meet: the stage of the next step is then in, and this step's, all of which has been read, free for the one after.
+// 8,192 x 4,096 x 4,096, bf16: 121 to 142 us by the box (1.9 to 2.3 PFLOP/s), 8,192 cubed 445 to 452 (2.4 to 2.5); matrix pipe 54 % busy, waves at waits and the barrier 29 %,
+// waiting to issue 30 %.
 template <class T>
 __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int tiles_n) {
     using R = F8Ring<4, 2, 4, 8, 1, 2>;
@@ -408,7 +411,8 @@ __global__ __launch_bounds__(512, 2) void k_f8_big(F8MatArgs a, int tiles_m, int
     if (again) f8_strange_tile<T>(a, a.w, a.ws, a.bias, [](int64_t r) { return r; }, m0, min(m0 + R::TM, a.m), n0, R::TN);
 }
 
-// Sorted rows times their experts' matrices: a tile of up to 128 positions, 64 NW columns.
+// Sorted rows times their experts' matrices: a tile of up to 128 positions, 64 NW columns. 8,192 positions over 128 experts of 2,880 x 2,880: 249 to 256 us, 4.4 TB/s
+// (1.1 GB of weights, 47 MB of results); 64 over 256 of 1,024 x 2,048 24 (5.0).
 template <class T, int NW, bool EXACT>
 __global__ __launch_bounds__(256, 2) void k_f8_experts(F8MatArgs a, int n_blocks) {
     extern __shared__ __align__(1024) uint8_t lds[];

@@ -25,7 +25,8 @@ struct F8FewArgs {
 // Gate and up of one pick of a token, 16 columns a block: 16 rows of either matrix against the token's row (in all 16 columns of the
 // instruction: its sums cost nothing here, unpacking the codes for the vector unit 1.3 times the bytes' time), the steps of 128
 // codes dealt to eight waves, even ones gate, odd ones up, their sums joined in LDS in the waves' order. One wave routes the token for its block, no
-// further than this pick; the last pick's first block, which goes all the way, stores the routing.
+// further than this pick; the last pick's first block, which goes all the way, stores the routing. One token of 8 picks of 512 x 2,048: 7.1 us for 16.8 MB, a
+// chain of logits, routing, weights, sums; 4 tokens of 4 picks of 2,880 x 2,880, with down: 96 us, 4.1 TB/s.
 template <int PER, int NS, bool EXACT>
 __global__ __launch_bounds__(64 * F8_FEW_WAVES, NS > 4 ? 2 : 4) void k_f8_few_gateup(F8FewArgs a) {
     __shared__ uint32_t expert;
@@ -96,7 +97,8 @@ __global__ __launch_bounds__(64 * F8_FEW_WAVES, NS > 4 ? 2 : 4) void k_f8_few_ga
 
 // Down and the weighted sum of a token, 16 outputs a block: the block makes the token's K hidden rows codes in LDS (every block of the token does,
 // one, two, four or eight waves a row; 32 lanes hold a group of 128 columns), then its waves take the steps of the K rows end to end in turn. The hidden
-// rows are asked for before the weights: loads return in order, and the codes are made while the weights come in.
+// rows are asked for before the weights: loads return in order, and the codes are made while the weights come in. One token of 8 picks of 512 x 2,048: 5.7
+// us for 8.4 MB, a chain of the hidden rows, their codes, the sums.
 template <class T, int NS, bool EXACT>
 __global__ __launch_bounds__(64 * F8_FEW_WAVES, NS > 4 ? 2 : 4) void k_f8_few_down(F8FewArgs a) {
     constexpr int NH = NS < 12 ? (NS + 1) / 2 : 6;  // pieces of a hidden row held in registers (the others are read later)
@@ -233,6 +235,7 @@ struct F8GateUpArgs {
 // Gate and up of a tile of up to 128 positions, 128 columns of both, and their activation as codes: a block holds whole groups of 128 columns of
 // its rows, so that the hidden rows leave it as codes and nothing else is written (f32 hidden rows of 2,048 tokens of 4 picks of 2,880 columns: 94 MB
 // written and read again). A wave has 32 columns: the largest magnitude of a row's 128 meets in LDS, as do the codes, which leave as whole rows of 128.
+// 2,048 tokens of 4 picks over 128 experts of 2,880 x 2,880: 470 to 490 us, 4.4 TB/s of weights; the waves wait for loads 35 % of their cycles and to issue 46 %.
 template <bool EXACT>
 __global__ __launch_bounds__(256, 2) void k_f8_gateup(F8GateUpArgs a, int n_blocks) {
     extern __shared__ __align__(1024) uint8_t lds[];
@@ -354,7 +357,7 @@ static int check_desc(const cw_f8_moe_desc *d, int T) {
     CW_REQUIRE(d->act == CW_ACT_SILU || d->act == CW_ACT_CLAMPED_SWIGLU, "f8 moe: unknown activation %d", d->act);
     // (a launch holds fewer than 2^32 threads)
     const int64_t TK = (int64_t)T * d->top_k, blocks = pile_max_tiles(TK, d->n_experts) * f8_blocks(std::max(d->inter, d->hidden));
-    if (TK >= 1 << 28 || blocks >= 1 << 23 || TK * f8_blocks(d->inter) >= 1 << 27)
+    if (TK >= 1 << 28 || blocks >= 1 << 23)
         return set_error(CW_ENOTSUP, "f8 moe: %d tokens of %d picks, hidden %d, inter %d", T, d->top_k, d->hidden, d->inter);
     for (int m = 0; m < 3; m++) {
         const int64_t need = (m == 2 ? d->hidden : d->inter) * f8_row_bytes(m == 2 ? d->inter : d->hidden);
