@@ -52,5 +52,14 @@ inline int f8_few_groups(bool exact, int64_t m, int64_t n, int cus) {
 inline bool f8_four_groups(int E, int64_t picks, int64_t n, int cus) {
     return picks >= 32ll * E && picks <= 128ll * E && E * ((n + 255) / 256) >= 2 * cus;
 }
+// Few experts of many picks: tiles of 128 sorted rows x 128 of W, one workgroup a CU, whose eight waves share every code through LDS (the kernel of two
+// groups reads each expert's rows once for 32 of W). With three blocks of W or more to a CU the two workgroups that the other kernel keeps there hide
+// more. Measured in a graph, two groups / tiles, bf16: 8 experts of 4,096 x 2,048, 32 picks each 17.4 / 19.3 us, 64 23.6 / 19.9, 256 57.0 / 48.5,
+// 512 90.4 / 80.7, 2,048 256 / 259; 16 of 512 x 4,096 (256) 49.3 / 27.2; 32 of 2,048 x 2,048 (256) 84.1 / 74.7; 64 of 1,408 x 2,048 (64) 45.6 / 47.7,
+// (96) 59.5 / 50.9, (384) 158 / 154; 128 of 1,024 x 1,024, four blocks to a CU (64) 36.9 / 44.2, (128) 62.0 / 63.2; 128 of 2,880 x 2,880 (192) 456 / 506.
+// Exact sums: 8 of 4,096 x 2,048 (64) 30.7 / 28.1, (128) 59.6 / 53.1, (512) 140 / 116; 64 of 1,408 x 2,048 (64) 62.8 / 71.9, (384) 265 / 253.
+inline bool f8_sorted_tiles(bool exact, int E, int64_t picks, int64_t n, int cus) {
+    return picks >= (exact ? 128ll : 64ll) * E && E * ((n + 127) / 128) <= 3 * cus;
+}
 
 }  // namespace cw

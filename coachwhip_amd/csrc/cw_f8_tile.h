@@ -90,10 +90,11 @@ __device__ __forceinline__ bool f8_strange_sums(const uint8_t *x, const float *x
 
 // A weights' scale by a scalar load, at a wave-uniform place. (A vector load, which the compiler makes of it beside the inline waits, returns after
 // all loads asked for before it: with the weights of the steps ahead in flight it waits for them.)
-__device__ __forceinline__ const float *f8_uniform(const float *p) {
+template <class P>
+__device__ __forceinline__ const P *f8_uniform(const P *p) {
     const uint64_t u = (uint64_t)p;
     const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)u), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
-    return (const float *)(lo | (uint64_t)hi << 32);
+    return (const P *)(lo | (uint64_t)hi << 32);
 }
 __device__ __forceinline__ float f8_scale_at(const float *p) { return *(const __attribute__((address_space(4))) float *)(uint64_t)p; }
 
@@ -280,6 +281,9 @@ __device__ __forceinline__ bool f8_item_of_block(const void *list, int n_blocks,
     nb = __builtin_amdgcn_readfirstlane(in / any.of);
     if (any.of == 1) tl = any;
     else tl = tiles[__builtin_amdgcn_readfirstlane(any.first + in - nb * any.of)];
+    tl.expert = __builtin_amdgcn_readfirstlane(tl.expert);
+    tl.pos0 = __builtin_amdgcn_readfirstlane(tl.pos0);
+    tl.m = __builtin_amdgcn_readfirstlane(tl.m);
     return true;
 }
 // f(the number of 16s that a tile's positions take), of those that a kernel is built for

@@ -31,3 +31,26 @@ def test_groups_of_the_experts():
     assert not r.four_groups(8, 4096, 4096, CUS)  # 512 picks an expert
     assert not r.four_groups(256, 4096, 1024, CUS)  # 16
     assert not r.four_groups(64, 4096, 1024, CUS)  # 256 blocks
+
+
+# (exact, tokens, experts, picks a token, n, k) of every kernel of the experts' products, which tests/test_gpu_f8_instances.py runs
+EXPERTS = {"two": [(False, 37, 8, 2, 300, 260), (True, 200, 8, 4, 300, 260)], "four": [(False, 2100, 256, 4, 300, 260), (True, 2100, 256, 4, 300, 260)],
+           "tiles": [(False, 131, 4, 2, 300, 260), (True, 131, 2, 2, 300, 260), (False, 1000, 5, 3, 129, 1000), (True, 1000, 5, 3, 129, 1000)]}
+
+
+def experts_form(exact, t, e, kp, n, k):
+    r = rules()
+    return "tiles" if r.sorted_tiles(exact, e, t * kp, n, CUS) else "four" if r.four_groups(e, t * kp, n, CUS) else "two"
+
+
+@pytest.mark.parametrize("form", EXPERTS)
+def test_every_kernel_of_the_experts_is_reached(form):
+    assert {experts_form(*i) for i in EXPERTS[form]} == {form}
+
+
+@pytest.mark.parametrize("exact", [0, 1])
+def test_few_experts_of_many_picks_take_tiles(exact):
+    r = rules()
+    few = 127 if exact else 63  # picks an expert, one under the least
+    assert r.sorted_tiles(exact, 8, 4096, 4096, CUS) and r.sorted_tiles(exact, 8, 8 * (few + 1), 4096, CUS) and not r.sorted_tiles(exact, 8, 8 * few, 4096, CUS)
+    assert r.sorted_tiles(exact, 64, 64 * 200, 12 * 128, CUS) and not r.sorted_tiles(exact, 64, 64 * 200, 12 * 128 + 1, CUS)  # three blocks of W to a CU
