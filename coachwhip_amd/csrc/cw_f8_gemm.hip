@@ -591,7 +591,7 @@ int f8_matmul_experts(const uint8_t *w, int64_t w_stride, const float *w_scale, 
     a.E = n_experts;
     const int cus = (int)resident_blocks(1);
     const bool sorted = most * ((n + 127) / 128) < F8_MAX_TILES && f8_sorted_tiles(exact, n_experts, picks, n, cus);
-    const bool four = f8_four_groups(n_experts, picks, n, cus);
+    const bool four = f8_four_groups(n_experts, picks, n, k, cus);
     if (ydtype == CW_F16) return f8_experts<_Float16, false>(a, most, sorted, four, s);
     if (ydtype == CW_BF16) return f8_experts<bf16_t, false>(a, most, sorted, four, s);
     return exact ? f8_experts<float, true>(a, most, sorted, four, s) : f8_experts<float, false>(a, most, sorted, four, s);

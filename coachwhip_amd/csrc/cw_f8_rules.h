@@ -46,14 +46,16 @@ inline int f8_few_groups(bool exact, int64_t m, int64_t n, int cus) {
 }
 
 // Four groups of weight rows a wave instead of two (whose steps are twice as wide and whose sums leave more registers): where both the weights' bytes
-// and the products count, and there is a block for every CU twice. Measured in a graph, two / four groups, bf16: 128 experts of 2,880 x 2,880, 4 picks of
-// 64 tokens (2 an expert) 183 / 196 us, of 2,048 (64) 290 / 276; 256 of 512 x 2,048, 8 of 512 (16) 47.0 / 46.3; 256 of 2,048 x 512, 8 of 2,048
-// (64) 94 / 92; 64 of 1,408 x 2,048, 6 of 2,048 (192) 100 / 132; 8 of 4,096 x 2,048, 2 of 2,048 (512) 90 / 123; 256 of 1,024 x 2,048, 8 of 8 23.9 / 24.3.
-inline bool f8_four_groups(int E, int64_t picks, int64_t n, int cus) {
-    return picks >= 32ll * E && picks <= 128ll * E && E * ((n + 255) / 256) >= 2 * cus;
+// and the products count, and there is a block for every CU twice. A long k ends that
+// at 64 picks. Measured in a graph, two / four groups, bf16: 128 experts of 2,880 x 2,880, 2 picks each 178 / 190 us, 32 230 / 218, 64 259 / 246, 94
+// 291 / 316, 128 360 / 358 to 389; 256 of 512 x 2,048 (16) 47.1 / 45.6, (64) 66.8 / 56.9; 256 of 1,024 x 2,048 (64) 136 / 125; 256 of 2,048 x 512
+// (16) 65.0 / 52.3, (128) 131 / 120, (192) 177 / 156, of 512 x 2,048 (256) 179 / 171. Exact sums: 128 of 2,880 x 2,880 (64) 326 / 319, (128)
+// 543 / 622. With fewer blocks: 64 of 1,408 x 2,048 (192) 100 / 132; 8 of 4,096 x 2,048 (512) 90 / 123.
+inline bool f8_four_groups(int E, int64_t picks, int64_t n, int64_t k, int cus) {
+    return picks >= 32ll * E && picks <= (k > 2048 ? 64ll : 128ll) * E && E * ((n + 255) / 256) >= 2 * cus;
 }
 // Few experts of many picks: tiles of 128 sorted rows x 128 of W, one workgroup a CU, whose eight waves share every code through LDS (the kernel of two
-// groups reads each expert's rows once for 32 of W). With three blocks of W or more to a CU the two workgroups that the other kernel keeps there hide
+// groups reads each expert's rows once for 32 of W). With more than three blocks of W to a CU the two workgroups that the other kernel keeps there hide
 // more. Measured in a graph, two groups / tiles, bf16: 8 experts of 4,096 x 2,048, 32 picks each 17.4 / 19.3 us, 64 23.6 / 19.9, 256 57.0 / 48.5,
 // 512 90.4 / 80.7, 2,048 256 / 259; 16 of 512 x 4,096 (256) 49.3 / 27.2; 32 of 2,048 x 2,048 (256) 84.1 / 74.7; 64 of 1,408 x 2,048 (64) 45.6 / 47.7,
 // (96) 59.5 / 50.9, (384) 158 / 154; 128 of 1,024 x 1,024, four blocks to a CU (64) 36.9 / 44.2, (128) 62.0 / 63.2; 128 of 2,880 x 2,880 (192) 456 / 506.

@@ -12,7 +12,8 @@ extern "C" {
 int few_groups(int exact, long m, long n, int cus) { return cw::f8_few_groups(exact, m, n, cus); }
 int pick_tile(int exact, long m, long n, int rb, int cus) { return cw::f8_pick_tile(exact, m, n, rb, cus); }
 int tile_rows(int i) { return cw::F8_TILES[0][i].tm; }
-int four_groups(int E, long picks, long n, int cus) { return cw::f8_four_groups(E, picks, n, cus); }
+int four_groups(int E, long picks, long n, int cus) { return cw::f8_four_groups(E, picks, n, 2048, cus); }
+int four_groups_of(int E, long picks, long n, long k, int cus) { return cw::f8_four_groups(E, picks, n, k, cus); }
 int sorted_tiles(int exact, int E, long picks, long n, int cus) { return cw::f8_sorted_tiles(exact, E, picks, n, cus); }
 }
 """
@@ -30,6 +31,7 @@ def rules():
     lib.few_groups.argtypes = [ctypes.c_int, ctypes.c_long, ctypes.c_long, ctypes.c_int]
     lib.pick_tile.argtypes = [ctypes.c_int, ctypes.c_long, ctypes.c_long, ctypes.c_int, ctypes.c_int]
     lib.four_groups.argtypes = [ctypes.c_int, ctypes.c_long, ctypes.c_long, ctypes.c_int]
+    lib.four_groups_of.argtypes = [ctypes.c_int, ctypes.c_long, ctypes.c_long, ctypes.c_long, ctypes.c_int]
     lib.sorted_tiles.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_long, ctypes.c_long, ctypes.c_int]
     return lib
 

@@ -40,7 +40,7 @@ EXPERTS = {"two": [(False, 37, 8, 2, 300, 260), (True, 200, 8, 4, 300, 260)], "f
 
 def experts_form(exact, t, e, kp, n, k):
     r = rules()
-    return "tiles" if r.sorted_tiles(exact, e, t * kp, n, CUS) else "four" if r.four_groups(e, t * kp, n, CUS) else "two"
+    return "tiles" if r.sorted_tiles(exact, e, t * kp, n, CUS) else "four" if r.four_groups_of(e, t * kp, n, k, CUS) else "two"
 
 
 @pytest.mark.parametrize("form", EXPERTS)
@@ -54,3 +54,9 @@ def test_few_experts_of_many_picks_take_tiles(exact):
     few = 127 if exact else 63  # picks an expert, one under the least
     assert r.sorted_tiles(exact, 8, 4096, 4096, CUS) and r.sorted_tiles(exact, 8, 8 * (few + 1), 4096, CUS) and not r.sorted_tiles(exact, 8, 8 * few, 4096, CUS)
     assert r.sorted_tiles(exact, 64, 64 * 200, 12 * 128, CUS) and not r.sorted_tiles(exact, 64, 64 * 200, 12 * 128 + 1, CUS)  # three blocks of W to a CU
+
+
+def test_four_groups_end_sooner_with_a_long_k():
+    r = rules()
+    assert r.four_groups_of(128, 8192, 2880, 2880, CUS) and not r.four_groups_of(128, 8193, 2880, 2880, CUS)
+    assert r.four_groups_of(128, 16384, 2880, 2048, CUS) and not r.four_groups_of(128, 16385, 2880, 2048, CUS)
