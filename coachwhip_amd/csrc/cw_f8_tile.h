@@ -203,8 +203,8 @@ __device__ __forceinline__ bool f8_stream(uint8_t *lds, const F8Operands<MATS> &
         for (int i = 0; i < MATS; i++)
 #pragma unroll
             for (int q = 0; q < Q; q++) {
-                sn[i][q] = sw[i][q];
-                odd |= f8_strange(sn[i][q]);
+                odd |= f8_strange(sw[i][q]);
+                sn[i][q] = step * Q + q < a.blocks ? sw[i][q] : 0.f;  // (past the end the last one again, which may be infinite)
             }
         fetch_sw(step + 1);
 #pragma unroll
