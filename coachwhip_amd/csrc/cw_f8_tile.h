@@ -51,11 +51,13 @@ struct F8Frag<true> {
 };
 
 // A step's sum, below 2^25, is multiplied with the product of two scales in f32, fma(p, sx sw, acc), where both are usual ones: zero, from
-// 2^-63 to 2^63, infinite or NaN (their product is zero, a normal number, infinite or NaN). Others, which a program's own codes may have,
-// take their outputs through f8_strange_sums: in 64 bits, so that nothing but the result leaves f32's range.
+// 2^-63 to 2^47, infinite or NaN. Their product is then zero, a normal number, infinite or NaN, and 256 steps' sums of finite ones stay below
+// 2^127, in any order. Others, which a program's own codes may have, take their outputs through f8_strange_sums: in 64 bits, so that nothing but
+// the result leaves f32's range.
 __device__ __forceinline__ bool f8_strange(float s) {
+    constexpr uint32_t LOW = 64u << 23, HIGH = 174u << 23, INF = 255u << 23;
     const uint32_t u = __float_as_uint(s) & 0x7FFFFFFFu;
-    return u - 1 < (64u << 23) - 1 || u - ((190u << 23) + 1) < (255u << 23) - ((190u << 23) + 1);
+    return u - 1 < LOW - 1 || u - (HIGH + 1) < INF - (HIGH + 1);
 }
 // Four neighbouring outputs, weight rows w .. w + 3 rb (of `valid`; the last again past them) times one row of x, into acc if one of its scales or
 // of theirs is strange (or it is said so): whether is a matter of this row and these weights alone, whatever lies beside them. Slow: a lane reads
