@@ -592,7 +592,7 @@ int f8_matmul_experts(const uint8_t *w, int64_t w_stride, const float *w_scale, 
     const int cus = (int)resident_blocks(1);
     const bool sorted = most * ((n + 127) / 128) < F8_MAX_TILES && f8_sorted_tiles(exact, n_experts, picks, n, cus);
     const bool four = f8_four_groups(n_experts, picks, n, k, cus);
-    if (ydtype == CW_F16) return f8_experts<_Float16, false>(a, most, sorted, four, s);
+    if (ydtype == CW_F16) return f8_experts<_Float16, true>(a, most, sorted, four, s);
     if (ydtype == CW_BF16) return f8_experts<bf16_t, false>(a, most, sorted, four, s);
     return exact ? f8_experts<float, true>(a, most, sorted, four, s) : f8_experts<float, false>(a, most, sorted, four, s);
 }
@@ -608,7 +608,7 @@ int cw_f8_matmul(const uint8_t *w, const float *w_scale, int64_t n, int64_t k, c
     if (int rc = check_product("f8_matmul", ydtype, n, k, m, ldy)) return rc;
     if (m == 0) return CW_OK;
     const int rb = (int)f8_row_bytes(k), cus = (int)resident_blocks(1);
-    const bool exact = ydtype == CW_F32;
+    const bool exact = ydtype != CW_BF16;
     const int few_groups = f8_few_groups(exact, m, n, cus), tile = few_groups ? 0 : f8_pick_tile(exact, m, n, rb, cus);
     if (tile < 0) return set_error(CW_ENOTSUP, "f8_matmul: %lld x %lld outputs", (long long)m, (long long)n);
     CW_REQUIRE(w && w_scale && x && x_scale && y, "f8_matmul: null pointer");
@@ -623,7 +623,7 @@ int cw_f8_matmul(const uint8_t *w, const float *w_scale, int64_t n, int64_t k, c
 int cw_f8_matmul_experts(const uint8_t *w, int64_t w_stride, const float *w_scale, int n_experts, int64_t n, int64_t k, const uint8_t *x,
                          const float *x_scale, int64_t m, const int32_t *order, int K, int64_t picks, const void *tiles, const float *bias,
                          int ydtype, void *y, int64_t ldy, cw_stream_t stream) {
-    return f8_matmul_experts(w, w_stride, w_scale, n_experts, n, k, x, x_scale, m, order, K, picks, tiles, bias, ydtype, y, ldy, ydtype == CW_F32,
+    return f8_matmul_experts(w, w_stride, w_scale, n_experts, n, k, x, x_scale, m, order, K, picks, tiles, bias, ydtype, y, ldy, ydtype != CW_BF16,
                              (hipStream_t)stream);
 }
 

@@ -425,9 +425,9 @@ int cw_f8_moe_layer(const cw_f8_moe_desc *d, const uint8_t *x, const float *x_sc
         a.wt = w;
         a.h = (float *)(base + L.h);
         a.out = out;
-        // (as below: hidden codes of results in f16 and f32 from exact products)
+        // (as below: results in f16 and f32 from exact products)
         if (int rc = ydtype == CW_BF16 ? few_gateup<false>(a, s) : few_gateup<true>(a, s)) return rc;
-        return ydtype == CW_F16 ? few_down<_Float16, false>(a, s) : ydtype == CW_BF16 ? few_down<bf16_t, false>(a, s) : few_down<float, true>(a, s);
+        return ydtype == CW_F16 ? few_down<_Float16, true>(a, s) : ydtype == CW_BF16 ? few_down<bf16_t, false>(a, s) : few_down<float, true>(a, s);
     }
     if (int rc = cw_route_topk(logits, T, E, K, d->norm, ids, w, stream)) return rc;
     if (int rc = cw_sort_picks(ids, TK, E, order, place, offsets, tiles, base + L.sort, cw_sort_picks_workspace_size(TK, E), stream)) return rc;
@@ -453,7 +453,7 @@ int cw_f8_moe_layer(const cw_f8_moe_desc *d, const uint8_t *x, const float *x_sc
     a.hq = hq;
     a.hs = hs;
     // bf16's rounding covers what the 8-bit instruction leaves out of gate and up (hidden codes that take their neighbour: 1.1e-3 of a result,
-    // beside 1.7e-3); results in f16 and f32 have hidden codes from exact products, those in f32 exact products in down too
+    // beside 1.7e-3); results in f16 and f32 have exact products in gate and up, whose codes hang on them, and in down
     const int blocks = (int)f8_blocks(I);
     const dim3 grid((unsigned)((pile_max_tiles(TK, E) * blocks + 7) / 8 * 8));
     constexpr int LDS = F8Stream<8, 4>::LDS;
@@ -461,7 +461,7 @@ int cw_f8_moe_layer(const cw_f8_moe_desc *d, const uint8_t *x, const float *x_sc
     else hipLaunchKernelGGL(k_f8_gateup<true>, grid, dim3(256), LDS, s, a, blocks);
     if (int rc = check_launch("k_f8_gateup")) return rc;
     if (int rc = f8_matmul_experts(d->w[2], d->slot_stride[2], d->scale[2], E, H, I, hq, hs, TK, nullptr, K, TK, tiles, d->bias[2], CW_F32, dn, H,
-                                   ydtype == CW_F32, s))
+                                   ydtype != CW_BF16, s))
         return rc;
     return from_piles_f32(ydtype, dn, w, T, K, E, H, place, offsets, out, s);
 }

@@ -9,7 +9,7 @@ namespace cw {
 constexpr int F8_FEW_WAVES = 8;  // waves of a block of the kernel for few rows
 
 // The tile whose estimated time is the least. A CU runs one block of any of them; a round of blocks on every CU takes b + s k / 1024 us, more than
-// one on some of them. Exact products (results in f32) take about twice the time. Measured in a graph (4096 x 4096 in bf16; launch 2.5 us
+// one on some of them. Exact products (results in f32 and f16) take about twice the time. Measured in a graph (4096 x 4096 in bf16; launch 2.5 us
 // included), estimate / measured: 64 x 64 at 128 rows 13.4 / 13.4, 256 rows (every CU) 14.3 / 14.3, 512 rows 26.1 / 29; 128 x 128 at 512 rows 26.9 / 26.9,
 // 1,024 rows 29.4 / 29.4, 2,048 rows 56.3 / 55.8; 256 x 256 at 2,048 rows 58.5 / 59.4, 4,096 rows 71.5 / 71.1. In f32: 64 x 64 at 77 rows of 4001 x
 // 2880 13.1 / 13.2; 128 x 128 at 512 rows of 4096 x 4096 44 / 44.5; 256 x 256 118 / 118.7.

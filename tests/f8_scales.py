@@ -64,13 +64,13 @@ def operands(kind, m, n, k, seed, experts=1, power=62):
 
 def result(kind, xq, sx, wq, sw, k, dtype, bias=None):
     """One matrix's product in 64 bits, and how far a result of the type may be: of each block's terms' magnitudes 2 U for each of 128
-    products, a rounding for each block and 16 that join them, for f16 and bf16 also what the 8-bit instruction leaves out: it cuts 7 of 8
+    products, a rounding for each block and 16 that join them, for bf16 also what the 8-bit instruction leaves out: it cuts 7 of 8
     neighbouring products to multiples of 2^-13 of the largest's power of two, 7 * 2^-13 of the sum at most; nothing for the parts of
     `cancel` that are exact; the rounding to the type."""
     n, kb = wq.shape[0], sw.shape[1]
     want = torch.zeros(xq.shape[0], n, dtype=torch.float64, device=xq.device)
     off = torch.zeros_like(want)
-    rel = (2 * 128 + kb + 16) * U + (0.0 if dtype == torch.float32 else 7 * 2.0 ** -13)
+    rel = (2 * 128 + kb + 16) * U + (7 * 2.0 ** -13 if dtype == torch.bfloat16 else 0.0)
     for b in range(kb):
         at = slice(128 * b, 128 * (b + 1))
         xv, wv = xq[:, at].double(), wq[:, at].double()
