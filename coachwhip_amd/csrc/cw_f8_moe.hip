@@ -328,7 +328,7 @@ static F8MoeLayout layout(const cw_f8_moe_desc *d, int T) {
     const size_t TK = (size_t)T * d->top_k;
     take(L.ids, TK * 4);
     take(L.w, TK * 4);
-    L.few = i8_few_tokens(d->n_experts, d->top_k, d->hidden, d->inter, T);
+    L.few = f8_few_tokens(d->n_experts, d->top_k, d->hidden, d->inter, T);
     if (L.few) {
         take(L.h, TK * ((d->inter + 3) & ~3) * 4);
         L.total = off;

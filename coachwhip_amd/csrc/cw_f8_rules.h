@@ -1,4 +1,4 @@
-// Which kernels the products of the 8-bit float path take, by their sizes and the device's compute units: plain functions of the host.
+// Which kernels the products and layers of the 8-bit float path take, by their sizes and the device's compute units: plain functions of the host.
 #pragma once
 #include <math.h>
 #include <stdint.h>
@@ -62,6 +62,28 @@ inline bool f8_four_groups(int E, int64_t picks, int64_t n, int64_t k, int cus) 
 // Exact sums: 8 of 4,096 x 2,048 (64) 30.7 / 28.1, (128) 59.6 / 53.1, (512) 140 / 116; 64 of 1,408 x 2,048 (64) 62.8 / 71.9, (384) 265 / 253.
 inline bool f8_sorted_tiles(bool exact, int E, int64_t picks, int64_t n, int cus) {
     return picks >= (exact ? 128ll : 64ll) * E && E * ((n + 127) / 128) <= 3 * cus;
+}
+
+// ------------------------------------------------------------------------------ layers
+
+// Whether a layer takes two launches, which read an expert once for each pick, or the sort and the grouped products, six launches, which
+// read it once for its picks. Estimates in us, for their difference: two launches 7 and for each pick the larger of its expert's bytes at 6.5
+// TB/s and 4.5 ns for each of its blocks (16 columns of gate and up; 16 outputs of down, which a token's picks share); grouped 26 and the bytes of
+// E (1 - (1 - K / E)^T) experts, as many as T tokens pick on average, at 7 TB/s. Measured in a graph that goes round over layers of 1.2 GB or 16, bf16, two
+// launches / grouped: 256 experts of 512 x 2,048, top-8, 1 token 12.5 / 36.5, 8 tokens 42 / 57, 20 85 / 93, 24 99 / 113 (which it has grouped), 32
+// 126 / 122, 48 182 / 152; 128 of 2,880 x 2,880, top-4, 4 tokens 88 / 104, 5 111 / 109, 8 161 / 152, 16 312 / 245; 8 of 4,096 x 2,048, top-2, 4 40 / 53, 6 54 / 56, 8 68 / 58;
+// 64 of 1,408 x 2,048, top-6, 6 70 / 76, 8 89 / 83, 12 128 / 89; 16 of 2,880 x 4,096, top-2, 4 66 / 71, 6 95 / 89; 256 of 1,024 x 4,096, top-8, 4 81 / 85, 8 153 / 151;
+// small experts, whose blocks count: 64 of 256 x 1,024, top-8, 24 33 / 36, 32 41 / 36; 16 of 200 x 256, top-4, 48 22 / 24, 64 28 / 24; 64 of 512 x 512, top-1, 64
+// 24 / 27, 256 75 / 29. Results in f32 the same but for wide experts, 10 % more in two launches (128 of 2,880 x 2,880, 5 tokens 122 / 112). Over all sizes
+// measured it loses 0.4 % to the better of both, 15 % at most.
+// The two launches hold a row of x in 32 steps of 128 codes and the K hidden rows in 16 KB of codes: layers beyond that (hidden above 4,096) are
+// grouped for any number of tokens.
+constexpr int F8_FEW_HIDDEN = 4096, F8_FEW_CODES = 16384;
+inline bool f8_few_tokens(int E_, int K_, int H, int I, int T) {
+    const int64_t rbh = (H + 127) / 128 * 128, rbi = (I + 127) / 128 * 128;
+    if (rbh > F8_FEW_HIDDEN || K_ * rbi > F8_FEW_CODES || T > 1024) return false;
+    const double K = K_, E = E_, bytes = 2.0 * I * rbh + (double)H * rbi, blocks = (I + 15) / 16 + (H + 15) / 16 / K;
+    return 7 + T * K * std::max(bytes / 6.5e6, 4.5e-3 * blocks) <= 26 + E * (1 - pow(1 - K / E, T)) * bytes / 7e6;
 }
 
 }  // namespace cw
