@@ -8,7 +8,7 @@ from tests.f8_layer_rules import FEW, GROUPED, down_form, few, few_kernels
 # (tokens, experts, top-k, hidden, inter), measured: two launches / grouped, us
 MEASURED = [((8, 256, 8, 2048, 512), 42, 57), ((20, 256, 8, 2048, 512), 85, 93), ((48, 256, 8, 2048, 512), 182, 152), ((4, 128, 4, 2880, 2880), 88, 104), ((8, 128, 4, 2880, 2880), 161, 152),
             ((4, 8, 2, 2048, 4096), 40, 53), ((8, 8, 2, 2048, 4096), 68, 58), ((6, 64, 6, 2048, 1408), 70, 76), ((8, 64, 6, 2048, 1408), 89, 83), ((4, 16, 2, 4096, 2880), 66, 71), ((6, 16, 2, 4096, 2880), 95, 89),
-            ((24, 64, 8, 1024, 256), 33, 36), ((32, 64, 8, 1024, 256), 41, 36), ((48, 16, 4, 256, 200), 22, 24), ((96, 16, 4, 256, 200), 37, 25), ((300, 16, 4, 256, 200), 102, 28), ((64, 64, 1, 512, 512), 24, 27),
+            ((24, 64, 8, 1024, 256), 33, 36), ((32, 64, 8, 1024, 256), 41, 36), ((48, 16, 4, 256, 200), 22, 24), ((96, 16, 4, 256, 200), 37, 25), ((256, 16, 4, 256, 200), 87, 28), ((64, 64, 1, 512, 512), 24, 27),
             ((256, 64, 1, 512, 512), 75, 29), ((64, 1024, 2, 256, 128), 15, 26), ((512, 1024, 2, 256, 128), 85, 54)]
 
 
