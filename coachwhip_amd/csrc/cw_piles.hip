@@ -288,9 +288,9 @@ __global__ __launch_bounds__(256) void k_from_piles_grad(PileArgs a) {
         const T *x = (const T *)a.x + p / a.K * a.ldx, *y = (const T *)a.y + pos * a.ldy;
         T *out = (T *)a.out + pos * a.h;
         float dot = 0.f;
-        for (int e = 8 * lane; e < a.h; e += 512) {
+        for (uint32_t e = 8 * lane; e < (uint32_t)a.h; e += 512) {  // (a row may have 2^31 - 1 values: the last step passes that)
             float g[8] = {}, v[8];
-            const int valid = a.h - e;
+            const int valid = a.h - (int)e;
             if (in) {
                 load_row<8>(x + e, valid, g);
                 load_row<8>(y + e, valid, v);
