@@ -20,7 +20,7 @@ from . import formats as F
 from . import ops
 from ._lib import CW_EINVAL, CW_F8_MAX_K, CwError, F8MoeDesc, check, lib
 from .i8 import _DTYPES, _SILU, _elsewhere, _fail, _floats, _ptr, _same_device, _stream, _vector, row_bytes
-from .piles import Piles
+from .piles import Piles, _count
 
 _E4M3 = torch.float8_e4m3fn
 
@@ -31,12 +31,13 @@ def blocks(n: int) -> int:
 
 
 def _codes(q, scale, k, lead, what):
+    k = _count(k, "codes of a row")
     if not isinstance(q, torch.Tensor) or not isinstance(scale, torch.Tensor) or not q.is_cuda or q.dtype != _E4M3 or scale.dtype != torch.float32:
         _fail("%s: float8_e4m3fn codes and f32 scales on a device", what)
     if q.device != scale.device or not q.is_contiguous() or not scale.is_contiguous():
         _fail("%s: contiguous codes and scales on one device", what)
     shape = q.shape
-    if len(shape) != lead + 1 or k <= 0 or shape[-1] != row_bytes(k):
+    if len(shape) != lead + 1 or shape[-1] != row_bytes(k):
         _fail("%s codes %s: rows of %d bytes for %d codes", what, tuple(shape), row_bytes(k), k)
     if q.data_ptr() % 16:
         _fail("%s codes must be 16-byte aligned", what)
@@ -205,8 +206,8 @@ class F8ExpertBank:
     @classmethod
     def from_float(cls, w: torch.Tensor):
         """Of (experts, n, k) floats."""
-        if w.dim() != 3:
-            _fail("bank: (experts, n, k) weights, got %s", tuple(w.shape))
+        if not isinstance(w, torch.Tensor) or w.dim() != 3:
+            _fail("bank: (experts, n, k) weights, got %s", tuple(w.shape) if isinstance(w, torch.Tensor) else type(w))
         q, scale = cls._new(*w.shape, w.device)
         for e in range(w.shape[0]):
             _quantize_matrix(w[e], q[e], scale[e])
@@ -261,7 +262,7 @@ class F8MoeLayer:
 
     def __init__(self, gate: F8ExpertBank, up: F8ExpertBank, down: F8ExpertBank, top_k: int, norm_topk_prob: bool = True,
                  act: Optional[ops.ExpertAct] = None):
-        act = act or _SILU
+        act, top_k = act or _SILU, _count(top_k, "top_k")
         e, inter, hidden = gate.q.shape[0], gate.n, gate.k
         for b, n, k, what in ((up, inter, hidden, "up"), (down, hidden, inter, "down")):
             if b.q.shape[0] != e or b.n != n or b.k != k:

@@ -10,6 +10,7 @@ stream of their own device; all arithmetic runs in libcwmoe.so, in a fixed order
 type errors raise ``CwError``.
 """
 import functools
+import operator
 from dataclasses import dataclass
 from typing import Optional
 
@@ -18,6 +19,17 @@ import torch
 from . import ops
 from ._lib import CW_EINVAL, CwError, check, lib
 from .i8 import _DTYPES, _elsewhere, _fail, _floats, _ptr, _same_device, _stream
+
+
+def _count(n, what):
+    """n as an int that the library's calls take as it is."""
+    try:
+        i = operator.index(n)
+    except TypeError:
+        i = 0
+    if not 0 < i < 1 << 31:
+        _fail("%s: %r", what, n)
+    return i
 
 
 @dataclass
@@ -39,6 +51,7 @@ class Piles:
 def sort_picks(ids: torch.Tensor, n_experts: int) -> Piles:
     """ids (T, K) int32, the experts of each token's picks: 0 .. n_experts - 1, or any other number (-1, say) for experts that
     another device holds."""
+    n_experts = _count(n_experts, "experts")
     if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dtype != torch.int32 or ids.dim() != 2 or not ids.is_contiguous():
         _fail("ids: a contiguous (tokens, picks) int32 device tensor")
     t, k = ids.shape
