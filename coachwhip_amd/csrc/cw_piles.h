@@ -21,7 +21,7 @@ inline int64_t pile_max_tiles(int64_t picks, int experts) { return (picks + PILE
 inline int64_t pile_tiles_bytes(int64_t picks, int experts) { return 16 + pile_max_tiles(picks, experts) * (int64_t)sizeof(PileTile); }
 __host__ __device__ __forceinline__ const PileTile *pile_tiles(const void *tiles) { return (const PileTile *)((const uint8_t *)tiles + 16); }
 
-// out (of type dtype) = sum_j w y of f32 rows
+// out (of type dtype) = sum_j w y of f32 rows (w not NULL)
 int from_piles_f32(int dtype, const float *rows, const float *w, int64_t T, int K, int E, int64_t h, const int *place, const int *offsets, void *out,
                    hipStream_t s);
 

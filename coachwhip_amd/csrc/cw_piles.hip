@@ -334,11 +334,14 @@ static int to_piles(const PileArgs &a, hipStream_t s) {
     hipLaunchKernelGGL(k_to_piles<R>, piece_grid(a, (int64_t)a.T * a.K), dim3(256), 0, s, a);
     return check_launch("k_to_piles");
 }
-template <class T, class O>
+template <class T, class O, bool WEIGHTS>
 static int from_piles(const PileArgs &a, hipStream_t s) {
-    if (a.w) hipLaunchKernelGGL((k_from_piles<T, O, true>), piece_grid(a, a.T), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_from_piles<T, O, false>), piece_grid(a, a.T), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_from_piles<T, O, WEIGHTS>), piece_grid(a, a.T), dim3(256), 0, s, a);
     return check_launch("k_from_piles");
+}
+template <class T>
+static int from_piles(const PileArgs &a, hipStream_t s) {
+    return a.w ? from_piles<T, T, true>(a, s) : from_piles<T, T, false>(a, s);
 }
 int from_piles_f32(int dtype, const float *rows, const float *w, int64_t T, int K, int E, int64_t h, const int *place, const int *offsets, void *out,
                    hipStream_t s) {
@@ -347,7 +350,8 @@ int from_piles_f32(int dtype, const float *rows, const float *w, int64_t T, int 
     a.ldy = h;
     a.w = w;
     a.out = out;
-    return dtype == CW_F16 ? from_piles<float, _Float16>(a, s) : dtype == CW_BF16 ? from_piles<float, bf16_t>(a, s) : from_piles<float, float>(a, s);
+    return dtype == CW_F16 ? from_piles<float, _Float16, true>(a, s) : dtype == CW_BF16 ? from_piles<float, bf16_t, true>(a, s)
+                                                                                      : from_piles<float, float, true>(a, s);
 }
 template <class T>
 static int from_piles_grad(const PileArgs &a, hipStream_t s) {
@@ -449,7 +453,7 @@ int cw_from_piles(int dtype, const void *rows, int64_t ldr, const float *w, int6
     a.w = w;
     a.out = out;
     hipStream_t s = (hipStream_t)stream;
-    return dtype == CW_F16 ? from_piles<_Float16, _Float16>(a, s) : dtype == CW_BF16 ? from_piles<bf16_t, bf16_t>(a, s) : from_piles<float, float>(a, s);
+    return dtype == CW_F16 ? from_piles<_Float16>(a, s) : dtype == CW_BF16 ? from_piles<bf16_t>(a, s) : from_piles<float>(a, s);
 }
 
 int cw_from_piles_grad(int dtype, const void *dout, int64_t ldd, const void *rows, int64_t ldr, const float *w, int64_t T, int K, int n_experts,
