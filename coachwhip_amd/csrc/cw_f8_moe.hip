@@ -26,7 +26,7 @@ struct F8FewArgs {
 // instruction: its sums cost nothing here, unpacking the codes for the vector unit 1.3 times the bytes' time), the steps of 128
 // codes dealt to eight waves, even ones gate, odd ones up, their sums joined in LDS in the waves' order. One wave routes the token for its block, no
 // further than this pick; the last pick's first block, which goes all the way, stores the routing. One token of 8 picks of 512 x 2,048: 7.1 us for 16.8 MB, a
-// chain of logits, routing, weights, sums; 4 tokens of 4 picks of 2,880 x 2,880, with down: 96 us, 4.1 TB/s.
+// chain of logits, routing, weights, sums; 4 tokens of 4 picks of 2,880 x 2,880, with down: 88 to 96 us, 4.1 to 4.6 TB/s.
 template <int PER, int NS, bool EXACT>
 __global__ __launch_bounds__(64 * F8_FEW_WAVES, NS > 4 ? 2 : 4) void k_f8_few_gateup(F8FewArgs a) {
     __shared__ uint32_t expert;
@@ -235,7 +235,7 @@ struct F8GateUpArgs {
 // Gate and up of a tile of up to 128 positions, 128 columns of both, and their activation as codes: a block holds whole groups of 128 columns of
 // its rows, so that the hidden rows leave it as codes and nothing else is written (f32 hidden rows of 2,048 tokens of 4 picks of 2,880 columns: 94 MB
 // written and read again). A wave has 32 columns: the largest magnitude of a row's 128 meets in LDS, as do the codes, which leave as whole rows of 128.
-// 2,048 tokens of 4 picks over 128 experts of 2,880 x 2,880: 470 to 490 us, 4.4 TB/s of weights; the waves wait for loads 35 % of their cycles and to issue 46 %.
+// 2,048 tokens of 4 picks over 128 experts of 2,880 x 2,880: 470 to 496 us, 4.3 to 4.5 TB/s of weights (exact products 617); the waves wait for loads 35 % of their cycles and to issue 46 %.
 template <bool EXACT>
 __global__ __launch_bounds__(256, 2) void k_f8_gateup(F8GateUpArgs a, int n_blocks) {
     extern __shared__ __align__(1024) uint8_t lds[];

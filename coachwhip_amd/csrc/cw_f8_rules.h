@@ -47,8 +47,8 @@ inline int f8_few_groups(bool exact, int64_t m, int64_t n, int cus) {
 
 // Four groups of weight rows a wave instead of two (whose steps are twice as wide and whose sums leave more registers): where both the weights' bytes
 // and the products count, and there is a block for every CU twice. A long k ends that
-// at 64 picks. Measured in a graph, two / four groups, bf16: 128 experts of 2,880 x 2,880, 2 picks each 178 / 190 us, 32 230 / 218, 64 259 / 246, 94
-// 291 / 316, 128 360 / 358 to 389; 256 of 512 x 2,048 (16) 47.1 / 45.6, (64) 66.8 / 56.9; 256 of 1,024 x 2,048 (64) 136 / 125; 256 of 2,048 x 512
+// at 64 picks. Measured in a graph, two / four groups, bf16: 128 experts of 2,880 x 2,880, 2 picks each 178 / 190 us, 32 230 / 218, 64 259 / 246, 68 263 / 250, 72 265 / 260, 80
+// 274 / 280, 94 291 / 316, 128 360 / 358 to 389 (a k of 2,560: 80 249 / 256; 2,304: 64 212 / 201, 80 225 / 222, 100 244 / 251: the line at 64 gives away 5 % up to 75); 256 of 512 x 2,048 (16) 47.1 / 45.6, (64) 66.8 / 56.9; 256 of 1,024 x 2,048 (64) 136 / 125; 256 of 2,048 x 512
 // (16) 65.0 / 52.3, (128) 131 / 120, (192) 177 / 156, of 512 x 2,048 (256) 179 / 171. Exact sums: 128 of 2,880 x 2,880 (64) 326 / 319, (128)
 // 543 / 622. With fewer blocks: 64 of 1,408 x 2,048 (192) 100 / 132; 8 of 4,096 x 2,048 (512) 90 / 123.
 inline bool f8_four_groups(int E, int64_t picks, int64_t n, int64_t k, int cus) {

@@ -16,7 +16,7 @@ typedef int i32x8v __attribute__((ext_vector_type(8)));
 //
 // v_mfma_f32_16x16x128_f8f6f4 takes the codes as they are. Of the products of 8 neighbouring codes it keeps what is at least 2^(e - 13), e the
 // largest sum of two codes' exponents among them, and cuts the rest off towards zero (measured on this part: beside 2^16 a product of 2^3 is kept,
-// 2^2 lost, 27.5 becomes 24; so does the 16 x 16 x 32 form); those sums it adds in f32. So 7 of 8 products lose up to 2^-13 of the largest:
+// 2^2 lost, 27.5 becomes 24, whichever of the 8 it is); those sums it adds in f32. So 7 of 8 products lose up to 2^-13 of the largest:
 // 7 * 2^-13 of the terms' magnitudes at most, below a quarter of bf16's half step (f16's it may pass); 1.5e-5 of a result of random codes. EXACT: as
 // f16, which holds every e4m3 value, at half the rate: each product exact and added in f32 (of 128 widely
 // spread products 3e-7 of their magnitudes at the most seen, of random ones 1e-8 of the result), for results in f32 and f16 and for hidden values whose codes hang on them.

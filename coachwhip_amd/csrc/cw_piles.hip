@@ -243,7 +243,8 @@ __global__ __launch_bounds__(256) void k_to_piles(PileArgs a) {
 }
 
 // out[t] = sum_j w[t][j] y[place[t][j]] (w NULL: 1), in pick order, in f32, rounded once; picks of no expert add nothing, whatever
-// their rows hold (8,192 tokens of 8 picks, half of no expert, 2,048 bf16 values: 54 us, 31 with the rows in the caches)
+// their rows hold (8,192 tokens of 8 picks, half of no expert, 2,048 bf16 values: 54 us, 3.1 TB/s, 87 % of the waves'
+// cycles waits for the places and then the rows; 31 with the rows in the caches)
 template <class T, class O, bool WEIGHTS>
 __global__ __launch_bounds__(256) void k_from_piles(PileArgs a) {
     const int here = a.offsets[a.E];
@@ -276,8 +277,8 @@ __global__ __launch_bounds__(256) void k_from_piles(PileArgs a) {
 }
 
 // A wave a pick: dy = w x[t] (x: the gradient of the tokens' output) into its position, dw = <x[t], y>. The picks of a token are a
-// block's neighbours: its row comes from the caches after the first (4,095 tokens of 4 picks, 2,880 bf16 values: 35 us, 6.0 TB/s; a wave a
-// position, whose long rows are then read and written in order: 44; 8,192 of 8, half of no expert, 91 and 88).
+// block's neighbours: its row comes from the caches after the first (4,095 tokens of 4 picks, 2,880 bf16 values: 42 us over sets of inputs in turn, 5.0 TB/s. In a graph on
+// one set, which the caches hold in part: 35; a wave a position, whose long rows are then read and written in order: 44; 8,192 of 8, half of no expert, 91 and 88).
 template <class T>
 __global__ __launch_bounds__(256) void k_from_piles_grad(PileArgs a) {
     const int here = a.offsets[a.E], lane = threadIdx.x & 63;
