@@ -16,7 +16,7 @@ def say(*a):
 
 
 def types_of(exact):
-    return [torch.float32] if exact else [torch.float16, torch.bfloat16]
+    return [torch.float32, torch.float16] if exact else [torch.bfloat16]
 
 
 def on_device(*a):
